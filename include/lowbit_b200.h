@@ -55,6 +55,7 @@ extern "C" {
 #define LBC_ERR_CUDA (-5)   /* a CUDA call or launch failed (see lbc_last_error) */
 #define LBC_ERR_DEVICE (-6) /* current device is not sm_100 */
 #define LBC_ERR_TIMEOUT (-7) /* a bounded device-side wait gave up */
+#define LBC_ERR_PAGE (-8) /* device status only: a page id, position or row offset out of range */
 
 /*
  * Tuning parameters.  Same memory layout as the reference's lb_params
@@ -325,6 +326,86 @@ int lbc_rope_attention(const float *qkv, const float *bias, const float *cos_t, 
 int lbc_silu_mul(const float *gu, float *out, int T, int I, void *stream);
 /* *pos += n on the device, in stream order (end of a captured decode step). */
 int lbc_advance_pos(int32_t *pos, int n, void *stream);
+
+/* ---- paged 8-bit KV cache: no reference counterpart (its cache is one fp32
+ * array per layer, src/lowbit/model.py:216-230). One layer's pool of pages:
+ *
+ *   k, v         : int8 codes [pages][kv_heads][page][head_dim]; page i at
+ *                  + i * page_stride bytes (a multiple of 16, at least
+ *                  kv_heads * page * head_dim), the rest contiguous, both
+ *                  16-byte aligned;
+ *   k_exp, v_exp : one E8M0 byte e per page and head, page i at
+ *                  + i * exp_stride: a code stands for code * 2^(e - 127);
+ *                  e = 255: the whole block is NaN.
+ *
+ * page (tokens per page) is 16, 32, 64 or 128, head_dim 32, 64 or 128. A
+ * block is the `page` tokens of one page and head. The exponent is the
+ * smallest e >= 0 with max|x| <= 127 * 2^(e - 127); codes are
+ * rne(x * 2^(127 - e)), at most 127 in magnitude (63 at e = 249, where 64
+ * would stand for 2^128). Values are exact in bf16.
+ *
+ * Both operators below take the new tokens of B sequences as N rows:
+ * sequence b owns rows starts[b] .. starts[b+1]-1 (starts: DEVICE int32
+ * [B + 1], starts[0] = 0, starts[B] = N; NULL: N / B rows each), at most
+ * max_tokens of them; its t-th row sits at position pos[b] + t (pos: DEVICE
+ * int32 [B], the tokens already held). Position p lives in slot p % page of
+ * page table[b * table_width + p / page] (table: DEVICE int32). Rows at
+ * negative positions are padding: nothing is stored, their outputs are 0.
+ * Page ids outside the pool, positions outside the table and sequences with
+ * more than max_tokens rows are skipped and recorded as LBC_ERR_PAGE in
+ * lbc_device_status. Pages may be shared between sequences for reading;
+ * appending to one page from two sequences in one call is a race.
+ * Everything is read on the device: CUDA graphs of these calls replay with
+ * new positions, tables and row counts. All return 0 or a negative LBC_ERR_*. */
+#define LBC_F32 0
+#define LBC_BF16 1
+#define LBC_F16 2
+typedef struct {
+    int8_t *k;
+    int8_t *v;
+    uint8_t *k_exp;
+    uint8_t *v_exp;
+    long long page_stride;
+    long long exp_stride;
+    int pages;
+    int page;
+    int kv_heads;
+    int head_dim;
+} lbc_kv8;
+
+/* Fused q/k/v rows [N, (H + 2*KV)*D] of type dtype, ld elements apart (plus
+ * bias, fp32, when non-NULL): rotate-half RoPE on the q and k heads at each
+ * row's position (cos/sin fp32 tables [positions, D/2]; positions past them
+ * are skipped and recorded), q to q_out [N, H, D] in dtype, k and v quantised
+ * into the cache. A block's exponent is at least its old one unless slot 0 is
+ * among the new rows; where it grows, the block's older codes become
+ * rne(code * 2^(e_old - e_new)). Non-finite k or v: the block reads as NaN.
+ * qkv and ld * element size must be 16-byte aligned. */
+int lbc_kv8_append(const lbc_kv8 *c, int dtype, const void *qkv, long long ld, const float *bias,
+                   const float *cos_t, const float *sin_t, int positions, const int32_t *table,
+                   int table_width, const int32_t *pos, const int32_t *starts, int B, int N,
+                   int max_tokens, int H, void *q_out, void *stream);
+
+/* Causal grouped-query attention over the cache (the new tokens' k and v
+ * already appended): row (i, h) at position p attends to positions
+ * max(0, p - window + 1) .. p (window <= 0: 0 .. p) of KV head h / (H / KV),
+ * softmax of scale * q.k; q [N, H, D] of type dtype, rows ld elements apart
+ * (16-byte aligned rows), out [N, H, D] in dtype; a row without keys is 0.
+ * Softmax and sums in fp32. workspace: device scratch of
+ * lbc_kv8_attention_workspace(...) bytes (0: may be NULL), 256-byte aligned,
+ * used by this call only; its contents need no initialisation. */
+size_t lbc_kv8_attention_workspace(const lbc_kv8 *c, int dtype, int table_width, int B, int N,
+                                   int max_tokens, int H, int window);
+int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, const int32_t *table,
+                      int table_width, const int32_t *pos, const int32_t *starts, int B, int N,
+                      int max_tokens, int H, int window, float scale, void *out, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/* Pages back as values: k_out, v_out [n, kv_heads, page, head_dim] of type
+ * dtype for the n page ids in `ids` (DEVICE int32); an id outside the pool
+ * gives zeros and LBC_ERR_PAGE in lbc_device_status. Exact in bf16 and fp32. */
+int lbc_kv8_read(const lbc_kv8 *c, int dtype, const int32_t *ids, int n, void *k_out, void *v_out,
+                 void *stream);
 
 #ifdef __cplusplus
 }

@@ -605,6 +605,14 @@ int run_tc(lbc::TcCall c, cudaStream_t st) {
 
 }  // namespace
 
+int lbc::device_ready(int **status, int *sms) {
+  if (int rc = device_gate()) return rc;
+  const DevInfo di = dev_info();
+  *status = di.status;
+  *sms = di.sms;
+  return 0;
+}
+
 void lbc::set_last_error(const char *msg) { snprintf(g_err, sizeof g_err, "%s", msg); }
 
 // ====================================================================== C ABI

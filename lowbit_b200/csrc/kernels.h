@@ -60,6 +60,10 @@ size_t tc_scratch_bytes(int fmt, int M, int Kp, int ctas);
 // returns LBC_PATH_TCGEN05 or a negative LBC_ERR_* with a message in err
 int tc_gemm(const TcCall &c, cudaStream_t st, char *err, size_t errlen);
 
+// 0 when the current device is sm_100 (with its status block and SM count), else a
+// negative LBC_ERR_* with the text recorded
+int device_ready(int **status, int *sms);
+
 // records `msg` as the text lbc_last_error() returns on this thread
 void set_last_error(const char *msg);
 

@@ -38,7 +38,8 @@ PATH_IDS = {"auto": -1, "simt": 0, "tcgen05": 1, "mma": 3}
 REFERENCE_ISAS = ("scalar", "avx2", "avx512")
 KIND_IDS = {"w4a16": 0, "mxfp4": 1, "w4a8": 2}
 ERR_NAMES = {-1: "bad shape or pointer", -2: "tile parameters not supported", -3: "allocation failed",
-             -5: "CUDA error", -6: "device is not sm_100", -7: "device-side wait timed out"}
+             -5: "CUDA error", -6: "device is not sm_100", -7: "device-side wait timed out",
+             -8: "page id, position or row offset out of range"}
 
 
 class _Params(C.Structure):
@@ -122,6 +123,12 @@ def lib() -> C.CDLL:
         "lbc_gemm_w4a16_glu": ([_vp, _int, _int, _vp, _vp, _vp, _int, _vp, _pp, _vp], _int),
         "lbc_rope_attention": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _int, _vp], _int),
         "lbc_advance_pos": ([_vp, _int, _vp], _int),
+        "lbc_kv8_append": ([_vp, _int, _vp, C.c_longlong, _vp, _vp, _vp, _int, _vp, _int, _vp, _vp, _int, _int, _int,
+                            _int, _vp, _vp], _int),
+        "lbc_kv8_attention_workspace": ([_vp, _int, _int, _int, _int, _int, _int, _int], C.c_size_t),
+        "lbc_kv8_attention": ([_vp, _int, _vp, C.c_longlong, _vp, _int, _vp, _vp, _int, _int, _int, _int, _int,
+                               C.c_float, _vp, _vp, C.c_size_t, _vp], _int),
+        "lbc_kv8_read": ([_vp, _int, _vp, _int, _vp, _vp, _vp], _int),
         "lbc_quantize_int4": ([_vp, _int, _int, _int, _vp, _vp, _vp, _vp], _int),
         "lbc_quantize_mxfp4": ([_vp, _int, _int, _vp, _vp, _vp], _int),
     }

@@ -1,0 +1,87 @@
+"""Paged 8-bit KV cache without a GPU: what the C entry points refuse, and the
+oracle's own properties."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+from lowbit_b200 import kernels as K
+from lowbit_b200.kvcache import _KV8
+from oracle import kv8_ref as R
+
+A = 1 << 20  # an aligned address; refused calls touch no memory
+
+
+def pool(**over):
+    f = dict(k=A, v=A, k_exp=A, v_exp=A, page_stride=2 * 64 * 64, exp_stride=2, pages=4, page=64, kv_heads=2, head_dim=64)
+    f.update(over)
+    return C.byref(_KV8(*(f[n] for n, _ in _KV8._fields_)))
+
+
+@pytest.mark.parametrize("over", [
+    dict(k=None), dict(v_exp=None), dict(page=48), dict(page=0), dict(head_dim=96), dict(pages=0), dict(kv_heads=0),
+    dict(page_stride=2 * 64 * 64 - 16), dict(page_stride=2 * 64 * 64 + 8), dict(exp_stride=1), dict(k=A + 8)])
+def test_c_entries_refuse_bad_pools(over):
+    L = K.lib()
+    for rc in (L.lbc_kv8_read(pool(**over), 1, A, 1, A, A, None),
+               L.lbc_kv8_attention(pool(**over), 0, A, 256, A, 4, A, None, 1, 1, 1, 4, 0, 0.125, A, None, 0, None),
+               L.lbc_kv8_append(pool(**over), 0, A, 512, None, A, A, 64, A, 4, A, None, 1, 1, 1, 4, A, None)):
+        assert rc == -1
+        assert b"kv8" in L.lbc_last_error()
+
+
+def test_c_entries_refuse_null_pools():
+    L = K.lib()
+    assert L.lbc_kv8_read(None, 1, A, 1, A, A, None) == -1
+    assert L.lbc_kv8_attention_workspace(None, 0, 4, 1, 1, 1, 4, 0) == 0
+
+
+def test_python_refuses_host_tensors():
+    import torch
+
+    import lowbit_b200 as lb
+    k = torch.zeros((4, 2, 64, 64), dtype=torch.int8)
+    e = torch.zeros((4, 2), dtype=torch.uint8)
+    with pytest.raises(ValueError, match="CUDA"):
+        lb.KV8Cache(k, k.clone(), e, e.clone())
+    with pytest.raises(ValueError, match="int8"):
+        lb.KV8Cache(k.float(), k.float(), e, e)
+    with pytest.raises(ValueError, match="uint8"):
+        lb.KV8Cache(k, k, e.int(), e)
+
+
+def test_every_kv8_name_is_exported():
+    import lowbit_b200 as lb
+    for n in ("KV8Cache", "kv8_append", "kv8_attention", "kv8_read"):
+        assert n in lb.__all__ and callable(getattr(lb, n))
+    with pytest.raises(AttributeError):
+        lb.kv8_nothing
+
+
+def test_scale_byte_of_the_oracle():
+    assert R.scale_byte(0.0) == 0 and R.scale_byte(127.0) == 127 and R.scale_byte(np.nextafter(127.0, 200)) == 128
+    assert R.scale_byte(float(np.finfo(np.float32).max)) == 249 and R.scale_byte(math.inf) == 255
+    assert R.scale_byte(1e-45) == 0 and R.scale_byte(63.5) == 126
+
+
+@pytest.mark.parametrize("cut", [1, 7, 16, 30])
+def test_oracle_append_in_pieces_grows_only_the_step(cut):
+    """Pieces give the same exponents as one call, and codes at most one step apart
+    (older codes are rounded once more when their block's step grows)."""
+    rng = np.random.default_rng(cut)
+    x = rng.standard_normal((40, (2 + 2) * 32)).astype(np.float32) * np.exp(rng.standard_normal((40, 1))).astype(np.float32)
+    ang = np.arange(64)[:, None] * 0.1 ** np.arange(16)
+    cos, sin = np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
+    table = np.array([[2, 0, 1]])
+
+    def empty():
+        return {n: np.zeros((3, 1, 16, 32) if len(n) == 1 else (3, 1), np.int8 if len(n) == 1 else np.uint8)
+                for n in ("k", "v", "k_exp", "v_exp")}
+    one, two = empty(), empty()
+    q = R.append(one, x, table, [0], cos, sin, 2)
+    q2 = np.concatenate([R.append(two, x[:cut], table, [0], cos, sin, 2), R.append(two, x[cut:], table, [cut], cos, sin, 2)])
+    np.testing.assert_array_equal(q, q2)
+    for n in ("k", "v"):
+        np.testing.assert_array_equal(one[n + "_exp"], two[n + "_exp"])
+        assert np.abs(one[n].astype(int) - two[n]).max() <= 1

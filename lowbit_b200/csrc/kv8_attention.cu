@@ -1,15 +1,48 @@
 // Causal grouped-query attention over the paged 8-bit KV cache
-// (include/lowbit_b200.h: lbc_kv8_attention).
+// (include/lowbit_b200.h: lbc_kv8_attention): softmax(scale q.k) v with a
+// running maximum, one pass over the codes.
+//
+// Scores and outputs are computed transposed on mma.sync m16n8k16: 16 tokens
+// (scores) or 16 elements (outputs) by 8 query rows, so that few rows (one
+// token's G = H / KV heads) fill the tile. int8 codes are exact in fp16;
+// queries are scaled by a power of two per row into fp16's range (fp32 ones as
+// two pieces, 22 bits), weights likewise (fp32: two pieces; 16-bit types: one).
+// Contraction indices may be permuted freely, and are: a lane loads 16
+// contiguous bytes of its token's key (or of four tokens' values) straight
+// from global memory into the operand registers, no shared memory between.
+//
+// With z_j = log2(e) scale q.k_j the weights carry their block's value scale
+// 2^b_j: t_j = z_j + b_j, M about max t_j - 14 the running reference,
+//   O = sum_j 2^(t_j - M) code_j,  l = sum_j 2^(t_j - M) 2^(f - b_j),
+//   out = 2^f O / l,  f = max b_j,
+// so weights stay within fp16 whatever the scales, and all rescaling is by
+// powers of two (M is a whole number).
+//
+// Work: an item is (sequence, tile of 8 NQ rows, KV head); its visible tokens
+// are cut into units of 128 (32 a warp). The units of all items form one line
+// that is cut evenly over the grid, wherever lengths differ: a CTA runs
+// through the ends of items and whole ones; cut items leave partial
+// (O, M, l, f) records that a second kernel joins in order (no atomics).
+#include <algorithm>
 #include <cstdio>
 
 #include "kernels.h"
 #include "kv8.cuh"
+#include "kv8_mma.cuh"
 
 namespace lbc {
 namespace kv8 {
 namespace {
 
-constexpr int WARPS = 8;
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int WTOK = 32;            // tokens of a warp in a unit: two 16-token tiles
+constexpr int UNIT = WARPS * WTOK;  // 128 tokens: page sizes divide it
+constexpr int META = 128;           // pages looked up at a time
+constexpr float LOWEST = -3e38f;    // M before any visible token
+// weights 2^(t - M) fill fp16's range: M is the maximum (rounded up) less 14,
+// left alone while no weight passes 2^15. Two pieces then hold a weight to 22
+// bits down to 2^-17 of the largest, one piece to 11 bits down to 2^-28.
+constexpr float HEAD = 14.f, SLACK = 15.f;
 
 struct AttnArgs {
   Pool c;
@@ -17,78 +50,553 @@ struct AttnArgs {
   const void *q;
   long long ld;
   void *out;
-  int H, window;
+  int H, G, window;
   float scale_log2;  // scale * log2(e)
+  int tiles;         // row tiles a sequence can have
+  int split;         // 0: one CTA an item, no partials
+  int2 *desc;        // [B][tiles][KV] first and last CTA of an item
+  float *part;       // [grid][2] records: O [8 NQ][D], then M, l, f [8 NQ] each
 };
 
-// One CTA per row and head; warp w takes keys first + w, first + w + 8, ...
-// with a running maximum and sum, lane l the elements l, l + 32, ...
-template <typename T, int D>
-__global__ void __launch_bounds__(WARPS * 32) attention_kernel(AttnArgs a) {
-  constexpr int E = D / 32;
-  __shared__ float sm[WARPS], sl[WARPS], so[WARPS][D];
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int r0, n;
-  const int b = row_seq(a.r, row);
-  seq_rows(a.r, b, r0, n);
-  if (row < r0 || row >= r0 + n) return;
-  int p = a.r.pos[b] + row - r0;
-  if (p >= a.r.width << a.c.lg_page) {  // past the table: no keys
+// the units and row tiles of sequence b
+struct Seq {
+  int r0, n, p0, u0, units, tiles;
+};
+template <int NQ>
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
+  Seq s;
+  seq_rows(a.r, b, s.r0, s.n);
+  s.p0 = a.r.pos[b];
+  const long long cap = (long long)a.r.width << a.c.lg_page;
+  long long last = (long long)s.p0 + s.n - 1;
+  if (s.n > 0 && last >= cap) {  // rows past the table see nothing
     set_status(a.r.status, LBC_ERR_PAGE);
-    p = -1;
+    last = cap - 1;
   }
-  const int kvh = h / (a.H / a.c.KV);
-  const int first = a.window > 0 ? max(0, p - a.window + 1) : 0;
-  const T *q = static_cast<const T *>(a.q) + row * a.ld + (size_t)h * D;
-  float qv[E], acc[E], m = -INFINITY, l = 0.f;
+  int first = 0;
+  if (a.window > 0) first = max(0, max(s.p0, 0) - a.window + 1);
+  s.u0 = first / UNIT;
+  s.units = s.n > 0 && last >= first ? (int)last / UNIT - s.u0 + 1 : 0;
+  s.tiles = (s.n * a.G + 8 * NQ - 1) / (8 * NQ);
+  return s;
+}
+
+// position of row `rho` (token rho / G) of a sequence, -1 for rows that see
+// nothing; the rows that fill up the last tile (never stored) copy the last one
+__device__ __forceinline__ int row_pos(const AttnArgs &a, const Seq &s, int rho) {
+  const long long p = (long long)s.p0 + min(rho, s.n * a.G - 1) / a.G;
+  return p >= ((long long)a.r.width << a.c.lg_page) ? -1 : (int)p;
+}
+
+struct Meta {
+  int id[META];  // -1: no such page
+  uint8_t ek[META], ev[META];
+  int f;  // largest value exponent so far (255 left out)
+};
+
+template <typename T, int D, int NQ>
+struct Warp {
+  static constexpr int PIECES = sizeof(T) == 4 ? 2 : 1;
+  static constexpr int KW = D / 16, VW = D / 32, MT = D / 16;
+  uint32_t q[NQ][PIECES][KW][2];  // query operand
+  float rowf[NQ][2];              // score = accumulator * rowf * 2^(ek - 127), in log2 units
+  int p[NQ][2];                   // positions of the lane's rows 8 n + 2 t + i
+  float m[NQ][2], l[NQ][2], o[NQ][MT][4];
+  uint32_t k[2][2][KW], v[2][4][VW];
+
+  // first element of the four that lane t's word s of a key row holds
+  __device__ static int key_dim(int t, int s) { return D == 32 ? 8 * t + 4 * s : 64 * (s / 4) + 16 * t + 4 * (s % 4); }
+
+  __device__ __forceinline__ void start(const AttnArgs &a, const Seq &s, int tile, int kvh, int lane) {
+    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qv[e] = to_f<T>(q[lane + 32 * e]);
-    acc[e] = 0.f;
-  }
-  for (int j = first + warp; j <= p; j += WARPS) {
-    const int id = page_id(a.c, a.r, b, j >> a.c.lg_page);
-    if (id < 0) continue;
-    const size_t at = id * a.c.page_stride + ((size_t)kvh * a.c.page + (j & (a.c.page - 1))) * D;
-    const float ks = pow2_e8m0(a.c.k_exp[id * a.c.exp_stride + kvh]);
-    const float vs = pow2_e8m0(a.c.v_exp[id * a.c.exp_stride + kvh]);
-    float s = 0.f;
+    for (int n = 0; n < NQ; ++n) {
+      const int rho = (tile * NQ + n) * 8 + g;
+      const bool live = rho < s.n * a.G;
+      const T *src = static_cast<const T *>(a.q) + (s.r0 + rho / a.G) * a.ld + (size_t)(kvh * a.G + rho % a.G) * D;
+      float x[KW][4], amax = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(qv[e], (float)a.c.k[at + lane + 32 * e], s);
+      for (int w = 0; w < KW; ++w) {
+        if (live) {
+          load4<T>(src + key_dim(t, w), x[w]);
+        } else {
+          x[w][0] = x[w][1] = x[w][2] = x[w][3] = 0.f;
+        }
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s = s * ks * a.scale_log2;
-    const float mn = fmaxf(m, s), f = exp2f(m - mn), w = exp2f(s - mn);
-    l = fmaf(l, f, w);
+        for (int i = 0; i < 4; ++i) amax = x[w][i] == x[w][i] ? fmaxf(amax, fabsf(x[w][i])) : INFINITY;
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const float f = fp16_range(amax);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(acc[e], f, w * vs * (float)a.c.v[at + lane + 32 * e]);
-    m = mn;
-  }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
+      for (int w = 0; w < KW; ++w)
 #pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][lane + 32 * e] = acc[e];
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += WARPS * 32) {
-    float mx = -INFINITY, den = 0.f, num = 0.f;
-    for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, sm[w]);
-    for (int w = 0; w < WARPS; ++w) {
-      const float f = sm[w] == -INFINITY ? (sl[w] == 0.f ? 0.f : sl[w]) : exp2f(sm[w] - mx);  // a warp without keys adds nothing
-      den = fmaf(sl[w], f, den);
-      num = fmaf(so[w][d], f, num);
+        for (int h = 0; h < 2; ++h) {
+          const float x0 = x[w][2 * h] * f, x1 = x[w][2 * h + 1] * f;
+          q[n][0][w][h] = pack_half(x0, x1);
+          if constexpr (PIECES == 2) q[n][1][w][h] = pack_rest(x0, x1, q[n][0][w][h]);
+        }
+      const float back = a.scale_log2 / f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        rowf[n][i] = __shfl_sync(0xffffffffu, back, (2 * t + i) * 4);
+        p[n][i] = row_pos(a, s, (tile * NQ + n) * 8 + 2 * t + i);
+        m[n][i] = LOWEST;
+        l[n][i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
-    static_cast<T *>(a.out)[((size_t)row * a.H + h) * D + d] = from_f<T>(den == 0.f ? 0.f : num / den);
+  }
+
+  // codes of the 16-token tile at position j, whose page is entry `e`
+  __device__ __forceinline__ void load_k(const AttnArgs &a, const Meta &x, int h, int e, int j, int kvh, int lane) {
+    const int g = lane >> 2, t = lane & 3, id = max(x.id[e], 0);
+    const int8_t *src = a.c.k + id * a.c.page_stride + ((size_t)kvh * a.c.page + (j & (a.c.page - 1))) * D;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int8_t *row = src + (g + 8 * r) * D;
+      if constexpr (D == 32) {
+        load_words<8>(row + 8 * t, k[h][r]);
+      } else {
+#pragma unroll
+        for (int w = 0; w < KW; w += 4) load_words<16>(row + 16 * w + 16 * t, k[h][r] + w);
+      }
+    }
+  }
+  __device__ __forceinline__ void load_v(const AttnArgs &a, const Meta &x, int h, int e, int j, int kvh, int lane) {
+    const int g = lane >> 2, t = lane & 3, id = max(x.id[e], 0);
+    const int8_t *src = a.c.v + id * a.c.page_stride + ((size_t)kvh * a.c.page + (j & (a.c.page - 1))) * D + g * (D / 8);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) load_words<D / 8>(src + (2 * t + (r & 1) + 8 * (r >> 1)) * D, v[h][r]);
+  }
+
+  __device__ __forceinline__ void scores(float (&z)[2][NQ][4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) z[h][n][0] = z[h][n][1] = z[h][n][2] = z[h][n][3] = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const uint32_t x0 = k[h][0][w] ^ 0x80808080u, x1 = k[h][1][w] ^ 0x80808080u;
+        const uint32_t op[4] = {half_lo(x0), half_lo(x1), half_hi(x0), half_hi(x1)};
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int c = 0; c < PIECES; ++c) mma16816(z[h][n], op, q[n][c][w][0], q[n][c][w][1]);
+      }
+    }
+  }
+
+  // z: scores to weights (in place); j: position of the warp's first token; e: its pages
+  __device__ __forceinline__ void weights(const AttnArgs &a, const Meta &x, float (&z)[2][NQ][4], const int (&e)[2], int j,
+                                          int lane, int p_min, int p_max) {
+    const int g = lane >> 2;
+    float back[2];
+    bool rise = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j0 = j + 16 * h, ev = x.ev[e[h]];
+      const float ks = pow2_e8m0(x.ek[e[h]]);
+      // a block far below f would take its weights out of range: it counts in l only
+      const float b = ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(max(ev, x.f - 60) - 127);
+      back[h] = ev == 255 ? 1.f : pow2_e8m0(127 + x.f - max(ev, x.f - 60));
+      const bool whole = j0 + 15 <= p_min && (a.window <= 0 || j0 > p_max - a.window) && x.id[e[h]] >= 0;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float t = fmaf(z[h][n][i], rowf[n][i & 1] * ks, b);
+          if (!whole) {
+            const int at = j0 + g + 8 * (i >> 1), pr = p[n][i & 1];
+            const bool seen = at <= pr && (a.window <= 0 || at > pr - a.window) && x.id[e[h]] >= 0;
+            t = seen ? t : -INFINITY;
+          }
+          z[h][n][i] = t;
+          rise |= t > m[n][i & 1] + SLACK;
+        }
+    }
+    if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float mx = fmaxf(fmaxf(z[0][n][i], z[0][n][i + 2]), fmaxf(z[1][n][i], z[1][n][i + 2]));
+#pragma unroll
+          for (int d = 4; d <= 16; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const float to = fmaxf(m[n][i], ceilf(mx) - HEAD), f = ex2(m[n][i] - to);
+          m[n][i] = to;
+          l[n][i] *= f;
+#pragma unroll
+          for (int c = 0; c < MT; ++c) {
+            o[n][c][i] *= f;
+            o[n][c][i + 2] *= f;
+          }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool far = x.ev[e[h]] != 255 && x.ev[e[h]] < x.f - 60;
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = ex2(z[h][n][i] - m[n][i & 1]);
+          l[n][i & 1] = fmaf(w, back[h], l[n][i & 1]);
+          z[h][n][i] = far ? 0.f : w;
+        }
+    }
+  }
+
+  __device__ __forceinline__ void outputs(const float (&z)[2][NQ][4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t b[NQ][PIECES][2];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t hi = pack_half(z[h][n][2 * i], z[h][n][2 * i + 1]);
+          b[n][0][i] = transpose8(hi);
+          if constexpr (PIECES == 2) b[n][1][i] = transpose8(pack_rest(z[h][n][2 * i], z[h][n][2 * i + 1], hi));
+        }
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        // four tokens' words -> for each element the pairs (token 2t, 2t + 1) and (2t + 8, 2t + 9)
+        const uint32_t x0 = v[h][0][w] ^ 0x80808080u, x1 = v[h][1][w] ^ 0x80808080u;
+        const uint32_t x2 = v[h][2][w] ^ 0x80808080u, x3 = v[h][3][w] ^ 0x80808080u;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t y0 = prmt(x0, x1, c ? 0x7362 : 0x5140), y1 = prmt(x2, x3, c ? 0x7362 : 0x5140);
+          const uint32_t op[4] = {half_lo(y0), half_hi(y0), half_lo(y1), half_hi(y1)};
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int r = 0; r < PIECES; ++r) mma16816(o[n][2 * w + c], op, b[n][r][0], b[n][r][1]);
+        }
+      }
+    }
+  }
+
+  // f grew by d: keeps M - f, so that l and its bound stay, when d is large
+  __device__ __forceinline__ void raise(int d) {
+    const float by = (float)max(0, d - 40), f = ex2(-by), fl = ex2((float)d - by);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (m[n][i] > LOWEST) m[n][i] += by;
+        l[n][i] *= fl;
+#pragma unroll
+        for (int c = 0; c < MT; ++c) {
+          o[n][c][i] *= f;
+          o[n][c][i + 2] *= f;
+        }
+      }
+  }
+};
+
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(THREADS) attention_kernel(AttnArgs a) {
+  constexpr int R = 8 * NQ, PAD = D + 4;
+  __shared__ Meta meta;
+  __shared__ long long total_s, scan[WARPS];
+  __shared__ int found[2];
+  __shared__ long long found_at;
+  __shared__ float so[R * PAD], sm[WARPS][R], sl[WARPS][R];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const long long cta = blockIdx.x;
+
+  // where this CTA's share of the line of units begins: [lo, hi), in sequence b from unit `at` of b on
+  int b, tile, kvh, u;
+  long long lo = 0, hi = 0, total = 0, base = 0, grid = 1;
+  Seq s;
+  if (a.split) {
+    const int per = (a.r.B + THREADS - 1) / THREADS, b0 = min(tid * per, a.r.B), b1 = min(b0 + per, a.r.B);
+    long long mine = 0;
+    for (int i = b0; i < b1; ++i) {
+      const Seq x = seq_of<NQ>(a, i);
+      mine += (long long)x.units * x.tiles * a.c.KV;
+    }
+    long long upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long y = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += y;
+    }
+    if (lane == 31) scan[warp] = upto;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) upto += scan[i];
+    for (int i = 0; i < WARPS; ++i) total += scan[i];
+    grid = min((long long)gridDim.x, total);  // no CTA between two others is without a unit
+    if (cta >= grid) return;
+    lo = cta * total / grid;
+    hi = (cta + 1) * total / grid;
+    if (lo < upto && lo >= upto - mine) {
+      long long x0 = upto - mine;
+      int i = b0;
+      for (; i < b1 - 1; ++i) {
+        const Seq x = seq_of<NQ>(a, i);
+        const long long w = (long long)x.units * x.tiles * a.c.KV;
+        if (lo < x0 + w) break;
+        x0 += w;
+      }
+      found[0] = i;
+      found_at = x0;
+    }
+    __syncthreads();
+    b = found[0];
+    base = found_at;  // line index of sequence b's first unit
+    s = seq_of<NQ>(a, b);
+    if (s.units == 0) return;  // only if lengths changed under the call
+    const long long at = lo - base;
+    u = (int)(at % s.units);
+    const long long item = at / s.units;
+    kvh = (int)(item % a.c.KV);
+    tile = (int)(item / a.c.KV);
+  } else {
+    kvh = (int)(cta % a.c.KV);
+    tile = (int)(cta / a.c.KV % a.tiles);
+    b = (int)(cta / a.c.KV / a.tiles);
+    s = seq_of<NQ>(a, b);
+    if (tile >= s.tiles) return;
+    u = 0;
+    lo = 0;
+    hi = s.units;
+  }
+
+  Warp<T, D, NQ> w;
+  long long at = lo;
+  do {
+    // one segment: units [u, u1) of item (b, tile, kvh)
+    const int u1 = (int)min((long long)s.units, u + (hi - at));
+    w.start(a, s, tile, kvh, lane);
+    const int first_rho = tile * R;
+    int p_min = w.p[0][0], p_max = p_min;  // of the tile's rows
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        p_min = min(p_min, w.p[n][i]);
+        p_max = max(p_max, w.p[n][i]);
+      }
+    p_min = __reduce_min_sync(0xffffffffu, p_min);
+    p_max = __reduce_max_sync(0xffffffffu, p_max);
+    // the sequence's rows see positions see0 .. see1
+    const int cap = a.r.width << a.c.lg_page, see0 = a.window > 0 ? max(0, max(s.p0, 0) - a.window + 1) : 0;
+    const int see1 = min((long long)s.p0 + s.n - 1, (long long)cap - 1);
+    const int per_unit = UNIT >> a.c.lg_page;
+    if (tid == 0) meta.f = 0;
+    for (int c0 = u; c0 < u1; c0 += META / per_unit) {
+      const int c1 = min(u1, c0 + META / per_unit);
+      const int o0 = (s.u0 + c0) * per_unit, pages = (c1 - c0) * per_unit;
+      __syncthreads();  // every warp is done with the entries before
+      const int f_old = meta.f;
+      __syncthreads();
+      if (tid < pages) {
+        const int o = o0 + tid;
+        int id = -1, ev = 0, ek = 0;
+        if ((o + 1) << a.c.lg_page > see0 && o << a.c.lg_page <= see1) {
+          id = page_id(a.c, a.r, b, o);
+          if (id >= 0) {
+            ek = a.c.k_exp[id * a.c.exp_stride + kvh];
+            ev = a.c.v_exp[id * a.c.exp_stride + kvh];
+            if (ev != 255) atomicMax(&meta.f, ev);
+          }
+        }
+        meta.id[tid] = id;
+        meta.ek[tid] = (uint8_t)ek;
+        meta.ev[tid] = (uint8_t)ev;
+      }
+      __syncthreads();
+      if (c0 > u && meta.f > f_old) w.raise(meta.f - f_old);
+      int e[2];
+      auto entry = [&](int c) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) e[h] = (((c - c0) * UNIT + warp * WTOK + 16 * h) >> a.c.lg_page);
+      };
+      auto first_token = [&](int c) { return (s.u0 + c) * UNIT + warp * WTOK; };
+      entry(c0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) w.load_k(a, meta, h, e[h], first_token(c0) + 16 * h, kvh, lane);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) w.load_v(a, meta, h, e[h], first_token(c0) + 16 * h, kvh, lane);
+      for (int c = c0; c < c1; ++c) {
+        const int j = first_token(c);
+        const int en[2] = {e[0], e[1]};
+        float z[2][NQ][4];
+        w.scores(z);
+        if (c + 1 < c1) {
+          entry(c + 1);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) w.load_k(a, meta, h, e[h], first_token(c + 1) + 16 * h, kvh, lane);
+        }
+        w.weights(a, meta, z, en, j, lane, p_min, p_max);
+        w.outputs(z);
+        if (c + 1 < c1) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) w.load_v(a, meta, h, e[h], first_token(c + 1) + 16 * h, kvh, lane);
+        }
+      }
+    }
+    // the warps' sums: a common M, then O added warp after warp
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d <= 16; d *= 2) w.l[n][i] += __shfl_xor_sync(0xffffffffu, w.l[n][i], d);
+        if (g == 0) {
+          sm[warp][8 * n + 2 * t + i] = w.m[n][i];
+          sl[warp][8 * n + 2 * t + i] = w.l[n][i];
+        }
+      }
+    __syncthreads();
+    for (int x = 0; x < WARPS; ++x) {
+      if (warp == x) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = 8 * n + 2 * t + i;
+            const float f = ex2(w.m[n][i] - fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])));
+#pragma unroll
+            for (int c = 0; c < Warp<T, D, NQ>::MT; ++c) {
+              float *d = so + r * PAD + g * (D / 8) + 2 * c;
+              d[0] = (x ? d[0] : 0.f) + w.o[n][c][i] * f;
+              d[1] = (x ? d[1] : 0.f) + w.o[n][c][i + 2] * f;
+            }
+          }
+      }
+      __syncthreads();
+    }
+    const bool whole = u == 0 && u1 == s.units;
+    float *rec = whole ? nullptr : a.part + (cta * 2 + (u == 0 ? 1 : 0)) * (size_t)(R * (D + 3));
+    const float top = pow2_e8m0(meta.f);
+    for (int x = tid; x < R * (D / 4); x += THREADS) {
+      const int r = x / (D / 4), d = x % (D / 4) * 4, rho = first_rho + r;
+      if (rho >= s.n * a.G) continue;
+      const float mx = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+      float l = 0.f;
+#pragma unroll
+      for (int i = 0; i < WARPS; ++i) l = fmaf(sl[i][r], ex2(sm[i][r] - mx), l);
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = so[r * PAD + d + i];
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = l == 0.f ? 0.f : y[i] / l * top;
+        store4<T>(static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D + d, y);
+      } else {
+        *reinterpret_cast<float4 *>(rec + r * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+        if (d == 0) {
+          rec[R * D + r] = mx;
+          rec[R * (D + 1) + r] = l;
+          rec[R * (D + 2) + r] = (float)(meta.f - 127);
+        }
+      }
+    }
+    if (!whole && u == 0 && tid == 0) {
+      // the item ends at line index base + its units; the CTA that holds its last one
+      const long long end = at + s.units;
+      a.desc[((size_t)b * a.tiles + tile) * a.c.KV + kvh] = make_int2((int)cta, (int)((end * grid - 1) / total));
+    } else if (whole && a.split && tid == 0) {
+      a.desc[((size_t)b * a.tiles + tile) * a.c.KV + kvh] = make_int2((int)cta, (int)cta);
+    }
+    at += u1 - u;
+    if (at >= hi) break;
+    u = 0;
+    if (++kvh == a.c.KV) {
+      kvh = 0;
+      if (++tile == s.tiles) {
+        tile = 0;
+        do {
+          if (++b == a.r.B) return;  // (lengths changed under the call)
+          s = seq_of<NQ>(a, b);
+        } while (s.units == 0);
+      }
+    }
+    __syncthreads();  // so, sm and sl are read until here
+  } while (true);
+}
+
+// joins the records of an item that several CTAs share; zeros for rows of sequences without visible tokens
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
+  constexpr int R = 8 * NQ;
+  const int kvh = blockIdx.x % a.c.KV, tile = blockIdx.x / a.c.KV, b = blockIdx.y;
+  const Seq s = seq_of<NQ>(a, b);
+  if (tile >= s.tiles) return;
+  int2 span = make_int2(0, -1);
+  if (s.units) {
+    span = a.desc[((size_t)b * a.tiles + tile) * a.c.KV + kvh];
+    if (span.x == span.y) return;
+  }
+  for (int x = threadIdx.x; x < R * (D / 4); x += THREADS) {
+    const int r = x / (D / 4), d = x % (D / 4) * 4, rho = tile * R + r;
+    if (rho >= s.n * a.G) continue;
+    auto record = [&](int c) { return a.part + ((size_t)c * 2 + (c == span.x ? 1 : 0)) * (size_t)(R * (D + 3)); };
+    // N = sum O 2^(M - Mg), L = sum l 2^(M - f - Ag), out = N / L 2^(Mg - Ag)
+    float mg = LOWEST, ag = LOWEST, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = span.x; c <= span.y; ++c) {
+      const float *q = record(c);
+      const float m = q[R * D + r];
+      mg = fmaxf(mg, m);
+      if (m > LOWEST) ag = fmaxf(ag, m - q[R * (D + 2) + r]);
+    }
+    for (int c = span.x; c <= span.y; ++c) {
+      const float *q = record(c);
+      const float m = q[R * D + r], f = ex2(m - mg);
+      const float4 v = *reinterpret_cast<const float4 *>(q + r * D + d);
+      y[0] = fmaf(v.x, f, y[0]);
+      y[1] = fmaf(v.y, f, y[1]);
+      y[2] = fmaf(v.z, f, y[2]);
+      y[3] = fmaf(v.w, f, y[3]);
+      l = fmaf(q[R * (D + 1) + r], m > LOWEST ? ex2(m - q[R * (D + 2) + r] - ag) : 1.f, l);
+    }
+    const float top = mg > LOWEST ? ex2(mg - ag) : 1.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = l == 0.f ? 0.f : y[i] / l * top;
+    store4<T>(static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D + d, y);
   }
 }
 
+struct Plan {
+  int nq, tiles, split, grid;
+  size_t desc, bytes;
+};
+
+// row tile: 8 rows, or 16 when a sequence has more (32 spill registers)
+Plan plan_of(const Pool &c, int width, int B, int most, int H, int window, int sms) {
+  Plan p;
+  const long long rows = (long long)most * (H / c.KV);
+  p.nq = rows <= 8 ? 1 : 2;
+  p.tiles = (int)((rows + 8 * p.nq - 1) / (8 * p.nq));
+  long long len = (long long)width << c.lg_page;
+  if (window > 0) len = std::min(len, (long long)window + most + UNIT);
+  const long long units = (len + UNIT - 1) / UNIT, items = (long long)B * c.KV * p.tiles;
+  p.split = units > 1;
+  p.grid = (int)std::min<long long>(p.split ? std::min<long long>(items * units, 3LL * sms) : items, 0x7fffffff);
+  p.desc = p.split ? ((size_t)items * sizeof(int2) + 255) / 256 * 256 : 0;
+  p.bytes = p.split ? p.desc + (size_t)p.grid * 2 * 8 * p.nq * (c.D + 3) * sizeof(float) : 0;
+  return p;
+}
+
+template <typename T, int D, int NQ>
+void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {
+  attention_kernel<T, D, NQ><<<p.grid, THREADS, 0, st>>>(a);
+  if (p.split) join_kernel<T, D, NQ><<<dim3(a.c.KV * a.tiles, a.r.B), THREADS, 0, st>>>(a);
+}
+template <typename T, int D>
+void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {
+  if (p.nq == 1) launch<T, D, 1>(a, p, st);
+  else launch<T, D, 2>(a, p, st);
+}
 template <typename T>
-void launch(const AttnArgs &a, cudaStream_t st) {
-  const dim3 grid(a.r.N, a.H);
-  if (a.c.D == 32) attention_kernel<T, 32><<<grid, WARPS * 32, 0, st>>>(a);
-  else if (a.c.D == 64) attention_kernel<T, 64><<<grid, WARPS * 32, 0, st>>>(a);
-  else attention_kernel<T, 128><<<grid, WARPS * 32, 0, st>>>(a);
+void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {
+  if (a.c.D == 32) launch<T, 32>(a, p, st);
+  else if (a.c.D == 64) launch<T, 64>(a, p, st);
+  else launch<T, 128>(a, p, st);
 }
 
 }  // namespace
@@ -102,7 +610,11 @@ extern "C" {
 
 size_t lbc_kv8_attention_workspace(const lbc_kv8 *c, int dtype, int table_width, int B, int N, int max_tokens, int H,
                                    int window) {
-  return 0;
+  Pool p;
+  int *status = nullptr, sms = 0;
+  if (check_pool(c, p) || device_ready(&status, &sms) || table_width <= 0 || B <= 0 || H <= 0 || H % p.KV || max_tokens < 0)
+    return 0;
+  return plan_of(p, table_width, B, max_tokens, H, window, sms).bytes;
 }
 
 int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, const int32_t *table, int table_width,
@@ -114,18 +626,26 @@ int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, 
   if (int rc = device_ready(&status, &sms)) return rc;
   if (int rc = check_rows(a.c, table, table_width, pos, starts, B, N, max_tokens, status, a.r)) return rc;
   if (dtype < LBC_F32 || dtype > LBC_F16) return refuse("kv8_attention: dtype must be fp32, bf16 or fp16");
-  if (H <= 0 || H % a.c.KV || H > 65535) return refuse("kv8_attention: H must be a multiple of the KV heads");
-  if (N == 0) return 0;
+  if (H <= 0 || H % a.c.KV || H > 65535 || (long long)max_tokens * H > 0x7fffffff)
+    return refuse("kv8_attention: H must be a multiple of the KV heads");
+  if (N == 0 || max_tokens == 0) return 0;
   if (!q || !out) return refuse("kv8_attention: NULL argument");
   if (ld < (long long)H * a.c.D || ld * (dtype == LBC_F32 ? 4 : 2) % 16) return refuse("kv8_attention: bad row stride");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)
     return refuse("kv8_attention: q and out must be 16-byte aligned");
-  a.q = q; a.ld = ld; a.out = out; a.H = H; a.window = window;
+  a.q = q; a.ld = ld; a.out = out; a.H = H; a.G = H / a.c.KV; a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f;
+  const Plan p = plan_of(a.c, table_width, B, max_tokens, H, window, sms);
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return refuse("kv8_attention: workspace too small or not 256-byte aligned");
+  a.tiles = p.tiles;
+  a.split = p.split;
+  a.desc = static_cast<int2 *>(workspace);
+  a.part = p.split ? reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + p.desc) : nullptr;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == LBC_F32) launch<float>(a, st);
-  else if (dtype == LBC_BF16) launch<__nv_bfloat16>(a, st);
-  else launch<__half>(a, st);
+  if (dtype == LBC_F32) launch<float>(a, p, st);
+  else if (dtype == LBC_BF16) launch<__nv_bfloat16>(a, p, st);
+  else launch<__half>(a, p, st);
   return launched("kv8_attention");
 }
 

@@ -89,6 +89,10 @@ __device__ __forceinline__ int scale_byte(float amax) {
 
 // ------------------------------------------------------------ element types
 template <typename T>
+constexpr bool is_bf16 = false;
+template <>
+constexpr bool is_bf16<__nv_bfloat16> = true;
+template <typename T>
 __device__ __forceinline__ float to_f(T v);
 template <>
 __device__ __forceinline__ float to_f<float>(float v) { return v; }

@@ -34,15 +34,27 @@ namespace lbc {
 namespace kv8 {
 namespace {
 
+#ifndef HT
+#define HT 1
+#endif
+#ifndef RES1
+#define RES1 4
+#endif
+#ifndef RES2
+#define RES2 2
+#endif
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int WTOK = 32;            // tokens of a warp in a unit: two 16-token tiles
-constexpr int UNIT = WARPS * WTOK;  // 128 tokens: page sizes divide it
+constexpr int WTOK = 16 * HT;       // tokens of a warp in a unit
+constexpr int UNIT = WARPS * WTOK;
 constexpr int META = 128;           // pages looked up at a time
 constexpr float LOWEST = -3e38f;    // M before any visible token
 // weights 2^(t - M) fill fp16's range: M is the maximum (rounded up) less 14,
 // left alone while no weight passes 2^15. Two pieces then hold a weight to 22
 // bits down to 2^-17 of the largest, one piece to 11 bits down to 2^-28.
 constexpr float HEAD = 14.f, SLACK = 15.f;
+// blocks whose value scale is 2^60 below the largest count with 2^(f - 60): they
+// only matter to l (an all-zero block has exponent 0)
+constexpr int FAR = 60;
 
 struct AttnArgs {
   Pool c;
@@ -89,20 +101,23 @@ __device__ __forceinline__ int row_pos(const AttnArgs &a, const Seq &s, int rho)
 }
 
 struct Meta {
-  int id[META];  // -1: no such page
-  uint8_t ek[META], ev[META];
-  int f;  // largest value exponent so far (255 left out)
+  long long off[META];  // bytes to the block's codes (a page that does not exist: to page 0's)
+  float4 s[META];       // 2^(ek - 127), b = ev - 127, 2^(f - b), 1 if the page exists
+  int f;                // largest value exponent so far (255 left out)
 };
 
 template <typename T, int D, int NQ>
 struct Warp {
-  static constexpr int PIECES = sizeof(T) == 4 ? 2 : 1;
+  // fp16 pieces of queries and of weights: fp32 needs 22 bits of both; bf16 and
+  // fp16 queries are exact in one; fp16 outputs (11 bits) would show weights
+  // rounded to 11 bits (error 1.5 times the output's own), bf16 ones do not
+  static constexpr int QP = sizeof(T) == 4 ? 2 : 1, WP = is_bf16<T> ? 1 : 2;
   static constexpr int KW = D / 16, VW = D / 32, MT = D / 16;
-  uint32_t q[NQ][PIECES][KW][2];  // query operand
+  uint32_t q[NQ][QP][KW][2];  // query operand
   float rowf[NQ][2];              // score = accumulator * rowf * 2^(ek - 127), in log2 units
   int p[NQ][2];                   // positions of the lane's rows 8 n + 2 t + i
   float m[NQ][2], l[NQ][2], o[NQ][MT][4];
-  uint32_t k[2][2][KW], v[2][4][VW];
+  uint32_t k[HT][2][KW], v[HT][4][VW];
 
   // first element of the four that lane t's word s of a key row holds
   __device__ static int key_dim(int t, int s) { return D == 32 ? 8 * t + 4 * s : 64 * (s / 4) + 16 * t + 4 * (s % 4); }
@@ -134,7 +149,7 @@ struct Warp {
         for (int h = 0; h < 2; ++h) {
           const float x0 = x[w][2 * h] * f, x1 = x[w][2 * h + 1] * f;
           q[n][0][w][h] = pack_half(x0, x1);
-          if constexpr (PIECES == 2) q[n][1][w][h] = pack_rest(x0, x1, q[n][0][w][h]);
+          if constexpr (QP == 2) q[n][1][w][h] = pack_rest(x0, x1, q[n][0][w][h]);
         }
       const float back = a.scale_log2 / f;
 #pragma unroll
@@ -149,31 +164,28 @@ struct Warp {
     }
   }
 
-  // codes of the 16-token tile at position j, whose page is entry `e`
-  __device__ __forceinline__ void load_k(const AttnArgs &a, const Meta &x, int h, int e, int j, int kvh, int lane) {
-    const int g = lane >> 2, t = lane & 3, id = max(x.id[e], 0);
-    const int8_t *src = a.c.k + id * a.c.page_stride + ((size_t)kvh * a.c.page + (j & (a.c.page - 1))) * D;
+  // codes of the h-th 16-token tile, whose first token's are at `off` of the pools
+  __device__ __forceinline__ void load_k(const AttnArgs &a, int h, long long off, int lane) {
+    const int8_t *src = a.c.k + off + (lane >> 2) * D + (lane & 3) * (D == 32 ? 8 : 16);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int8_t *row = src + (g + 8 * r) * D;
       if constexpr (D == 32) {
-        load_words<8>(row + 8 * t, k[h][r]);
+        load_words<8>(src + 8 * r * D, k[h][r]);
       } else {
 #pragma unroll
-        for (int w = 0; w < KW; w += 4) load_words<16>(row + 16 * w + 16 * t, k[h][r] + w);
+        for (int w = 0; w < KW; w += 4) load_words<16>(src + 8 * r * D + 16 * w, k[h][r] + w);
       }
     }
   }
-  __device__ __forceinline__ void load_v(const AttnArgs &a, const Meta &x, int h, int e, int j, int kvh, int lane) {
-    const int g = lane >> 2, t = lane & 3, id = max(x.id[e], 0);
-    const int8_t *src = a.c.v + id * a.c.page_stride + ((size_t)kvh * a.c.page + (j & (a.c.page - 1))) * D + g * (D / 8);
+  __device__ __forceinline__ void load_v(const AttnArgs &a, int h, long long off, int lane) {
+    const int8_t *src = a.c.v + off + (lane & 3) * 2 * D + (lane >> 2) * (D / 8);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) load_words<D / 8>(src + (2 * t + (r & 1) + 8 * (r >> 1)) * D, v[h][r]);
+    for (int r = 0; r < 4; ++r) load_words<D / 8>(src + ((r & 1) + 8 * (r >> 1)) * D, v[h][r]);
   }
 
-  __device__ __forceinline__ void scores(float (&z)[2][NQ][4]) {
+  __device__ __forceinline__ void scores(float (&z)[HT][NQ][4]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < HT; ++h) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) z[h][n][0] = z[h][n][1] = z[h][n][2] = z[h][n][3] = 0.f;
 #pragma unroll
@@ -183,48 +195,54 @@ struct Warp {
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int c = 0; c < PIECES; ++c) mma16816(z[h][n], op, q[n][c][w][0], q[n][c][w][1]);
+          for (int c = 0; c < QP; ++c) mma16816(z[h][n], op, q[n][c][w][0], q[n][c][w][1]);
       }
     }
   }
 
-  // z: scores to weights (in place); j: position of the warp's first token; e: its pages
-  __device__ __forceinline__ void weights(const AttnArgs &a, const Meta &x, float (&z)[2][NQ][4], const int (&e)[2], int j,
-                                          int lane, int p_min, int p_max) {
-    const int g = lane >> 2;
-    float back[2];
+  // z: scores to weights (in place); j: position of the warp's first token; e: its tiles' pages
+  __device__ __forceinline__ void weights(const AttnArgs &a, const float4 (&e)[HT], float (&z)[HT][NQ][4], int j, int lane,
+                                          int p_min, int p_max) {
+    float mx[NQ][2];
     bool rise = false;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j0 = j + 16 * h, ev = x.ev[e[h]];
-      const float ks = pow2_e8m0(x.ek[e[h]]);
-      // a block far below f would take its weights out of range: it counts in l only
-      const float b = ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(max(ev, x.f - 60) - 127);
-      back[h] = ev == 255 ? 1.f : pow2_e8m0(127 + x.f - max(ev, x.f - 60));
-      const bool whole = j0 + 15 <= p_min && (a.window <= 0 || j0 > p_max - a.window) && x.id[e[h]] >= 0;
+    for (int h = 0; h < HT; ++h) {
+      const int j0 = j + 16 * h;
+      const bool whole = j0 + 15 <= p_min && (a.window <= 0 || j0 > p_max - a.window) && e[h].w != 0.f;
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float t = fmaf(z[h][n][i], rowf[n][i & 1] * ks, b);
-          if (!whole) {
-            const int at = j0 + g + 8 * (i >> 1), pr = p[n][i & 1];
-            const bool seen = at <= pr && (a.window <= 0 || at > pr - a.window) && x.id[e[h]] >= 0;
-            t = seen ? t : -INFINITY;
+        for (int i = 0; i < 4; ++i) z[h][n][i] = fmaf(z[h][n][i], rowf[n][i & 1] * e[h].x, e[h].y);
+      if (!whole) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = j0 + (lane >> 2) + 8 * (i >> 1), pr = p[n][i & 1];
+            const bool seen = at <= pr && (a.window <= 0 || at > pr - a.window) && e[h].w != 0.f;
+            z[h][n][i] = seen ? z[h][n][i] : -INFINITY;
           }
-          z[h][n][i] = t;
-          rise |= t > m[n][i & 1] + SLACK;
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float y = fmaxf(z[h][n][i], z[h][n][i + 2]);
+          mx[n][i] = h ? fmaxf(mx[n][i], y) : y;
         }
     }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) rise |= mx[n][i] > m[n][i] + SLACK;
     if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float mx = fmaxf(fmaxf(z[0][n][i], z[0][n][i + 2]), fmaxf(z[1][n][i], z[1][n][i + 2]));
 #pragma unroll
-          for (int d = 4; d <= 16; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-          const float to = fmaxf(m[n][i], ceilf(mx) - HEAD), f = ex2(m[n][i] - to);
+          for (int d = 4; d <= 16; d *= 2) mx[n][i] = fmaxf(mx[n][i], __shfl_xor_sync(0xffffffffu, mx[n][i], d));
+          const float to = fmaxf(m[n][i], ceilf(mx[n][i]) - HEAD), f = ex2(m[n][i] - to);
           m[n][i] = to;
           l[n][i] *= f;
 #pragma unroll
@@ -235,30 +253,27 @@ struct Warp {
         }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool far = x.ev[e[h]] != 255 && x.ev[e[h]] < x.f - 60;
+    for (int h = 0; h < HT; ++h)
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float w = ex2(z[h][n][i] - m[n][i & 1]);
-          l[n][i & 1] = fmaf(w, back[h], l[n][i & 1]);
-          z[h][n][i] = far ? 0.f : w;
+          z[h][n][i] = ex2(z[h][n][i] - m[n][i & 1]);
+          l[n][i & 1] = fmaf(z[h][n][i], e[h].z, l[n][i & 1]);
         }
-    }
   }
 
-  __device__ __forceinline__ void outputs(const float (&z)[2][NQ][4]) {
+  __device__ __forceinline__ void outputs(const float (&z)[HT][NQ][4]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t b[NQ][PIECES][2];
+    for (int h = 0; h < HT; ++h) {
+      uint32_t b[NQ][WP][2];
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t hi = pack_half(z[h][n][2 * i], z[h][n][2 * i + 1]);
           b[n][0][i] = transpose8(hi);
-          if constexpr (PIECES == 2) b[n][1][i] = transpose8(pack_rest(z[h][n][2 * i], z[h][n][2 * i + 1], hi));
+          if constexpr (WP == 2) b[n][1][i] = transpose8(pack_rest(z[h][n][2 * i], z[h][n][2 * i + 1], hi));
         }
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
@@ -272,7 +287,7 @@ struct Warp {
 #pragma unroll
           for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int r = 0; r < PIECES; ++r) mma16816(o[n][2 * w + c], op, b[n][r][0], b[n][r][1]);
+            for (int r = 0; r < WP; ++r) mma16816(o[n][2 * w + c], op, b[n][r][0], b[n][r][1]);
         }
       }
     }
@@ -297,12 +312,13 @@ struct Warp {
 };
 
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(THREADS) attention_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kernel(AttnArgs a) {
   constexpr int R = 8 * NQ, PAD = D + 4;
   __shared__ Meta meta;
   __shared__ long long total_s, scan[WARPS];
-  __shared__ int found[2];
+  __shared__ int found;
   __shared__ long long found_at;
+  __shared__ Seq found_seq;
   __shared__ float so[R * PAD], sm[WARPS][R], sl[WARPS][R];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const long long cta = blockIdx.x;
@@ -335,19 +351,19 @@ __global__ void __launch_bounds__(THREADS) attention_kernel(AttnArgs a) {
     if (lo < upto && lo >= upto - mine) {
       long long x0 = upto - mine;
       int i = b0;
-      for (; i < b1 - 1; ++i) {
-        const Seq x = seq_of<NQ>(a, i);
-        const long long w = (long long)x.units * x.tiles * a.c.KV;
-        if (lo < x0 + w) break;
-        x0 += w;
+      Seq x = seq_of<NQ>(a, i);
+      while (i < b1 - 1 && lo >= x0 + (long long)x.units * x.tiles * a.c.KV) {
+        x0 += (long long)x.units * x.tiles * a.c.KV;
+        x = seq_of<NQ>(a, ++i);
       }
-      found[0] = i;
+      found = i;
       found_at = x0;
+      found_seq = x;
     }
     __syncthreads();
-    b = found[0];
+    b = found;
     base = found_at;  // line index of sequence b's first unit
-    s = seq_of<NQ>(a, b);
+    s = found_seq;
     if (s.units == 0) return;  // only if lengths changed under the call
     const long long at = lo - base;
     u = (int)(at % s.units);
@@ -370,75 +386,91 @@ __global__ void __launch_bounds__(THREADS) attention_kernel(AttnArgs a) {
   do {
     // one segment: units [u, u1) of item (b, tile, kvh)
     const int u1 = (int)min((long long)s.units, u + (hi - at));
-    w.start(a, s, tile, kvh, lane);
     const int first_rho = tile * R;
-    int p_min = w.p[0][0], p_max = p_min;  // of the tile's rows
-#pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        p_min = min(p_min, w.p[n][i]);
-        p_max = max(p_max, w.p[n][i]);
-      }
-    p_min = __reduce_min_sync(0xffffffffu, p_min);
-    p_max = __reduce_max_sync(0xffffffffu, p_max);
+    int p_min = 0, p_max = 0;
     // the sequence's rows see positions see0 .. see1
     const int cap = a.r.width << a.c.lg_page, see0 = a.window > 0 ? max(0, max(s.p0, 0) - a.window + 1) : 0;
     const int see1 = min((long long)s.p0 + s.n - 1, (long long)cap - 1);
-    const int per_unit = UNIT >> a.c.lg_page;
+    const int chunk = ((META - 1) << a.c.lg_page) / UNIT;  // units whose pages are looked up together
+    const long long head = (long long)kvh * a.c.page * D;
+    int f = 0;
     if (tid == 0) meta.f = 0;
-    for (int c0 = u; c0 < u1; c0 += META / per_unit) {
-      const int c1 = min(u1, c0 + META / per_unit);
-      const int o0 = (s.u0 + c0) * per_unit, pages = (c1 - c0) * per_unit;
-      __syncthreads();  // every warp is done with the entries before
-      const int f_old = meta.f;
-      __syncthreads();
+    for (int c0 = u; c0 < u1; c0 += chunk) {
+      const int c1 = min(u1, c0 + chunk);
+      const int o0 = (s.u0 + c0) * UNIT >> a.c.lg_page, pages = (((s.u0 + c1) * UNIT - 1) >> a.c.lg_page) - o0 + 1;
+      int id = -1;
+      if (c0 > u) __syncthreads();  // every warp is done with the entries before
       if (tid < pages) {
         const int o = o0 + tid;
-        int id = -1, ev = 0, ek = 0;
-        if ((o + 1) << a.c.lg_page > see0 && o << a.c.lg_page <= see1) {
-          id = page_id(a.c, a.r, b, o);
-          if (id >= 0) {
-            ek = a.c.k_exp[id * a.c.exp_stride + kvh];
-            ev = a.c.v_exp[id * a.c.exp_stride + kvh];
-            if (ev != 255) atomicMax(&meta.f, ev);
-          }
-        }
-        meta.id[tid] = id;
-        meta.ek[tid] = (uint8_t)ek;
-        meta.ev[tid] = (uint8_t)ev;
+        if ((o + 1) << a.c.lg_page > see0 && o << a.c.lg_page <= see1) id = page_id(a.c, a.r, b, o);
+        meta.off[tid] = max(id, 0) * a.c.page_stride + head;
       }
       __syncthreads();
-      if (c0 > u && meta.f > f_old) w.raise(meta.f - f_old);
-      int e[2];
-      auto entry = [&](int c) {
+      int en[HT];
+      long long off[HT];
+      // pages and code offsets of the warp's tiles in unit c
+      auto locate = [&](int c) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) e[h] = (((c - c0) * UNIT + warp * WTOK + 16 * h) >> a.c.lg_page);
+        for (int h = 0; h < HT; ++h) {
+          const int j = (s.u0 + c) * UNIT + warp * WTOK + 16 * h;
+          en[h] = (j >> a.c.lg_page) - o0;
+          off[h] = meta.off[en[h]] + (j & (a.c.page - 1)) * D;
+        }
       };
-      auto first_token = [&](int c) { return (s.u0 + c) * UNIT + warp * WTOK; };
-      entry(c0);
+      locate(c0);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) w.load_k(a, meta, h, e[h], first_token(c0) + 16 * h, kvh, lane);
+      for (int h = 0; h < HT; ++h) w.load_k(a, h, off[h], lane);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) w.load_v(a, meta, h, e[h], first_token(c0) + 16 * h, kvh, lane);
+      for (int h = 0; h < HT; ++h) w.load_v(a, h, off[h], lane);
+      int ek = 0, ev = 0;
+      if (id >= 0) {
+        ek = a.c.k_exp[id * a.c.exp_stride + kvh];
+        ev = a.c.v_exp[id * a.c.exp_stride + kvh];
+      }
+      if (c0 == u) w.start(a, s, tile, kvh, lane);
+      if (id >= 0 && ev != 255) atomicMax(&meta.f, ev);
+      __syncthreads();
+      const int f_old = f;
+      f = meta.f;
+      if (tid < pages) {
+        const int at = max(ev, f - FAR);
+        meta.s[tid] = make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(at - 127),
+                                  ev == 255 ? 1.f : pow2_e8m0(127 + f - at), id >= 0 ? 1.f : 0.f);
+      }
+      __syncthreads();
+      if (c0 > u && f > f_old) w.raise(f - f_old);
+      if (c0 == u) {
+        p_min = p_max = w.p[0][0];  // of the tile's rows
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            p_min = min(p_min, w.p[n][i]);
+            p_max = max(p_max, w.p[n][i]);
+          }
+        p_min = __reduce_min_sync(0xffffffffu, p_min);
+        p_max = __reduce_max_sync(0xffffffffu, p_max);
+      }
       for (int c = c0; c < c1; ++c) {
-        const int j = first_token(c);
-        const int en[2] = {e[0], e[1]};
-        float z[2][NQ][4];
+        float z[HT][NQ][4];
+        float4 e[HT];
+#pragma unroll
+        for (int h = 0; h < HT; ++h) e[h] = meta.s[en[h]];
         w.scores(z);
         if (c + 1 < c1) {
-          entry(c + 1);
+          locate(c + 1);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) w.load_k(a, meta, h, e[h], first_token(c + 1) + 16 * h, kvh, lane);
+          for (int h = 0; h < HT; ++h) w.load_k(a, h, off[h], lane);
         }
-        w.weights(a, meta, z, en, j, lane, p_min, p_max);
+        w.weights(a, e, z, (s.u0 + c) * UNIT + warp * WTOK, lane, p_min, p_max);
         w.outputs(z);
         if (c + 1 < c1) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) w.load_v(a, meta, h, e[h], first_token(c + 1) + 16 * h, kvh, lane);
+          for (int h = 0; h < HT; ++h) w.load_v(a, h, off[h], lane);
         }
       }
     }
+    if (u == u1) w.start(a, s, tile, kvh, lane);  // an item without units: rows of zeros
     // the warps' sums: a common M, then O added warp after warp
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
@@ -472,7 +504,7 @@ __global__ void __launch_bounds__(THREADS) attention_kernel(AttnArgs a) {
     }
     const bool whole = u == 0 && u1 == s.units;
     float *rec = whole ? nullptr : a.part + (cta * 2 + (u == 0 ? 1 : 0)) * (size_t)(R * (D + 3));
-    const float top = pow2_e8m0(meta.f);
+    const float top = pow2_e8m0(f);
     for (int x = tid; x < R * (D / 4); x += THREADS) {
       const int r = x / (D / 4), d = x % (D / 4) * 4, rho = first_rho + r;
       if (rho >= s.n * a.G) continue;
@@ -492,7 +524,7 @@ __global__ void __launch_bounds__(THREADS) attention_kernel(AttnArgs a) {
         if (d == 0) {
           rec[R * D + r] = mx;
           rec[R * (D + 1) + r] = l;
-          rec[R * (D + 2) + r] = (float)(meta.f - 127);
+          rec[R * (D + 2) + r] = (float)(f - 127);
         }
       }
     }
@@ -520,45 +552,85 @@ __global__ void __launch_bounds__(THREADS) attention_kernel(AttnArgs a) {
   } while (true);
 }
 
-// joins the records of an item that several CTAs share; zeros for rows of sequences without visible tokens
+// joins the records of a row that several CTAs share, in their order: with
+// Mg = max M and Ag = max (M - f) over the records,
+//   out = 2^(Mg - Ag) sum O 2^(M - Mg) / sum l 2^(M - f - Ag).
+// One CTA a row: its threads are D / 4 columns by THREADS / (D / 4) record
+// slices. Writes the zeros of sequences without visible tokens.
 template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
-  constexpr int R = 8 * NQ;
-  const int kvh = blockIdx.x % a.c.KV, tile = blockIdx.x / a.c.KV, b = blockIdx.y;
+  constexpr int R = 8 * NQ, C = D / 4, SLICES = THREADS / C;
+  __shared__ float red[2][WARPS], wo[THREADS];
+  __shared__ float4 part[SLICES][C];
+  __shared__ float den[WARPS];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int r = blockIdx.x % R, kvh = blockIdx.x / R % a.c.KV, tile = blockIdx.x / R / a.c.KV, b = blockIdx.y;
+  const int tid = threadIdx.x, col = tid % C, slice = tid / C, rho = tile * R + r;
   const Seq s = seq_of<NQ>(a, b);
-  if (tile >= s.tiles) return;
-  int2 span = make_int2(0, -1);
-  if (s.units) {
-    span = a.desc[((size_t)b * a.tiles + tile) * a.c.KV + kvh];
-    if (span.x == span.y) return;
+  if (rho >= s.n * a.G) return;
+  T *dst = static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D + 4 * col;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (s.units == 0) {
+    if (slice == 0) store4<T>(dst, reinterpret_cast<const float(&)[4]>(y));
+    return;
   }
-  for (int x = threadIdx.x; x < R * (D / 4); x += THREADS) {
-    const int r = x / (D / 4), d = x % (D / 4) * 4, rho = tile * R + r;
-    if (rho >= s.n * a.G) continue;
-    auto record = [&](int c) { return a.part + ((size_t)c * 2 + (c == span.x ? 1 : 0)) * (size_t)(R * (D + 3)); };
-    // N = sum O 2^(M - Mg), L = sum l 2^(M - f - Ag), out = N / L 2^(Mg - Ag)
-    float mg = LOWEST, ag = LOWEST, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = span.x; c <= span.y; ++c) {
-      const float *q = record(c);
-      const float m = q[R * D + r];
-      mg = fmaxf(mg, m);
-      if (m > LOWEST) ag = fmaxf(ag, m - q[R * (D + 2) + r]);
-    }
-    for (int c = span.x; c <= span.y; ++c) {
-      const float *q = record(c);
-      const float m = q[R * D + r], f = ex2(m - mg);
-      const float4 v = *reinterpret_cast<const float4 *>(q + r * D + d);
-      y[0] = fmaf(v.x, f, y[0]);
-      y[1] = fmaf(v.y, f, y[1]);
-      y[2] = fmaf(v.z, f, y[2]);
-      y[3] = fmaf(v.w, f, y[3]);
-      l = fmaf(q[R * (D + 1) + r], m > LOWEST ? ex2(m - q[R * (D + 2) + r] - ag) : 1.f, l);
-    }
-    const float top = mg > LOWEST ? ex2(mg - ag) : 1.f;
+  const int2 span = a.desc[((size_t)b * a.tiles + tile) * a.c.KV + kvh];
+  if (span.x == span.y) return;
+  auto record = [&](int c) { return a.part + ((size_t)c * 2 + (c == span.x ? 1 : 0)) * (size_t)(R * (D + 3)); };
+  float mg = LOWEST, ag = LOWEST, l = 0.f;
+  for (int c = span.x + tid; c <= span.y; c += THREADS) {
+    const float *q = record(c) + R * D + r;
+    mg = fmaxf(mg, q[0]);
+    if (q[0] > LOWEST) ag = fmaxf(ag, q[0] - q[2 * R]);
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = l == 0.f ? 0.f : y[i] / l * top;
-    store4<T>(static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D + d, y);
+  for (int d = 16; d >= 1; d /= 2) {
+    mg = fmaxf(mg, __shfl_xor_sync(0xffffffffu, mg, d));
+    ag = fmaxf(ag, __shfl_xor_sync(0xffffffffu, ag, d));
   }
+  if ((tid & 31) == 0) {
+    red[0][tid >> 5] = mg;
+    red[1][tid >> 5] = ag;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) {
+    mg = fmaxf(mg, red[0][i]);
+    ag = fmaxf(ag, red[1][i]);
+  }
+  for (int c0 = span.x; c0 <= span.y; c0 += THREADS) {
+    const int n = min(THREADS, span.y - c0 + 1);
+    if (tid < n) {
+      const float *q = record(c0 + tid) + R * D + r;
+      wo[tid] = ex2(q[0] - mg);
+      l = fmaf(q[R], q[0] > LOWEST ? ex2(q[0] - q[2 * R] - ag) : 1.f, l);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int c = slice; c < n; c += SLICES) {
+      const float4 v = *reinterpret_cast<const float4 *>(record(c0 + c) + r * D + 4 * col);
+      const float f = wo[c];
+      y.x = fmaf(v.x, f, y.x);
+      y.y = fmaf(v.y, f, y.y);
+      y.z = fmaf(v.z, f, y.z);
+      y.w = fmaf(v.w, f, y.w);
+    }
+    __syncthreads();
+  }
+  part[slice][col] = y;
+#pragma unroll
+  for (int d = 16; d >= 1; d /= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if ((tid & 31) == 0) den[tid >> 5] = l;
+  __syncthreads();
+  if (slice) return;
+  for (int i = 1; i < SLICES; ++i) {
+    const float4 v = part[i][col];
+    y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
+  }
+  l = den[0] + den[1] + den[2] + den[3];
+  const float f = l == 0.f ? 0.f : (mg > LOWEST ? ex2(mg - ag) : 1.f) / l;
+  const float out[4] = {y.x * f, y.y * f, y.z * f, y.w * f};
+  store4<T>(dst, out);
 }
 
 struct Plan {
@@ -576,7 +648,7 @@ Plan plan_of(const Pool &c, int width, int B, int most, int H, int window, int s
   if (window > 0) len = std::min(len, (long long)window + most + UNIT);
   const long long units = (len + UNIT - 1) / UNIT, items = (long long)B * c.KV * p.tiles;
   p.split = units > 1;
-  p.grid = (int)std::min<long long>(p.split ? std::min<long long>(items * units, 3LL * sms) : items, 0x7fffffff);
+  p.grid = (int)std::min<long long>(p.split ? std::min<long long>(items * units, (long long)(p.nq == 1 ? RES1 : RES2) * sms) : items, 0x7fffffff);
   p.desc = p.split ? ((size_t)items * sizeof(int2) + 255) / 256 * 256 : 0;
   p.bytes = p.split ? p.desc + (size_t)p.grid * 2 * 8 * p.nq * (c.D + 3) * sizeof(float) : 0;
   return p;
@@ -585,7 +657,18 @@ Plan plan_of(const Pool &c, int width, int B, int most, int H, int window, int s
 template <typename T, int D, int NQ>
 void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {
   attention_kernel<T, D, NQ><<<p.grid, THREADS, 0, st>>>(a);
-  if (p.split) join_kernel<T, D, NQ><<<dim3(a.c.KV * a.tiles, a.r.B), THREADS, 0, st>>>(a);
+  if (!p.split) return;
+  // started while the last CTAs of the first kernel run; it waits for their records
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(8 * NQ * a.c.KV * a.tiles, a.r.B);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, join_kernel<T, D, NQ>, a);
 }
 template <typename T, int D>
 void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {

@@ -8,8 +8,11 @@
 // queries are scaled by a power of two per row into fp16's range (fp32 ones as
 // two pieces, 22 bits), weights likewise (fp32: two pieces; 16-bit types: one).
 // Contraction indices may be permuted freely, and are: a lane loads 16
-// contiguous bytes of its token's key (or of four tokens' values) straight
-// from global memory into the operand registers, no shared memory between.
+// contiguous bytes of its token's key (or of four tokens' values) as operand
+// registers. Codes reach shared memory by cp.async in whole rows (half rows
+// cost twice the L2 traffic), 16-byte pieces permuted so that neither read
+// meets a bank twice; every warp has its own ring, so warps keep several
+// steps in flight and need no barriers.
 //
 // With z_j = log2(e) scale q.k_j the weights carry their block's value scale
 // 2^b_j: t_j = z_j + b_j, M about max t_j - 14 the running reference,
@@ -22,7 +25,10 @@
 // are cut into units of 128 (32 a warp). The units of all items form one line
 // that is cut evenly over the grid, wherever lengths differ: a CTA runs
 // through the ends of items and whole ones; cut items leave partial
-// (O, M, l, f) records that a second kernel joins in order (no atomics).
+// (O, M, l, f) records that a second kernel joins in order (no atomics). When
+// all items' longest possible ranges fit one wave of the grid anyway (few
+// sequences, short tables), a cluster of up to 8 CTAs takes an item instead and
+// joins its sums through distributed shared memory: one launch, no workspace.
 #include <algorithm>
 #include <cstdio>
 
@@ -36,6 +42,9 @@ namespace {
 
 #ifndef HT
 #define HT 1
+#endif
+#ifndef STAGES
+#define STAGES 2
 #endif
 #ifndef RES1
 #define RES1 4
@@ -65,7 +74,7 @@ struct AttnArgs {
   int H, G, window;
   float scale_log2;  // scale * log2(e)
   int tiles;         // row tiles a sequence can have
-  int split;         // 0: one CTA an item, no partials
+  int split;         // 0: a cluster an item
   int2 *desc;        // [B][tiles][KV] first and last CTA of an item
   float *part;       // [grid][2] records: O [8 NQ][D], then M, l, f [8 NQ] each
 };
@@ -117,10 +126,10 @@ struct Warp {
   float rowf[NQ][2];              // score = accumulator * rowf * 2^(ek - 127), in log2 units
   int p[NQ][2];                   // positions of the lane's rows 8 n + 2 t + i
   float m[NQ][2], l[NQ][2], o[NQ][MT][4];
-  uint32_t k[HT][2][KW], v[HT][4][VW];
+  
 
   // first element of the four that lane t's word s of a key row holds
-  __device__ static int key_dim(int t, int s) { return D == 32 ? 8 * t + 4 * s : 64 * (s / 4) + 16 * t + 4 * (s % 4); }
+  __device__ static int key_dim(int t, int s) { return t * (D / 4) + 4 * s; }
 
   __device__ __forceinline__ void start(const AttnArgs &a, const Seq &s, int tile, int kvh, int lane) {
     const int g = lane >> 2, t = lane & 3;
@@ -164,33 +173,43 @@ struct Warp {
     }
   }
 
-  // codes of the h-th 16-token tile, whose first token's are at `off` of the pools
-  __device__ __forceinline__ void load_k(const AttnArgs &a, int h, long long off, int lane) {
-    const int8_t *src = a.c.k + off + (lane >> 2) * D + (lane & 3) * (D == 32 ? 8 : 16);
+  // one ring step: 16 tokens' keys, then their values
+  static constexpr int STEP = 32 * D;
+  // byte offset of 16-byte piece c of row r: pieces change places within their 128-byte line
+  __device__ static int place(int r, int c) {
+    constexpr int RL = 128 / D, PR = D / 16;  // rows a line, pieces a row
+    return (r / RL) * 128 + (((r % RL * PR + c) ^ (D == 128 ? r & 7 : D == 64 ? (r >> 1 & 3) << 1 : (r >> 2 & 1) << 1)) << 4);
+  }
+  __device__ __forceinline__ void fetch(const AttnArgs &a, uint32_t step, long long off, int lane) {
+    constexpr int PR = D / 16, RI = 32 / PR;  // rows an instruction copies
+    const int8_t *k = a.c.k + off + lane * 16, *v = a.c.v + off + lane * 16;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      if constexpr (D == 32) {
-        load_words<8>(src + 8 * r * D, k[h][r]);
-      } else {
-#pragma unroll
-        for (int w = 0; w < KW; w += 4) load_words<16>(src + 8 * r * D + 16 * w, k[h][r] + w);
-      }
+    for (int i = 0; i < 16 / RI; ++i) {
+      const int at = place(lane / PR + i * RI, lane % PR);
+      copy_async16(step + at, k + i * 512);
+      copy_async16(step + 16 * D + at, v + i * 512);
     }
   }
-  __device__ __forceinline__ void load_v(const AttnArgs &a, int h, long long off, int lane) {
-    const int8_t *src = a.c.v + off + (lane & 3) * 2 * D + (lane >> 2) * (D / 8);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) load_words<D / 8>(src + ((r & 1) + 8 * (r >> 1)) * D, v[h][r]);
-  }
 
-  __device__ __forceinline__ void scores(float (&z)[HT][NQ][4]) {
+  __device__ __forceinline__ void scores(float (&z)[HT][NQ][4], const uint32_t (&step)[HT], int lane) {
 #pragma unroll
     for (int h = 0; h < HT; ++h) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) z[h][n][0] = z[h][n][1] = z[h][n][2] = z[h][n][3] = 0.f;
+      uint32_t k[2][KW];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = (lane >> 2) + 8 * i, t = lane & 3;
+        if constexpr (D == 32) shared_words<8>(step[h] + place(r, t >> 1) + (t & 1) * 8, k[i]);
+        if constexpr (D == 64) shared_words<16>(step[h] + place(r, t), k[i]);
+        if constexpr (D == 128) {
+          shared_words<16>(step[h] + place(r, 2 * t), k[i]);
+          shared_words<16>(step[h] + place(r, 2 * t + 1), k[i] + 4);
+        }
+      }
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const uint32_t x0 = k[h][0][w] ^ 0x80808080u, x1 = k[h][1][w] ^ 0x80808080u;
+        const uint32_t x0 = k[0][w] ^ 0x80808080u, x1 = k[1][w] ^ 0x80808080u;
         const uint32_t op[4] = {half_lo(x0), half_lo(x1), half_hi(x0), half_hi(x1)};
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
@@ -263,10 +282,16 @@ struct Warp {
         }
   }
 
-  __device__ __forceinline__ void outputs(const float (&z)[HT][NQ][4]) {
+  __device__ __forceinline__ void outputs(const float (&z)[HT][NQ][4], const uint32_t (&step)[HT], int lane) {
 #pragma unroll
     for (int h = 0; h < HT; ++h) {
-      uint32_t b[NQ][WP][2];
+      uint32_t b[NQ][WP][2], v[4][VW];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        constexpr int VB = D / 8;  // bytes of a token's row that a lane needs
+        const int r = 2 * (lane & 3) + (i & 1) + 8 * (i >> 1), at = (lane >> 2) * VB;
+        shared_words<VB>(step[h] + 16 * D + place(r, at >> 4) + (at & 15), v[i]);
+      }
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -278,8 +303,8 @@ struct Warp {
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
         // four tokens' words -> for each element the pairs (token 2t, 2t + 1) and (2t + 8, 2t + 9)
-        const uint32_t x0 = v[h][0][w] ^ 0x80808080u, x1 = v[h][1][w] ^ 0x80808080u;
-        const uint32_t x2 = v[h][2][w] ^ 0x80808080u, x3 = v[h][3][w] ^ 0x80808080u;
+        const uint32_t x0 = v[0][w] ^ 0x80808080u, x1 = v[1][w] ^ 0x80808080u;
+        const uint32_t x2 = v[2][w] ^ 0x80808080u, x3 = v[3][w] ^ 0x80808080u;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const uint32_t y0 = prmt(x0, x1, c ? 0x7362 : 0x5140), y1 = prmt(x2, x3, c ? 0x7362 : 0x5140);
@@ -311,6 +336,65 @@ struct Warp {
   }
 };
 
+__device__ __forceinline__ int cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return (int)n;
+}
+
+// joins the sums of a cluster's CTAs (each the four warps' O in `so`, M and l in
+// sm and sl) and writes the item's rows; the formula is join_kernel's
+template <typename T, int D, int NQ>
+__device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, int tile, int kvh, int b, int f, float *so,
+                                             float (*sm)[8 * NQ], float (*sl)[8 * NQ]) {
+  constexpr int R = 8 * NQ, PAD = D + 4;
+  __shared__ float mine[3][R];  // M, M - f, l
+  const int tid = threadIdx.x, size = cluster_size(), rank = (int)cluster_ctarank();
+  for (int x = tid; x < R * (D / 4); x += THREADS) {  // the four warps' O into the first one's place
+    float4 *y = reinterpret_cast<float4 *>(so + x / (D / 4) * PAD + x % (D / 4) * 4);
+    constexpr int Q = R * PAD / 4;
+    const float4 v0 = y[0], v1 = y[Q], v2 = y[2 * Q], v3 = y[3 * Q];
+    y[0] = make_float4((v0.x + v1.x) + (v2.x + v3.x), (v0.y + v1.y) + (v2.y + v3.y), (v0.z + v1.z) + (v2.z + v3.z),
+                       (v0.w + v1.w) + (v2.w + v3.w));
+  }
+  if (tid < R) {
+    const float m = fmaxf(fmaxf(sm[0][tid], sm[1][tid]), fmaxf(sm[2][tid], sm[3][tid]));
+    float l = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) l = fmaf(sl[i][tid], ex2(sm[i][tid] - m), l);
+    mine[0][tid] = m;
+    mine[1][tid] = m > LOWEST ? m - (float)(f - 127) : LOWEST;
+    mine[2][tid] = l;
+  }
+  cluster_sync();
+  const int work = R * (D / 4), x0 = rank * work / size, x1 = (rank + 1) * work / size;
+  for (int x = x0 + tid; x < x1; x += THREADS) {
+    const int r = x / (D / 4), d = x % (D / 4) * 4, rho = tile * R + r;
+    if (rho >= s.n * a.G) continue;
+    float mg = LOWEST, ag = LOWEST, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < size; ++c) {
+      mg = fmaxf(mg, ld_dsmem_f32(dsmem_addr(&mine[0][r], c)));
+      ag = fmaxf(ag, ld_dsmem_f32(dsmem_addr(&mine[1][r], c)));
+    }
+#pragma unroll 2
+    for (int c = 0; c < size; ++c) {
+      const float m = ld_dsmem_f32(dsmem_addr(&mine[0][r], c)), af = ld_dsmem_f32(dsmem_addr(&mine[1][r], c));
+      const uint4 v = ld_dsmem_v4(dsmem_addr(so + r * PAD + d, c));
+      const float w = ex2(m - mg);
+      l = fmaf(ld_dsmem_f32(dsmem_addr(&mine[2][r], c)), m > LOWEST ? ex2(af - ag) : 1.f, l);
+      y[0] = fmaf(u2f(v.x), w, y[0]);
+      y[1] = fmaf(u2f(v.y), w, y[1]);
+      y[2] = fmaf(u2f(v.z), w, y[2]);
+      y[3] = fmaf(u2f(v.w), w, y[3]);
+    }
+    const float w = l == 0.f ? 0.f : (mg > LOWEST ? ex2(mg - ag) : 1.f) / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] *= w;
+    store4<T>(static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D + d, y);
+  }
+  cluster_sync();  // this CTA's sums are read until here
+}
+
 template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kernel(AttnArgs a) {
   constexpr int R = 8 * NQ, PAD = D + 4;
@@ -319,7 +403,8 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
   __shared__ int found;
   __shared__ long long found_at;
   __shared__ Seq found_seq;
-  __shared__ float so[R * PAD], sm[WARPS][R], sl[WARPS][R];
+  __shared__ float sm[WARPS][R], sl[WARPS][R];
+  extern __shared__ __align__(16) uint8_t ring[];  // [WARPS][STAGES][HT] steps; then the warps' O [WARPS][R][PAD]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const long long cta = blockIdx.x;
 
@@ -371,17 +456,21 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
     kvh = (int)(item % a.c.KV);
     tile = (int)(item / a.c.KV);
   } else {
-    kvh = (int)(cta % a.c.KV);
-    tile = (int)(cta / a.c.KV % a.tiles);
-    b = (int)(cta / a.c.KV / a.tiles);
+    const int size = cluster_size(), item = (int)(cta / size), rank = (int)(cta % size);
+    kvh = item % a.c.KV;
+    tile = item / a.c.KV % a.tiles;
+    b = item / a.c.KV / a.tiles;
     s = seq_of<NQ>(a, b);
-    if (tile >= s.tiles) return;
-    u = 0;
-    lo = 0;
-    hi = s.units;
+    if (tile >= s.tiles) return;  // the whole cluster
+    lo = (long long)rank * s.units / size;
+    hi = (long long)(rank + 1) * s.units / size;
+    u = (int)lo;
   }
 
-  Warp<T, D, NQ> w;
+  using W = Warp<T, D, NQ>;
+  W w;
+  const uint32_t mine = smem_u32(ring) + warp * (STAGES * HT * W::STEP);
+  float *so = reinterpret_cast<float *>(ring);
   long long at = lo;
   do {
     // one segment: units [u, u1) of item (b, tile, kvh)
@@ -406,22 +495,20 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
         meta.off[tid] = max(id, 0) * a.c.page_stride + head;
       }
       __syncthreads();
-      int en[HT];
-      long long off[HT];
-      // pages and code offsets of the warp's tiles in unit c
-      auto locate = [&](int c) {
+      // fetches the warp's tiles of unit c, if the chunk has it, into their ring steps
+      auto fetch = [&](int c) {
+        if (c < c1) {
 #pragma unroll
-        for (int h = 0; h < HT; ++h) {
-          const int j = (s.u0 + c) * UNIT + warp * WTOK + 16 * h;
-          en[h] = (j >> a.c.lg_page) - o0;
-          off[h] = meta.off[en[h]] + (j & (a.c.page - 1)) * D;
+          for (int h = 0; h < HT; ++h) {
+            const int j = (s.u0 + c) * UNIT + warp * WTOK + 16 * h;
+            w.fetch(a, mine + ((c - c0) % STAGES * HT + h) * W::STEP,
+                    meta.off[(j >> a.c.lg_page) - o0] + (j & (a.c.page - 1)) * D, lane);
+          }
         }
+        copy_commit();
       };
-      locate(c0);
 #pragma unroll
-      for (int h = 0; h < HT; ++h) w.load_k(a, h, off[h], lane);
-#pragma unroll
-      for (int h = 0; h < HT; ++h) w.load_v(a, h, off[h], lane);
+      for (int i = 0; i < STAGES - 1; ++i) fetch(c0 + i);
       int ek = 0, ev = 0;
       if (id >= 0) {
         ek = a.c.k_exp[id * a.c.exp_stride + kvh];
@@ -454,24 +541,24 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
       for (int c = c0; c < c1; ++c) {
         float z[HT][NQ][4];
         float4 e[HT];
+        uint32_t step[HT];
+        const int j = (s.u0 + c) * UNIT + warp * WTOK;
 #pragma unroll
-        for (int h = 0; h < HT; ++h) e[h] = meta.s[en[h]];
-        w.scores(z);
-        if (c + 1 < c1) {
-          locate(c + 1);
-#pragma unroll
-          for (int h = 0; h < HT; ++h) w.load_k(a, h, off[h], lane);
+        for (int h = 0; h < HT; ++h) {
+          e[h] = meta.s[((j + 16 * h) >> a.c.lg_page) - o0];
+          step[h] = mine + ((c - c0) % STAGES * HT + h) * W::STEP;
         }
-        w.weights(a, e, z, (s.u0 + c) * UNIT + warp * WTOK, lane, p_min, p_max);
-        w.outputs(z);
-        if (c + 1 < c1) {
-#pragma unroll
-          for (int h = 0; h < HT; ++h) w.load_v(a, h, off[h], lane);
-        }
+        copy_wait<STAGES - 2>();
+        __syncwarp();  // every lane's copies of this step are there, and its reads of the last one done
+        w.scores(z, step, lane);
+        fetch(c + STAGES - 1);  // into the step that the last iteration read
+        w.weights(a, e, z, j, lane, p_min, p_max);
+        w.outputs(z, step, lane);
       }
+      copy_wait<0>();
     }
     if (u == u1) w.start(a, s, tile, kvh, lane);  // an item without units: rows of zeros
-    // the warps' sums: a common M, then O added warp after warp
+    // the warps' sums, brought to a common M
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -484,23 +571,21 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
         }
       }
     __syncthreads();
-    for (int x = 0; x < WARPS; ++x) {
-      if (warp == x) {
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = 8 * n + 2 * t + i;
-            const float f = ex2(w.m[n][i] - fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])));
+      for (int i = 0; i < 2; ++i) {
+        const int r = 8 * n + 2 * t + i;
+        const float f = ex2(w.m[n][i] - fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])));
 #pragma unroll
-            for (int c = 0; c < Warp<T, D, NQ>::MT; ++c) {
-              float *d = so + r * PAD + g * (D / 8) + 2 * c;
-              d[0] = (x ? d[0] : 0.f) + w.o[n][c][i] * f;
-              d[1] = (x ? d[1] : 0.f) + w.o[n][c][i + 2] * f;
-            }
-          }
+        for (int c = 0; c < W::MT; ++c)
+          *reinterpret_cast<float2 *>(so + (warp * R + r) * PAD + g * (D / 8) + 2 * c) =
+              make_float2(w.o[n][c][i] * f, w.o[n][c][i + 2] * f);
       }
-      __syncthreads();
+    __syncthreads();
+    if (!a.split && cluster_size() > 1) {
+      join_cluster<T, D, NQ>(a, s, tile, kvh, b, f, so, sm, sl);
+      return;
     }
     const bool whole = u == 0 && u1 == s.units;
     float *rec = whole ? nullptr : a.part + (cta * 2 + (u == 0 ? 1 : 0)) * (size_t)(R * (D + 3));
@@ -514,7 +599,8 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
       for (int i = 0; i < WARPS; ++i) l = fmaf(sl[i][r], ex2(sm[i][r] - mx), l);
       float y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = so[r * PAD + d + i];
+      for (int i = 0; i < 4; ++i)
+        y[i] = (so[r * PAD + d + i] + so[(R + r) * PAD + d + i]) + (so[(2 * R + r) * PAD + d + i] + so[(3 * R + r) * PAD + d + i]);
       if (whole) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = l == 0.f ? 0.f : y[i] / l * top;
@@ -532,7 +618,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
       // the item ends at line index base + its units; the CTA that holds its last one
       const long long end = at + s.units;
       a.desc[((size_t)b * a.tiles + tile) * a.c.KV + kvh] = make_int2((int)cta, (int)((end * grid - 1) / total));
-    } else if (whole && a.split && tid == 0) {
+    } else if (a.split && whole && tid == 0) {
       a.desc[((size_t)b * a.tiles + tile) * a.c.KV + kvh] = make_int2((int)cta, (int)cta);
     }
     at += u1 - u;
@@ -634,11 +720,14 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
 }
 
 struct Plan {
-  int nq, tiles, split, grid;
+  int nq, tiles, split, cluster, grid;
   size_t desc, bytes;
 };
 
-// row tile: 8 rows, or 16 when a sequence has more (32 spill registers)
+// row tile: 8 rows, or 16 when a sequence has more (32 spill registers).
+// A cluster an item where one wave holds every item's CTAs and a CTA has at
+// most 16 units (1024 tokens) to go through; the even cut with its second
+// kernel otherwise.
 Plan plan_of(const Pool &c, int width, int B, int most, int H, int window, int sms) {
   Plan p;
   const long long rows = (long long)most * (H / c.KV);
@@ -647,8 +736,10 @@ Plan plan_of(const Pool &c, int width, int B, int most, int H, int window, int s
   long long len = (long long)width << c.lg_page;
   if (window > 0) len = std::min(len, (long long)window + most + UNIT);
   const long long units = (len + UNIT - 1) / UNIT, items = (long long)B * c.KV * p.tiles;
-  p.split = units > 1;
-  p.grid = (int)std::min<long long>(p.split ? std::min<long long>(items * units, (long long)(p.nq == 1 ? RES1 : RES2) * sms) : items, 0x7fffffff);
+  const long long wave = (long long)(p.nq == 1 ? RES1 : RES2) * sms;
+  p.cluster = units >= 8 ? 8 : units >= 4 ? 4 : units >= 2 ? 2 : 1;
+  p.split = p.cluster > 1 && (items * p.cluster > wave || units > 16 * p.cluster);
+  p.grid = (int)std::min<long long>(p.split ? std::min(items * units, wave) : items * p.cluster, 0x7fffffff);
   p.desc = p.split ? ((size_t)items * sizeof(int2) + 255) / 256 * 256 : 0;
   p.bytes = p.split ? p.desc + (size_t)p.grid * 2 * 8 * p.nq * (c.D + 3) * sizeof(float) : 0;
   return p;
@@ -656,17 +747,28 @@ Plan plan_of(const Pool &c, int width, int B, int most, int H, int window, int s
 
 template <typename T, int D, int NQ>
 void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {
-  attention_kernel<T, D, NQ><<<p.grid, THREADS, 0, st>>>(a);
-  if (!p.split) return;
-  // started while the last CTAs of the first kernel run; it waits for their records
+  constexpr int smem = std::max(WARPS * STAGES * HT * Warp<T, D, NQ>::STEP, (int)sizeof(float) * WARPS * 8 * NQ * (D + 4));
+  if (smem > 40 * 1024) cudaFuncSetAttribute(attention_kernel<T, D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(8 * NQ * a.c.KV * a.tiles, a.r.B);
+  cfg.gridDim = dim3(p.grid);
   cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = &attr;
+  if (!p.split && p.cluster > 1) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = p.cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  cudaLaunchKernelEx(&cfg, attention_kernel<T, D, NQ>, a);
+  if (!p.split) return;
+  // started while the last CTAs of the first kernel run; it waits for their records
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(8 * NQ * a.c.KV * a.tiles, a.r.B);
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, join_kernel<T, D, NQ>, a);
 }

@@ -59,17 +59,23 @@ __device__ __forceinline__ float fp16_range(float amax) {
   return __uint_as_float((uint32_t)(min(13 + 127 - e, 126) + 127) << 23);
 }
 
+// 16 bytes from global to shared memory, asynchronously
+__device__ __forceinline__ void copy_async16(uint32_t dst, const int8_t *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 template <int BYTES>
-__device__ __forceinline__ void load_words(const int8_t *p, uint32_t *w) {
-  if constexpr (BYTES == 16) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else if constexpr (BYTES == 8) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
-  }
+__device__ __forceinline__ void shared_words(uint32_t src, uint32_t *w) {
+  if constexpr (BYTES == 16)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src) : "memory");
+  else if constexpr (BYTES == 8)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(src) : "memory");
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(src) : "memory");
 }
 
 }  // namespace kv8

@@ -29,7 +29,6 @@ The reference has no counterpart: its cache is one fp32 array per layer
 from __future__ import annotations
 
 import ctypes as C
-import math
 
 import torch
 
@@ -53,7 +52,8 @@ class KV8Cache:
     multiple of 16 bytes, the same for k and v); within a page the layout is
     contiguous."""
 
-    __slots__ = ("k", "v", "k_exp", "v_exp", "device", "pages", "kv_heads", "page", "head_dim", "_c", "_ref")
+    __slots__ = ("k", "v", "k_exp", "v_exp", "device", "pages", "kv_heads", "page", "head_dim", "_c", "_ref",
+                 "_scratch")
 
     def __init__(self, k, v, k_exp, v_exp):
         if k.dim() != 4 or v.shape != k.shape or k.dtype != torch.int8 or v.dtype != torch.int8:
@@ -80,6 +80,7 @@ class KV8Cache:
         self._c = _KV8(k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), stride,
                        k_exp.stride(0) if pages > 1 else kv, pages, page, kv, d)
         self._ref = C.byref(self._c)
+        self._scratch = {}  # workspace bytes of attention calls, by their sizes
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page: int = 64, device=None) -> "KV8Cache":
@@ -97,11 +98,11 @@ class KV8Cache:
 
 def _rows(cache, n, table, pos, starts, max_tokens):
     """Checks the row description; (width, B, max_tokens, starts pointer)."""
-    dev = cache.device
-    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.device != dev:
+    dev, i32 = cache.device, torch.int32
+    if table.dim() != 2 or table.dtype is not i32 or not table.is_contiguous() or table.device != dev:
         raise ValueError("table must be a contiguous int32 [B, pages] tensor on the cache's device")
     b, width = table.shape
-    if pos.shape != (b,) or pos.dtype != torch.int32 or not pos.is_contiguous() or pos.device != dev:
+    if pos.dim() != 1 or len(pos) != b or pos.dtype is not i32 or not pos.is_contiguous() or pos.device != dev:
         raise ValueError("pos must be a contiguous int32 [B] tensor on the cache's device")
     if b == 0 or width == 0:
         raise ValueError("table must hold at least one sequence and one page")
@@ -121,8 +122,6 @@ def _rows(cache, n, table, pos, starts, max_tokens):
 
 
 def _out(out, shape, dtype, device):
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
     if out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous, 16-byte aligned {dtype} tensor of shape {tuple(shape)}")
@@ -162,7 +161,7 @@ def kv8_append(qkv, cache: KV8Cache, table, pos, cos, sin, bias=None, starts=Non
                              or bias.device != dev):
         raise ValueError("bias must be a contiguous fp32 tensor of qkv's width")
     width, b, most, sp = _rows(cache, n, table, pos, starts, max_tokens)
-    q = _out(out, (n, heads, d), qkv.dtype, dev)
+    q = qkv.new_empty((n, heads, d)) if out is None else _out(out, (n, heads, d), qkv.dtype, dev)
     if n == 0:
         return q
     if torch.cuda.current_device() != dev.index:
@@ -182,7 +181,7 @@ def kv8_attention(q, cache: KV8Cache, table, pos, starts=None, max_tokens: int |
     q's type. The row at position p sees positions p - window + 1 .. p (all up
     to p without a window); scale defaults to 1/sqrt(D). Rows that see nothing
     are 0."""
-    kv, d, dev = cache.kv_heads, cache.head_dim, cache.device
+    kv, d, dev, L = cache.kv_heads, cache.head_dim, cache.device, lib()
     if q.dim() != 3 or q.dtype not in _DTYPES or q.device != dev or q.shape[2] != d:
         raise ValueError(f"q must be an fp32, bf16 or fp16 [N, H, {d}] tensor on the cache's device")
     n, heads, _ = q.shape
@@ -191,20 +190,28 @@ def kv8_attention(q, cache: KV8Cache, table, pos, starts=None, max_tokens: int |
     if window < 0:
         raise ValueError("window must not be negative")
     width, b, most, sp = _rows(cache, n, table, pos, starts, max_tokens)
-    y = _out(out, (n, heads, d), q.dtype, dev)
+    if out is None:
+        y = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, heads, d))
+    else:
+        y = _out(out, (n, heads, d), q.dtype, dev)
     if n == 0:
         return y
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
             return kv8_attention(q, cache, table, pos, starts, max_tokens, window, scale, y)
     q = _aligned_rows(q, (d, 1))
-    dt, L = _DTYPES[q.dtype], lib()
-    nb = L.lbc_kv8_attention_workspace(cache._ref, dt, width, b, n, most, heads, window)
+    dt = _DTYPES[q.dtype]
+    sizes = (width, b, most, heads, window)
+    nb = cache._scratch.get(sizes)
+    if nb is None:
+        nb = cache._scratch[sizes] = L.lbc_kv8_attention_workspace(cache._ref, dt, width, b, n, most, heads, window)
     # from torch's allocator: private to this call in stream order, and to a graph when captured
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-    _check(L.lbc_kv8_attention(cache._ref, dt, q.data_ptr(), q.stride(0), table.data_ptr(), width, pos.data_ptr(), sp,
-                               b, n, most, heads, window, 1.0 / math.sqrt(d) if scale is None else scale, y.data_ptr(),
-                               _ptr(ws), nb, _raw_stream(dev.index)), "lbc_kv8_attention")
+    rc = L.lbc_kv8_attention(cache._ref, dt, q.data_ptr(), q.stride(0), table.data_ptr(), width, pos.data_ptr(), sp,
+                             b, n, most, heads, window, d ** -0.5 if scale is None else scale, y.data_ptr(),
+                             _ptr(ws), nb, _raw_stream(dev.index))
+    if rc < 0:
+        _check(rc, "lbc_kv8_attention")
     return y
 
 
@@ -219,9 +226,13 @@ def kv8_read(cache: KV8Cache, pages, dtype=torch.bfloat16):
         raise ValueError("dtype must be torch.float32, bfloat16 or float16")
     n = pages.shape[0]
     shape = (n, cache.kv_heads, cache.page, cache.head_dim)
-    k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
-    if n:
+    k = torch.empty(shape, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    if n == 0:
+        return k, v
+    if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
-            _check(lib().lbc_kv8_read(cache._ref, _DTYPES[dtype], pages.data_ptr(), n, k.data_ptr(), v.data_ptr(),
-                                      _raw_stream(dev.index)), "lbc_kv8_read")
+            return kv8_read(cache, pages, dtype)
+    _check(lib().lbc_kv8_read(cache._ref, _DTYPES[dtype], pages.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+                              _raw_stream(dev.index)), "lbc_kv8_read")
     return k, v

@@ -33,8 +33,7 @@
 #include <cstdio>
 
 #include "kernels.h"
-#include "kv8.cuh"
-#include "kv8_mma.cuh"
+#include "kv8_attn.cuh"
 
 namespace lbc {
 namespace kv8 {
@@ -56,58 +55,10 @@ constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int WTOK = 16 * HT;       // tokens of a warp in a unit
 constexpr int UNIT = WARPS * WTOK;
 constexpr int META = 128;           // pages looked up at a time
-constexpr float LOWEST = -3e38f;    // M before any visible token
 // weights 2^(t - M) fill fp16's range: M is the maximum (rounded up) less 14,
 // left alone while no weight passes 2^15. Two pieces then hold a weight to 22
 // bits down to 2^-17 of the largest, one piece to 11 bits down to 2^-28.
 constexpr float HEAD = 14.f, SLACK = 15.f;
-// blocks whose value scale is 2^60 below the largest count with 2^(f - 60): they
-// only matter to l (an all-zero block has exponent 0)
-constexpr int FAR = 60;
-
-struct AttnArgs {
-  Pool c;
-  Rows r;
-  const void *q;
-  long long ld;
-  void *out;
-  int H, G, window;
-  float scale_log2;  // scale * log2(e)
-  int tiles;         // row tiles a sequence can have
-  int split;         // 0: a cluster an item
-  int2 *desc;        // [B][tiles][KV] first and last CTA of an item
-  float *part;       // [grid][2] records: O [8 NQ][D], then M, l, f [8 NQ] each
-};
-
-// the units and row tiles of sequence b
-struct Seq {
-  int r0, n, p0, u0, units, tiles;
-};
-template <int NQ>
-__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int b) {
-  Seq s;
-  seq_rows(a.r, b, s.r0, s.n);
-  s.p0 = a.r.pos[b];
-  const long long cap = (long long)a.r.width << a.c.lg_page;
-  long long last = (long long)s.p0 + s.n - 1;
-  if (s.n > 0 && last >= cap) {  // rows past the table see nothing
-    set_status(a.r.status, LBC_ERR_PAGE);
-    last = cap - 1;
-  }
-  int first = 0;
-  if (a.window > 0) first = max(0, max(s.p0, 0) - a.window + 1);
-  s.u0 = first / UNIT;
-  s.units = s.n > 0 && last >= first ? (int)last / UNIT - s.u0 + 1 : 0;
-  s.tiles = (s.n * a.G + 8 * NQ - 1) / (8 * NQ);
-  return s;
-}
-
-// position of row `rho` (token rho / G) of a sequence, -1 for rows that see
-// nothing; the rows that fill up the last tile (never stored) copy the last one
-__device__ __forceinline__ int row_pos(const AttnArgs &a, const Seq &s, int rho) {
-  const long long p = (long long)s.p0 + min(rho, s.n * a.G - 1) / a.G;
-  return p >= ((long long)a.r.width << a.c.lg_page) ? -1 : (int)p;
-}
 
 struct Meta {
   long long off[META];  // bytes to the block's codes (a page that does not exist: to page 0's)
@@ -117,10 +68,7 @@ struct Meta {
 
 template <typename T, int D, int NQ>
 struct Warp {
-  // fp16 pieces of queries and of weights: fp32 needs 22 bits of both; bf16 and
-  // fp16 queries are exact in one; fp16 outputs (11 bits) would show weights
-  // rounded to 11 bits (error 1.5 times the output's own), bf16 ones do not
-  static constexpr int QP = sizeof(T) == 4 ? 2 : 1, WP = is_bf16<T> ? 1 : 2;
+  static constexpr int QP = QUERY_PIECES<T>, WP = WEIGHT_PIECES<T>;
   static constexpr int KW = D / 16, VW = D / 32, MT = D / 16;
   uint32_t q[NQ][QP][KW][2];  // query operand
   float rowf[NQ][2];              // score = accumulator * rowf * 2^(ek - 127), in log2 units
@@ -416,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
     const int per = (a.r.B + THREADS - 1) / THREADS, b0 = min(tid * per, a.r.B), b1 = min(b0 + per, a.r.B);
     long long mine = 0;
     for (int i = b0; i < b1; ++i) {
-      const Seq x = seq_of<NQ>(a, i);
+      const Seq x = seq_of<UNIT, 8 * NQ>(a, i);
       mine += (long long)x.units * x.tiles * a.c.KV;
     }
     long long upto = mine;
@@ -436,10 +384,10 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
     if (lo < upto && lo >= upto - mine) {
       long long x0 = upto - mine;
       int i = b0;
-      Seq x = seq_of<NQ>(a, i);
+      Seq x = seq_of<UNIT, 8 * NQ>(a, i);
       while (i < b1 - 1 && lo >= x0 + (long long)x.units * x.tiles * a.c.KV) {
         x0 += (long long)x.units * x.tiles * a.c.KV;
-        x = seq_of<NQ>(a, ++i);
+        x = seq_of<UNIT, 8 * NQ>(a, ++i);
       }
       found = i;
       found_at = x0;
@@ -460,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
     kvh = item % a.c.KV;
     tile = item / a.c.KV % a.tiles;
     b = item / a.c.KV / a.tiles;
-    s = seq_of<NQ>(a, b);
+    s = seq_of<UNIT, 8 * NQ>(a, b);
     if (tile >= s.tiles) return;  // the whole cluster
     lo = (long long)rank * s.units / size;
     hi = (long long)(rank + 1) * s.units / size;
@@ -630,7 +578,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
         tile = 0;
         do {
           if (++b == a.r.B) return;  // (lengths changed under the call)
-          s = seq_of<NQ>(a, b);
+          s = seq_of<UNIT, 8 * NQ>(a, b);
         } while (s.units == 0);
       }
     }
@@ -652,7 +600,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int r = blockIdx.x % R, kvh = blockIdx.x / R % a.c.KV, tile = blockIdx.x / R / a.c.KV, b = blockIdx.y;
   const int tid = threadIdx.x, col = tid % C, slice = tid / C, rho = tile * R + r;
-  const Seq s = seq_of<NQ>(a, b);
+  const Seq s = seq_of<UNIT, 8 * NQ>(a, b);
   if (rho >= s.n * a.G) return;
   T *dst = static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D + 4 * col;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -719,8 +667,11 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
   store4<T>(dst, out);
 }
 
+#ifndef PROMPT_ROWS
+#define PROMPT_ROWS 128
+#endif
 struct Plan {
-  int nq, tiles, split, cluster, grid;
+  int prompt, nq, tiles, split, cluster, grid;
   size_t desc, bytes;
 };
 
@@ -729,8 +680,10 @@ struct Plan {
 // most 16 units (1024 tokens) to go through; the even cut with its second
 // kernel otherwise.
 Plan plan_of(const Pool &c, int width, int B, int most, int H, int window, int sms) {
-  Plan p;
+  Plan p{};
   const long long rows = (long long)most * (H / c.KV);
+  p.prompt = rows >= PROMPT_ROWS;
+  if (p.prompt) return p;
   p.nq = rows <= 8 ? 1 : 2;
   p.tiles = (int)((rows + 8 * p.nq - 1) / (8 * p.nq));
   long long len = (long long)width << c.lg_page;
@@ -813,6 +766,7 @@ int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, 
   if (dtype < LBC_F32 || dtype > LBC_F16) return refuse("kv8_attention: dtype must be fp32, bf16 or fp16");
   if (H <= 0 || H % a.c.KV || H > 65535 || (long long)max_tokens * H > 0x7fffffff)
     return refuse("kv8_attention: H must be a multiple of the KV heads");
+  if ((long long)max_tokens * (H / a.c.KV) > 255LL * 65535) return refuse("kv8_attention: too many rows a sequence");
   if (N == 0 || max_tokens == 0) return 0;
   if (!q || !out) return refuse("kv8_attention: NULL argument");
   if (ld < (long long)H * a.c.D || ld * (dtype == LBC_F32 ? 4 : 2) % 16) return refuse("kv8_attention: bad row stride");
@@ -828,7 +782,8 @@ int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, 
   a.desc = static_cast<int2 *>(workspace);
   a.part = p.split ? reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + p.desc) : nullptr;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == LBC_F32) launch<float>(a, p, st);
+  if (p.prompt) launch_prompt(a, dtype, st);
+  else if (dtype == LBC_F32) launch<float>(a, p, st);
   else if (dtype == LBC_BF16) launch<__nv_bfloat16>(a, p, st);
   else launch<__half>(a, p, st);
   return launched("kv8_attention");

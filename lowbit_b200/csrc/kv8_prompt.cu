@@ -1,0 +1,480 @@
+// Causal grouped-query attention over the paged 8-bit KV cache for many rows
+// (prompts and prompt chunks), on tcgen05.
+//
+// A CTA takes 256 rows (token t, head g of the group: row t G + g) of one
+// sequence and KV head as two tiles of 128, and runs through the visible tokens
+// 64 at a time:
+//   warps 8-11  codes from global memory to fp16 operand tiles in shared memory
+//               (exact; keys K-major as they lie, values transposed 8 x 8 in
+//               registers), one conversion for both row tiles; block scales
+//   warp 12     S = Q K^T (both operands in shared memory) and O += P V (P, fp16,
+//               in tensor memory where S was), the scores of step j + 1 before
+//               the outputs of step j, so that the tensor cores work while the
+//               weights of a step are computed
+//   warps 0-7   a thread a row: scores from tensor memory, scale, mask, running
+//               reference M, weights 2^(t - M), sums l; O is rescaled only when a
+//               row's maximum has risen by more than 2^3
+// Scales, M, l and f are those of the few-row kernel (kv8_attention.cu); queries
+// are scaled into fp16's range per row, fp32 ones in two pieces, and weights of
+// fp32 and fp16 calls in two pieces (twice the products).
+#include <algorithm>
+#include <cstdio>
+
+#include "kernels.h"
+#include "kv8_attn.cuh"
+#include "tc.cuh"
+
+namespace lbc {
+namespace kv8 {
+namespace {
+
+constexpr int NT = 64;        // tokens a step
+constexpr int TILE = 128;     // rows of a row tile
+constexpr int ROWS = 2 * TILE;
+constexpr int W_DEQ = 8, W_MMA = 12, THREADS = 13 * 32;
+constexpr int META = 8;       // steps whose block scales are kept
+// weights: M is the maximum (rounded up) less 12, left alone up to 2^15
+constexpr float HEAD = 12.f, SLACK = 15.f;
+
+struct StepMeta {
+  float4 g[NT / 16];  // of each 16 tokens: 2^(ek - 127), b = ev - 127, 2^(f - b), 1 if the page exists
+  int f, pad[3];
+};
+
+struct Shared {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], meta_full[META], q_full, fin;
+  uint32_t tmem;
+  int abort;
+  StepMeta meta[META];
+};
+
+// operand tiles, in bytes. K-major without swizzle: 8 rows x 16 bytes are one
+// core matrix; LBO steps along K, SBO along the rows. The strides carry a
+// pad that spreads a warp's stores over the banks.
+template <typename T, int D>
+struct Lay {
+  static constexpr int QP = QUERY_PIECES<T>, WP = WEIGHT_PIECES<T>;
+  static constexpr int Q_LBO = TILE / 8 * 128, Q_BYTES = D / 8 * Q_LBO;
+  static constexpr int K_LBO = NT / 8 * 128 + 16 * (128 / D), K_BYTES = D / 8 * K_LBO;
+  static constexpr int V_SBO = 144, V_LBO = D / 8 * V_SBO, V_BYTES = NT / 8 * V_LBO;
+  static constexpr int K_OFF = 2 * QP * Q_BYTES, V_OFF = K_OFF + 2 * K_BYTES, S_OFF = (V_OFF + 2 * V_BYTES + 127) / 128 * 128;
+  static constexpr int SMEM = S_OFF + (int)sizeof(Shared);
+  // position along K of the 8 elements from 16 c + 8 h on (the order is free, and the same in Q and K)
+  __device__ static int chunk(int c, int h) { return h * (D / 16) + c; }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
+  using L = Lay<T, D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  Shared &sh = *reinterpret_cast<Shared *>(smem + L::S_OFF);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kvh = blockIdx.x, b = blockIdx.y, tile = gridDim.z - 1 - blockIdx.z;  // late rows, the longest, first
+  const Seq s = seq_of<NT, ROWS>(a, b);
+  if (tile >= s.tiles) return;
+  const int rho0 = tile * ROWS, rho1 = min(rho0 + ROWS, s.n * a.G) - 1;
+  const long long cap = (long long)a.r.width << a.c.lg_page;
+  const long long p_first = max((long long)s.p0 + rho0 / a.G, 0LL), p_last = min((long long)s.p0 + rho1 / a.G, cap - 1);
+  const long long see0 = a.window > 0 ? max(0LL, p_first - a.window + 1) : 0;
+  const int t0 = (int)(see0 / NT), steps = p_last >= see0 ? (int)(p_last / NT) - t0 + 1 : 0;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.k_full[i], 128);
+      mbar_init(&sh.v_full[i], 128);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.pv_done[i], 1);
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&sh.s_full[i][j], 1);
+        mbar_init(&sh.p_full[i][j], 128);
+      }
+    }
+    for (int i = 0; i < META; ++i) mbar_init(&sh.meta_full[i], 1);
+    mbar_init(&sh.q_full, 256);
+    mbar_init(&sh.fin, 1);
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == W_MMA) {
+    tc::alloc(&sh.tmem, 512);
+    tc::relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = sh.tmem, base = smem_u32(smem);
+  volatile int *abort = &sh.abort;
+  // a wait of a whole warp: every lane goes on, or (time limit, recorded) none
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    const bool ok = !*abort && mbar_wait(bar, parity, a.r.status);
+    if (__all_sync(0xffffffffu, ok)) return true;
+    *abort = 1;
+    return false;
+  };
+  // tensor memory: S (and P in its place) of row tile i, buffer j; O of row tile i
+  auto s_col = [&](int i, int j) { return tmem + (2 * i + j) * NT; };
+  auto o_col = [&](int i) { return tmem + 4 * NT + i * D; };
+
+  if (warp == W_MMA) {
+    // ------------------------------------------------------------ products
+    if (lane == 0 && steps > 0 && mbar_wait(&sh.q_full, 0, a.r.status)) {
+      const uint64_t qd = tc::smem_desc(base, L::Q_LBO, 128);
+      for (int j = 0; j <= steps && !*abort; ++j) {
+        if (j < steps) {
+          const int st = j & 1;
+          if (!mbar_wait(&sh.k_full[st], (j >> 1) & 1, a.r.status)) {
+            *abort = 1;
+            break;
+          }
+          tc::fence_after_sync();
+          const uint64_t kd = tc::smem_desc(base + L::K_OFF + st * L::K_BYTES, L::K_LBO, 128);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+              for (int c = 0; c < L::QP; ++c)
+                tc::mma_f16_ss(s_col(i, st), qd + (uint64_t)((i * L::QP + c) * L::Q_BYTES + 2 * k * L::Q_LBO) / 16,
+                               kd + (uint64_t)(2 * k * L::K_LBO) / 16, tc::idesc_f16_f32(NT), k + c > 0);
+            tc::commit(&sh.s_full[i][st]);
+          }
+          tc::commit(&sh.k_empty[st]);
+        }
+        if (j > 0) {
+          const int st = (j - 1) & 1;
+          const uint32_t ph = ((j - 1) >> 1) & 1;
+          if (!mbar_wait(&sh.v_full[st], ph, a.r.status)) {
+            *abort = 1;
+            break;
+          }
+          const uint64_t vd = tc::smem_desc(base + L::V_OFF + st * L::V_BYTES, L::V_LBO, L::V_SBO);
+          bool ok = true;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            ok = ok && mbar_wait(&sh.p_full[i][st], ph, a.r.status);
+            if (!ok) break;
+            tc::fence_after_sync();
+#pragma unroll
+            for (int k = 0; k < NT / 16; ++k)
+#pragma unroll
+              for (int c = 0; c < L::WP; ++c)
+                tc::mma_bf16_ts(o_col(i), s_col(i, st) + 8 * k + NT / 2 * c, vd + (uint64_t)(2 * k * L::V_LBO) / 16,
+                                tc::idesc_f16_f32(D), j > 1 || k + c > 0);
+            tc::commit(&sh.pv_done[i]);
+          }
+          if (!ok) {
+            *abort = 1;
+            break;
+          }
+          tc::commit(&sh.v_empty[st]);
+        }
+      }
+      tc::commit(&sh.fin);
+      mbar_wait(&sh.fin, 0, a.r.status);
+    }
+  } else if (warp >= W_DEQ) {
+    // ------------------------------------------------------------ codes to operands
+    const int x = tid - W_DEQ * 32;  // 0 .. 127
+    constexpr int LR = D / 16, KP = D / 32;        // lanes a key row, 16-byte pieces a thread
+    constexpr int VB = D == 32 ? 4 : D / 16;       // bytes of a value row a thread transposes
+    constexpr int VL = D / VB, VW = VB / 4;        // lanes a value row
+    const bool v_live = x < 8 * VL;
+    const long long head = (long long)kvh * a.c.page * D;
+    // page of the 16 tokens from position j on; -1 when no row sees them or there is none
+    auto page_at = [&](int j) {
+      const int o = j >> a.c.lg_page;
+      return ((long long)(o + 1) << a.c.lg_page) > see0 && ((long long)o << a.c.lg_page) <= p_last ? page_id(a.c, a.r, b, o) : -1;
+    };
+    auto offset = [&](int id, int j) { return max(id, 0) * a.c.page_stride + head + (j & (a.c.page - 1)) * D; };
+    int kid[KP], vid, mid = -1, ek = 0, ev = 0, f = 0;
+    uint4 kx[KP];
+    uint32_t vx[8][VW];
+    auto look = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < KP; ++i) kid[i] = page_at((t0 + j) * NT + i * (128 / LR) + x / LR);
+      vid = page_at((t0 + j) * NT + min(x / VL, 7) * 8);
+      if (x < NT / 16) mid = page_at((t0 + j) * NT + x * 16);
+    };
+    auto load_k = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < KP; ++i)
+        kx[i] = __ldg(reinterpret_cast<const uint4 *>(a.c.k + offset(kid[i], (t0 + j) * NT + i * (128 / LR) + x / LR) + x % LR * 16));
+    };
+    auto load_v = [&](int j) {
+      const int8_t *src = a.c.v + offset(vid, (t0 + j) * NT + min(x / VL, 7) * 8) + x % VL * VB;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (VB == 8) {
+          const uint2 y = __ldg(reinterpret_cast<const uint2 *>(src + i * D));
+          vx[i][0] = y.x;
+          vx[i][1] = y.y;
+        } else {
+          vx[i][0] = __ldg(reinterpret_cast<const uint32_t *>(src + i * D));
+        }
+      }
+    };
+    auto load_scales = [&]() {
+      ek = ev = 0;
+      if (x < NT / 16 && mid >= 0) {
+        ek = a.c.k_exp[mid * a.c.exp_stride + kvh];
+        ev = a.c.v_exp[mid * a.c.exp_stride + kvh];
+      }
+    };
+    if (steps > 0) {
+      look(0);
+      load_k(0);
+      load_v(0);
+      load_scales();
+    }
+    for (int j = 0; j < steps; ++j) {
+      const int st = j & 1;
+      const uint32_t ph = (j >> 1) & 1;
+      const int mid_j = mid, ek_j = ek, ev_j = ev;
+      if (j + 1 < steps) look(j + 1);
+      if (!wait(&sh.k_empty[st], ph ^ 1u)) break;
+      if (warp == W_DEQ) {
+        // the step's block scales; f is the largest value exponent so far (255 left out)
+        int top = lane < NT / 16 && mid_j >= 0 && ev_j != 255 ? ev_j : 0;
+        f = max(f, __reduce_max_sync(0xffffffffu, top));
+        if (lane < NT / 16) {
+          const int at = max(ev_j, f - FAR);
+          sh.meta[j % META].g[lane] = make_float4(pow2_e8m0(ek_j), ev_j == 255 ? __uint_as_float(0x7fc00000u) : (float)(at - 127),
+                                                  ev_j == 255 ? 1.f : pow2_e8m0(127 + f - at), mid_j >= 0 ? 1.f : 0.f);
+          if (lane == 0) sh.meta[j % META].f = f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.meta_full[j % META]);
+      }
+      uint8_t *kt = smem + L::K_OFF + st * L::K_BYTES;
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        const int tok = i * (128 / LR) + x / LR, c = x % LR;
+        const uint32_t w[4] = {kx[i].x ^ 0x80808080u, kx[i].y ^ 0x80808080u, kx[i].z ^ 0x80808080u, kx[i].w ^ 0x80808080u};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<uint4 *>(kt + L::chunk(c, h) * L::K_LBO + tok / 8 * 128 + tok % 8 * 16) =
+              make_uint4(half_lo(w[2 * h]), half_hi(w[2 * h]), half_lo(w[2 * h + 1]), half_hi(w[2 * h + 1]));
+      }
+      tc::fence_proxy_async_smem();
+      mbar_arrive(&sh.k_full[st]);
+      if (j + 1 < steps) load_k(j + 1);
+      if (!wait(&sh.v_empty[st], ph ^ 1u)) break;
+      if (v_live) {
+        uint8_t *vt = smem + L::V_OFF + st * L::V_BYTES + x / VL * L::V_LBO;
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          uint32_t y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = vx[i][w] ^ 0x80808080u;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // elements 2 h and 2 h + 1 of the word, tokens in pairs
+            uint32_t z[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] = prmt(y[2 * i], y[2 * i + 1], h ? 0x7362 : 0x5140);
+            const int d = x % VL * VB + 4 * w + 2 * h;
+            uint8_t *dst = vt + d / 8 * L::V_SBO + d % 8 * 16;
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(half_lo(z[0]), half_lo(z[1]), half_lo(z[2]), half_lo(z[3]));
+            *reinterpret_cast<uint4 *>(dst + 16) = make_uint4(half_hi(z[0]), half_hi(z[1]), half_hi(z[2]), half_hi(z[3]));
+          }
+        }
+      }
+      tc::fence_proxy_async_smem();
+      mbar_arrive(&sh.v_full[st]);
+      if (j + 1 < steps) {
+        load_v(j + 1);
+        load_scales();
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ rows
+    const int i = warp >> 2, r = tid & (TILE - 1), rho = rho0 + i * TILE + r;
+    const bool live = rho < s.n * a.G;
+    const uint32_t quad = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
+    const int p = row_pos(a, s, rho);
+    const int p_min = __reduce_min_sync(0xffffffffu, p), p_max = __reduce_max_sync(0xffffffffu, p);
+    float rowf;
+    {
+      const T *src = static_cast<const T *>(a.q) + (s.r0 + min(rho, s.n * a.G - 1) / a.G) * a.ld +
+                     (size_t)(kvh * a.G + min(rho, s.n * a.G - 1) % a.G) * D;
+      float amax = 0.f;
+      for (int d = 0; d < D; d += 4) {
+        float y[4];
+        load4<T>(src + d, y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) amax = y[e] == y[e] ? fmaxf(amax, fabsf(y[e])) : INFINITY;
+      }
+      const float up = fp16_range(amax);
+      rowf = a.scale_log2 / up;
+      uint8_t *qt = smem + i * L::QP * L::Q_BYTES + r / 8 * 128 + r % 8 * 16;
+#pragma unroll 2
+      for (int d = 0; d < D; d += 8) {
+        float y[8];
+        load4<T>(src + d, reinterpret_cast<float(&)[4]>(y[0]));
+        load4<T>(src + d + 4, reinterpret_cast<float(&)[4]>(y[4]));
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y0 = y[2 * e] * up, y1 = y[2 * e + 1] * up;
+          hi[e] = pack_half(y0, y1);
+          if (L::QP == 2) lo[e] = pack_rest(y0, y1, hi[e]);
+        }
+        uint8_t *dst = qt + L::chunk(d / 16, d / 8 % 2) * L::Q_LBO;
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (L::QP == 2) *reinterpret_cast<uint4 *>(dst + L::Q_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      tc::fence_proxy_async_smem();
+      mbar_arrive(&sh.q_full);
+    }
+    float m = LOWEST, l = 0.f;
+    int f = 0;
+    bool ok = true;
+    for (int j = 0; j < steps; ++j) {
+      const int st = j & 1;
+      ok = wait(&sh.meta_full[j % META], (j / META) & 1) && wait(&sh.s_full[i][st], (j >> 1) & 1);
+      if (!ok) break;
+      tc::fence_after_sync();
+      uint32_t sv[4][16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) tc::ld16(s_col(i, st) + quad + 16 * g, sv[g]);
+      tc::wait_ld();
+      const StepMeta &meta = sh.meta[j % META];
+      const int pos0 = (t0 + j) * NT;
+      const bool inside = pos0 + NT - 1 <= p_min && (a.window <= 0 || pos0 > p_max - a.window);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 e = meta.g[g];
+        const float c = rowf * e.x;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float t = fmaf(u2f(sv[g][k]), c, e.y);
+          sv[g][k] = __float_as_uint(t);
+        }
+        if (!inside || e.w == 0.f) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const int at = pos0 + 16 * g + k;
+            if (!(at <= p && (a.window <= 0 || at > p - a.window) && e.w != 0.f)) sv[g][k] = __float_as_uint(-INFINITY);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, u2f(sv[g][k]));
+      }
+      // a larger f scales l; a much larger one also moves M (kv8_attention.cu: raise)
+      float by = 0.f;
+      if (meta.f > f) {
+        if (j > 0) {
+          by = (float)max(0, meta.f - f - 40);
+          l *= ex2((float)(meta.f - f) - by);
+        }
+        f = meta.f;
+      }
+      const bool rise = mx > m + SLACK;
+      if (__any_sync(0xffffffffu, rise) || by > 0.f) {
+        float to = m > LOWEST ? m + by : m;
+        float scale = ex2(-by);
+        const float up = fmaxf(to, ceilf(mx) - HEAD);
+        const float w = ex2(to - up);
+        l *= w;
+        scale *= w;
+        m = up;
+        if (j > 0) {
+          ok = wait(&sh.pv_done[i], (j - 1) & 1);
+          if (!ok) break;
+          tc::fence_after_sync();
+#pragma unroll
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tc::ld16(o_col(i) + quad + c, o);
+            tc::wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(u2f(o[k]) * scale);
+            tc::st16(o_col(i) + quad + c, o);
+          }
+        }
+      }
+      // weights, and P in the place of S (every thread has read its scores)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float back = meta.g[g].z;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float w = ex2(u2f(sv[g][k]) - m);
+          l = fmaf(w, back, l);
+          sv[g][k] = __float_as_uint(w);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float w0 = u2f(sv[2 * g + k / 8][2 * k % 16]), w1 = u2f(sv[2 * g + k / 8][2 * k % 16 + 1]);
+          hi[k] = pack_half(w0, w1);
+          if (L::WP == 2) lo[k] = pack_rest(w0, w1, hi[k]);
+        }
+        tc::st16(s_col(i, st) + quad + 16 * g, hi);
+        if (L::WP == 2) tc::st16(s_col(i, st) + quad + NT / 2 + 16 * g, lo);
+      }
+      tc::wait_st();
+      tc::fence_before_sync();
+      mbar_arrive(&sh.p_full[i][st]);
+    }
+    if (steps > 0 && ok) wait(&sh.pv_done[i], (steps - 1) & 1);
+    tc::fence_after_sync();
+    const float w = l == 0.f || steps == 0 ? 0.f : pow2_e8m0(f) / l;
+    T *dst = static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D;
+#pragma unroll 2
+    for (int c = 0; c < D; c += 16) {
+      uint32_t o[16];
+      if (steps > 0) {
+        tc::ld16(o_col(i) + quad + c, o);
+        tc::wait_ld();
+      }
+      if (live) {
+#pragma unroll
+        for (int k = 0; k < 16; k += 4) {
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = w == 0.f ? 0.f : u2f(o[k + e]) * w;
+          store4<T>(dst + c + k, y);
+        }
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == W_MMA) {
+    tc::fence_after_sync();
+    tc::dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int D>
+void launch(const AttnArgs &a, cudaStream_t st) {
+  constexpr int smem = Lay<T, D>::SMEM;
+  static_assert(smem <= 227 * 1024, "operand tiles fit an SM's shared memory");
+  cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  prompt_kernel<T, D><<<dim3(a.c.KV, a.r.B, a.tiles), THREADS, smem, st>>>(a);
+}
+template <typename T>
+void launch(const AttnArgs &a, cudaStream_t st) {
+  if (a.c.D == 32) launch<T, 32>(a, st);
+  else if (a.c.D == 64) launch<T, 64>(a, st);
+  else launch<T, 128>(a, st);
+}
+
+}  // namespace
+
+// a.tiles row tiles of ROWS rows at most
+void launch_prompt(const AttnArgs &a, int dtype, cudaStream_t st) {
+  AttnArgs b = a;
+  b.tiles = (int)(((long long)a.r.most * a.G + ROWS - 1) / ROWS);
+  if (dtype == LBC_F32) launch<float>(b, st);
+  else if (dtype == LBC_BF16) launch<__nv_bfloat16>(b, st);
+  else launch<__half>(b, st);
+}
+
+}  // namespace kv8
+}  // namespace lbc

@@ -766,7 +766,7 @@ int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, 
   if (dtype < LBC_F32 || dtype > LBC_F16) return refuse("kv8_attention: dtype must be fp32, bf16 or fp16");
   if (H <= 0 || H % a.c.KV || H > 65535 || (long long)max_tokens * H > 0x7fffffff)
     return refuse("kv8_attention: H must be a multiple of the KV heads");
-  if ((long long)max_tokens * (H / a.c.KV) > 255LL * 65535) return refuse("kv8_attention: too many rows a sequence");
+  if ((long long)max_tokens * (H / a.c.KV) > 128LL * 65535) return refuse("kv8_attention: too many rows a sequence");
   if (N == 0 || max_tokens == 0) return 0;
   if (!q || !out) return refuse("kv8_attention: NULL argument");
   if (ld < (long long)H * a.c.D || ld * (dtype == LBC_F32 ? 4 : 2) % 16) return refuse("kv8_attention: bad row stride");

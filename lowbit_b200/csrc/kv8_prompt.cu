@@ -2,7 +2,7 @@
 // (prompts and prompt chunks), on tcgen05.
 //
 // A CTA takes 256 rows (token t, head g of the group: row t G + g) of one
-// sequence and KV head as two tiles of 128, and runs through the visible tokens
+// sequence and KV head as two tiles of 128 (fp32 at D = 128: one), and runs through the visible tokens
 // 64 at a time:
 //   warps 8-11  codes from global memory to fp16 operand tiles in shared memory
 //               (exact; keys K-major as they lie, values transposed 8 x 8 in
@@ -30,7 +30,6 @@ namespace {
 
 constexpr int NT = 64;        // tokens a step
 constexpr int TILE = 128;     // rows of a row tile
-constexpr int ROWS = 2 * TILE;
 constexpr int W_DEQ = 8, W_MMA = 12, THREADS = 13 * 32;
 constexpr int META = 8;       // steps whose block scales are kept
 // weights: M is the maximum (rounded up) less 12, left alone up to 2^15
@@ -53,11 +52,16 @@ struct Shared {
 // pad that spreads a warp's stores over the banks.
 template <typename T, int D>
 struct Lay {
+  // row tiles of a CTA. Tensor cores add with truncation: over thousands of
+  // tokens that shows in fp32 outputs, so fp32 calls add O to a total (rounded
+  // to nearest, also in tensor memory) every FOLD steps; at D = 128 the total
+  // leaves room for one row tile.
+  static constexpr int FOLD = sizeof(T) == 4 ? 4 : 0, RT = FOLD && D == 128 ? 1 : 2, ROWS = RT * TILE;
   static constexpr int QP = QUERY_PIECES<T>, WP = WEIGHT_PIECES<T>;
   static constexpr int Q_LBO = TILE / 8 * 128, Q_BYTES = D / 8 * Q_LBO;
   static constexpr int K_LBO = NT / 8 * 128 + 16 * (128 / D), K_BYTES = D / 8 * K_LBO;
   static constexpr int V_SBO = 144, V_LBO = D / 8 * V_SBO, V_BYTES = NT / 8 * V_LBO;
-  static constexpr int K_OFF = 2 * QP * Q_BYTES, V_OFF = K_OFF + 2 * K_BYTES, S_OFF = (V_OFF + 2 * V_BYTES + 127) / 128 * 128;
+  static constexpr int K_OFF = RT * QP * Q_BYTES, V_OFF = K_OFF + 2 * K_BYTES, S_OFF = (V_OFF + 2 * V_BYTES + 127) / 128 * 128;
   static constexpr int SMEM = S_OFF + (int)sizeof(Shared);
   // position along K of the 8 elements from 16 c + 8 h on (the order is free, and the same in Q and K)
   __device__ static int chunk(int c, int h) { return h * (D / 16) + c; }
@@ -70,9 +74,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
   Shared &sh = *reinterpret_cast<Shared *>(smem + L::S_OFF);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.x, b = blockIdx.y, tile = gridDim.z - 1 - blockIdx.z;  // late rows, the longest, first
-  const Seq s = seq_of<NT, ROWS>(a, b);
+  const Seq s = seq_of<NT, L::ROWS>(a, b);
   if (tile >= s.tiles) return;
-  const int rho0 = tile * ROWS, rho1 = min(rho0 + ROWS, s.n * a.G) - 1;
+  const int rho0 = tile * L::ROWS, rho1 = min(rho0 + L::ROWS, s.n * a.G) - 1;
   const long long cap = (long long)a.r.width << a.c.lg_page;
   const long long p_first = max((long long)s.p0 + rho0 / a.G, 0LL), p_last = min((long long)s.p0 + rho1 / a.G, cap - 1);
   const long long see0 = a.window > 0 ? max(0LL, p_first - a.window + 1) : 0;
@@ -91,7 +95,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       }
     }
     for (int i = 0; i < META; ++i) mbar_init(&sh.meta_full[i], 1);
-    mbar_init(&sh.q_full, 256);
+    mbar_init(&sh.q_full, L::ROWS);
     mbar_init(&sh.fin, 1);
     sh.abort = 0;
     fence_mbar_init();
@@ -112,9 +116,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
     *abort = 1;
     return false;
   };
-  // tensor memory: S (and P in its place) of row tile i, buffer j; O of row tile i
+  // tensor memory: S (and P in its place) of row tile i, buffer j; O of row tile i; its total
   auto s_col = [&](int i, int j) { return tmem + (2 * i + j) * NT; };
-  auto o_col = [&](int i) { return tmem + 4 * NT + i * D; };
+  auto o_col = [&](int i) { return tmem + 2 * L::RT * NT + i * D; };
+  auto t_col = [&](int i) { return tmem + 2 * L::RT * NT + (L::RT + i) * D; };
 
   if (warp == W_MMA) {
     // ------------------------------------------------------------ products
@@ -130,7 +135,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
           tc::fence_after_sync();
           const uint64_t kd = tc::smem_desc(base + L::K_OFF + st * L::K_BYTES, L::K_LBO, 128);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < L::RT; ++i) {
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
 #pragma unroll
@@ -151,7 +156,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
           const uint64_t vd = tc::smem_desc(base + L::V_OFF + st * L::V_BYTES, L::V_LBO, L::V_SBO);
           bool ok = true;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < L::RT; ++i) {
             ok = ok && mbar_wait(&sh.p_full[i][st], ph, a.r.status);
             if (!ok) break;
             tc::fence_after_sync();
@@ -160,7 +165,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
 #pragma unroll
               for (int c = 0; c < L::WP; ++c)
                 tc::mma_bf16_ts(o_col(i), s_col(i, st) + 8 * k + NT / 2 * c, vd + (uint64_t)(2 * k * L::V_LBO) / 16,
-                                tc::idesc_f16_f32(D), j > 1 || k + c > 0);
+                                tc::idesc_f16_f32(D), k + c > 0 || (L::FOLD ? (j - 1) % L::FOLD > 0 : j > 1));
             tc::commit(&sh.pv_done[i]);
           }
           if (!ok) {
@@ -181,28 +186,39 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
     constexpr int VL = D / VB, VW = VB / 4;        // lanes a value row
     const bool v_live = x < 8 * VL;
     const long long head = (long long)kvh * a.c.page * D;
-    // page of the 16 tokens from position j on; -1 when no row sees them or there is none
-    auto page_at = [&](int j) {
+    // entry of the page table for the page of position j; pages outside what the rows see are not looked at
+    auto entry = [&](int j) {
       const int o = j >> a.c.lg_page;
-      return ((long long)(o + 1) << a.c.lg_page) > see0 && ((long long)o << a.c.lg_page) <= p_last ? page_id(a.c, a.r, b, o) : -1;
+      return a.r.table + (size_t)b * a.r.width + min(o, a.r.width - 1);
     };
-    auto offset = [&](int id, int j) { return max(id, 0) * a.c.page_stride + head + (j & (a.c.page - 1)) * D; };
-    int kid[KP], vid, mid = -1, ek = 0, ev = 0, f = 0;
+    auto seen = [&](int j) {
+      const int o = j >> a.c.lg_page;
+      return ((long long)(o + 1) << a.c.lg_page) > see0 && ((long long)o << a.c.lg_page) <= p_last;
+    };
+    auto offset = [&](int id, int j) {
+      return (seen(j) && (unsigned)id < (unsigned)a.c.pages ? id : 0) * a.c.page_stride + head + (j & (a.c.page - 1)) * D;
+    };
+    // positions of the thread's key rows, value rows and (threads 0-3) scales in step j
+    auto k_pos = [&](int j, int i) { return (t0 + j) * NT + i * (128 / LR) + x / LR; };
+    auto v_pos = [&](int j) { return (t0 + j) * NT + min(x / VL, 7) * 8; };
+    auto m_pos = [&](int j) { return (t0 + j) * NT + (x & 3) * 16; };
+    // page ids of the next step but one, taken up a step later
+    int kid[KP], vid, mid, mid_j = -1, ek = 0, ev = 0, f = 0;
     uint4 kx[KP];
     uint32_t vx[8][VW];
     auto look = [&](int j) {
 #pragma unroll
-      for (int i = 0; i < KP; ++i) kid[i] = page_at((t0 + j) * NT + i * (128 / LR) + x / LR);
-      vid = page_at((t0 + j) * NT + min(x / VL, 7) * 8);
-      if (x < NT / 16) mid = page_at((t0 + j) * NT + x * 16);
+      for (int i = 0; i < KP; ++i) kid[i] = __ldg(entry(k_pos(j, i)));
+      vid = __ldg(entry(v_pos(j)));
+      mid = __ldg(entry(m_pos(j)));
     };
     auto load_k = [&](int j) {
 #pragma unroll
       for (int i = 0; i < KP; ++i)
-        kx[i] = __ldg(reinterpret_cast<const uint4 *>(a.c.k + offset(kid[i], (t0 + j) * NT + i * (128 / LR) + x / LR) + x % LR * 16));
+        kx[i] = __ldg(reinterpret_cast<const uint4 *>(a.c.k + offset(kid[i], k_pos(j, i)) + x % LR * 16));
     };
     auto load_v = [&](int j) {
-      const int8_t *src = a.c.v + offset(vid, (t0 + j) * NT + min(x / VL, 7) * 8) + x % VL * VB;
+      const int8_t *src = a.c.v + offset(vid, v_pos(j)) + x % VL * VB;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if constexpr (VB == 8) {
@@ -214,33 +230,38 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         }
       }
     };
-    auto load_scales = [&]() {
+    auto load_scales = [&](int j) {
       ek = ev = 0;
-      if (x < NT / 16 && mid >= 0) {
-        ek = a.c.k_exp[mid * a.c.exp_stride + kvh];
-        ev = a.c.v_exp[mid * a.c.exp_stride + kvh];
+      mid_j = -1;
+      if (x < NT / 16 && seen(m_pos(j))) {
+        if ((unsigned)mid < (unsigned)a.c.pages) {
+          mid_j = mid;
+          ek = a.c.k_exp[mid * a.c.exp_stride + kvh];
+          ev = a.c.v_exp[mid * a.c.exp_stride + kvh];
+        } else {
+          set_status(a.r.status, LBC_ERR_PAGE);
+        }
       }
     };
     if (steps > 0) {
       look(0);
       load_k(0);
       load_v(0);
-      load_scales();
+      load_scales(0);
+      look(1);
     }
     for (int j = 0; j < steps; ++j) {
       const int st = j & 1;
       const uint32_t ph = (j >> 1) & 1;
-      const int mid_j = mid, ek_j = ek, ev_j = ev;
-      if (j + 1 < steps) look(j + 1);
       if (!wait(&sh.k_empty[st], ph ^ 1u)) break;
       if (warp == W_DEQ) {
         // the step's block scales; f is the largest value exponent so far (255 left out)
-        int top = lane < NT / 16 && mid_j >= 0 && ev_j != 255 ? ev_j : 0;
+        int top = lane < NT / 16 && mid_j >= 0 && ev != 255 ? ev : 0;
         f = max(f, __reduce_max_sync(0xffffffffu, top));
         if (lane < NT / 16) {
-          const int at = max(ev_j, f - FAR);
-          sh.meta[j % META].g[lane] = make_float4(pow2_e8m0(ek_j), ev_j == 255 ? __uint_as_float(0x7fc00000u) : (float)(at - 127),
-                                                  ev_j == 255 ? 1.f : pow2_e8m0(127 + f - at), mid_j >= 0 ? 1.f : 0.f);
+          const int at = max(ev, f - FAR);
+          sh.meta[j % META].g[lane] = make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(at - 127),
+                                                  ev == 255 ? 1.f : pow2_e8m0(127 + f - at), mid_j >= 0 ? 1.f : 0.f);
           if (lane == 0) sh.meta[j % META].f = f;
         }
         __syncwarp();
@@ -283,10 +304,11 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       mbar_arrive(&sh.v_full[st]);
       if (j + 1 < steps) {
         load_v(j + 1);
-        load_scales();
+        load_scales(j + 1);
+        look(j + 2);
       }
     }
-  } else {
+  } else if (warp < 4 * L::RT) {
     // ------------------------------------------------------------ rows
     const int i = warp >> 2, r = tid & (TILE - 1), rho = rho0 + i * TILE + r;
     const bool live = rho < s.n * a.G;
@@ -326,7 +348,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       tc::fence_proxy_async_smem();
       mbar_arrive(&sh.q_full);
     }
-    float m = LOWEST, l = 0.f;
+    float m = LOWEST;
+    uint64_t ls[2] = {0, 0};  // the sum l, in four parts
     int f = 0;
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
@@ -338,19 +361,18 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) tc::ld16(s_col(i, st) + quad + 16 * g, sv[g]);
       tc::wait_ld();
+#pragma unroll
+      for (int g = 0; g < 4; ++g) tc::loaded16(sv[g]);
       const StepMeta &meta = sh.meta[j % META];
       const int pos0 = (t0 + j) * NT;
       const bool inside = pos0 + NT - 1 <= p_min && (a.window <= 0 || pos0 > p_max - a.window);
-      float mx = -INFINITY;
+      float mg[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const float4 e = meta.g[g];
-        const float c = rowf * e.x;
+        const uint64_t c = pair(rowf * e.x, rowf * e.x), d = pair(e.y, e.y);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          float t = fmaf(u2f(sv[g][k]), c, e.y);
-          sv[g][k] = __float_as_uint(t);
-        }
+        for (int k = 0; k < 16; k += 2) split(fma2(pair(u2f(sv[g][k]), u2f(sv[g][k + 1])), c, d), sv[g][k], sv[g][k + 1]);
         if (!inside || e.w == 0.f) {
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
@@ -358,51 +380,73 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
             if (!(at <= p && (a.window <= 0 || at > p - a.window) && e.w != 0.f)) sv[g][k] = __float_as_uint(-INFINITY);
           }
         }
+        float m0 = u2f(sv[g][0]), m1 = u2f(sv[g][1]);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, u2f(sv[g][k]));
+        for (int k = 2; k < 16; k += 4) {
+          m0 = fmaxf(fmaxf(m0, u2f(sv[g][k])), u2f(sv[g][k + 1]));
+          if (k + 2 < 16) m1 = fmaxf(fmaxf(m1, u2f(sv[g][k + 2])), u2f(sv[g][k + 3]));
+        }
+        mg[g] = fmaxf(m0, m1);
       }
+      const float mx = fmaxf(fmaxf(mg[0], mg[1]), fmaxf(mg[2], mg[3]));
       // a larger f scales l; a much larger one also moves M (kv8_attention.cu: raise)
       float by = 0.f;
       if (meta.f > f) {
         if (j > 0) {
           by = (float)max(0, meta.f - f - 40);
-          l *= ex2((float)(meta.f - f) - by);
+          const float w = ex2((float)(meta.f - f) - by);
+          ls[0] = mul2(ls[0], pair(w, w));
+          ls[1] = mul2(ls[1], pair(w, w));
         }
         f = meta.f;
       }
-      const bool rise = mx > m + SLACK;
-      if (__any_sync(0xffffffffu, rise) || by > 0.f) {
-        float to = m > LOWEST ? m + by : m;
-        float scale = ex2(-by);
-        const float up = fmaxf(to, ceilf(mx) - HEAD);
-        const float w = ex2(to - up);
-        l *= w;
-        scale *= w;
-        m = up;
+      const bool rise = __any_sync(0xffffffffu, mx > m + SLACK) || by > 0.f;
+      const bool fold = L::FOLD && j > 0 && j % (L::FOLD ? L::FOLD : 1) == 0;
+      if (rise || fold) {
+        float scale = 1.f;
+        if (rise) {
+          const float to = m > LOWEST ? m + by : m;
+          m = fmaxf(to, ceilf(mx) - HEAD);
+          scale = ex2(to - m);
+          ls[0] = mul2(ls[0], pair(scale, scale));
+          ls[1] = mul2(ls[1], pair(scale, scale));
+          scale *= ex2(-by);
+        }
         if (j > 0) {
           ok = wait(&sh.pv_done[i], (j - 1) & 1);
           if (!ok) break;
           tc::fence_after_sync();
 #pragma unroll
           for (int c = 0; c < D; c += 16) {
-            uint32_t o[16];
+            uint32_t o[16], t[16];
+            const bool both = L::FOLD && j > L::FOLD;
             tc::ld16(o_col(i) + quad + c, o);
+            if (both) tc::ld16(t_col(i) + quad + c, t);
             tc::wait_ld();
+            tc::loaded16(o);
+            if (both) tc::loaded16(t);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(u2f(o[k]) * scale);
-            tc::st16(o_col(i) + quad + c, o);
+            for (int k = 0; k < 16; ++k) {
+              if (both) t[k] = __float_as_uint((fold ? u2f(t[k]) + u2f(o[k]) : u2f(t[k])) * scale);
+              o[k] = __float_as_uint(u2f(o[k]) * scale);
+            }
+            if (both) tc::st16(t_col(i) + quad + c, t);
+            else if (fold) tc::st16(t_col(i) + quad + c, o);
+            if (!fold) tc::st16(o_col(i) + quad + c, o);
           }
         }
       }
       // weights, and P in the place of S (every thread has read its scores)
+      const uint64_t less = pair(-m, -m);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const float back = meta.g[g].z;
+        const uint64_t back = pair(meta.g[g].z, meta.g[g].z);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float w = ex2(u2f(sv[g][k]) - m);
-          l = fmaf(w, back, l);
-          sv[g][k] = __float_as_uint(w);
+        for (int k = 0; k < 16; k += 2) {
+          split(add2(pair(u2f(sv[g][k]), u2f(sv[g][k + 1])), less), sv[g][k], sv[g][k + 1]);
+          sv[g][k] = __float_as_uint(ex2(u2f(sv[g][k])));
+          sv[g][k + 1] = __float_as_uint(ex2(u2f(sv[g][k + 1])));
+          ls[g & 1] = fma2(pair(u2f(sv[g][k]), u2f(sv[g][k + 1])), back, ls[g & 1]);
         }
       }
 #pragma unroll
@@ -421,16 +465,34 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       tc::fence_before_sync();
       mbar_arrive(&sh.p_full[i][st]);
     }
-    if (steps > 0 && ok) wait(&sh.pv_done[i], (steps - 1) & 1);
+    // all products are done. (Not pv_done's last phase: two of its phases may be
+    // open here, and a parity names only the latest. Inside the loop scores j
+    // imply outputs j - 2, so one is.)
+    if (steps > 0 && ok) wait(&sh.fin, 0);
     tc::fence_after_sync();
+    float l;
+    {
+      uint32_t x0, x1, x2, x3;
+      split(ls[0], x0, x1);
+      split(ls[1], x2, x3);
+      l = (u2f(x0) + u2f(x1)) + (u2f(x2) + u2f(x3));
+    }
     const float w = l == 0.f || steps == 0 ? 0.f : pow2_e8m0(f) / l;
     T *dst = static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D;
 #pragma unroll 2
     for (int c = 0; c < D; c += 16) {
       uint32_t o[16];
       if (steps > 0) {
+        uint32_t t[16];
+        const bool both = L::FOLD && steps > L::FOLD;
         tc::ld16(o_col(i) + quad + c, o);
+        if (both) tc::ld16(t_col(i) + quad + c, t);
         tc::wait_ld();
+        tc::loaded16(o);
+        if (both) tc::loaded16(t);
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (both) o[k] = __float_as_uint(u2f(o[k]) + u2f(t[k]));
       }
       if (live) {
 #pragma unroll
@@ -456,7 +518,8 @@ void launch(const AttnArgs &a, cudaStream_t st) {
   constexpr int smem = Lay<T, D>::SMEM;
   static_assert(smem <= 227 * 1024, "operand tiles fit an SM's shared memory");
   cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  prompt_kernel<T, D><<<dim3(a.c.KV, a.r.B, a.tiles), THREADS, smem, st>>>(a);
+  const unsigned tiles = (unsigned)(((long long)a.r.most * a.G + Lay<T, D>::ROWS - 1) / Lay<T, D>::ROWS);
+  prompt_kernel<T, D><<<dim3(a.c.KV, a.r.B, tiles), THREADS, smem, st>>>(a);
 }
 template <typename T>
 void launch(const AttnArgs &a, cudaStream_t st) {
@@ -467,13 +530,10 @@ void launch(const AttnArgs &a, cudaStream_t st) {
 
 }  // namespace
 
-// a.tiles row tiles of ROWS rows at most
 void launch_prompt(const AttnArgs &a, int dtype, cudaStream_t st) {
-  AttnArgs b = a;
-  b.tiles = (int)(((long long)a.r.most * a.G + ROWS - 1) / ROWS);
-  if (dtype == LBC_F32) launch<float>(b, st);
-  else if (dtype == LBC_BF16) launch<__nv_bfloat16>(b, st);
-  else launch<__half>(b, st);
+  if (dtype == LBC_F32) launch<float>(a, st);
+  else if (dtype == LBC_BF16) launch<__nv_bfloat16>(a, st);
+  else launch<__half>(a, st);
 }
 
 }  // namespace kv8

@@ -88,6 +88,12 @@ __device__ __forceinline__ void ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// keeps arithmetic on loaded registers behind the wait before it: the compiler
+// orders volatile statements, but may move what only depends on the registers
+__device__ __forceinline__ void loaded16(uint32_t (&r)[16]) {
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+               "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
 
 // ------------------------------------------------------------ descriptors
 // Shared-memory matrix descriptor, K-major, no swizzle (layout type 0),

@@ -7,10 +7,9 @@
 //   warps 8-11  codes from global memory to fp16 operand tiles in shared memory
 //               (exact; keys K-major as they lie, values transposed 8 x 8 in
 //               registers), one conversion for both row tiles; block scales
-//   warp 12     S = Q K^T (both operands in shared memory) and O += P V (P, fp16,
-//               in tensor memory where S was), the scores of step j + 1 before
-//               the outputs of step j, so that the tensor cores work while the
-//               weights of a step are computed
+//   warp 12     S = Q K^T, both operands in shared memory, S in two buffers so that
+//               the scores of a step are ready when the weights of the last are done
+//   warp 13     O += P V, P (fp16) in tensor memory where S was
 //   warps 0-7   a thread a row: scores from tensor memory, scale, mask, running
 //               reference M, weights 2^(t - M), sums l; O is rescaled only when a
 //               row's maximum has risen by more than 2^3
@@ -30,7 +29,7 @@ namespace {
 
 constexpr int NT = 64;        // tokens a step
 constexpr int TILE = 128;     // rows of a row tile
-constexpr int W_DEQ = 8, W_MMA = 12, THREADS = 13 * 32;
+constexpr int W_DEQ = 8, W_MMA = 12, THREADS = 14 * 32;
 constexpr int META = 8;       // steps whose block scales are kept
 // weights: M is the maximum (rounded up) less 12, left alone up to 2^15
 constexpr float HEAD = 12.f, SLACK = 15.f;
@@ -40,8 +39,12 @@ struct StepMeta {
   int f, pad[3];
 };
 
+// Full / empty pairs of the rings (two stages each; phase j >> 1), S and P full
+// by row tile and buffer, outputs done by row tile and step parity. A parity
+// wait only tells neighbouring phases apart: every wait below follows from an
+// earlier one that its barrier is at most one phase behind.
 struct Shared {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], meta_full[META], q_full, fin;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2][2], meta_full[META], q_full, s_fin, fin;
   uint32_t tmem;
   int abort;
   StepMeta meta[META];
@@ -88,14 +91,15 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       mbar_init(&sh.v_full[i], 128);
       mbar_init(&sh.k_empty[i], 1);
       mbar_init(&sh.v_empty[i], 1);
-      mbar_init(&sh.pv_done[i], 1);
       for (int j = 0; j < 2; ++j) {
+        mbar_init(&sh.pv_done[i][j], 1);
         mbar_init(&sh.s_full[i][j], 1);
         mbar_init(&sh.p_full[i][j], 128);
       }
     }
     for (int i = 0; i < META; ++i) mbar_init(&sh.meta_full[i], 1);
     mbar_init(&sh.q_full, L::ROWS);
+    mbar_init(&sh.s_fin, 1);
     mbar_init(&sh.fin, 1);
     sh.abort = 0;
     fence_mbar_init();
@@ -122,58 +126,62 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
   auto t_col = [&](int i) { return tmem + 2 * L::RT * NT + (L::RT + i) * D; };
 
   if (warp == W_MMA) {
-    // ------------------------------------------------------------ products
+    // ------------------------------------------------------------ scores
     if (lane == 0 && steps > 0 && mbar_wait(&sh.q_full, 0, a.r.status)) {
       const uint64_t qd = tc::smem_desc(base, L::Q_LBO, 128);
-      for (int j = 0; j <= steps && !*abort; ++j) {
-        if (j < steps) {
-          const int st = j & 1;
-          if (!mbar_wait(&sh.k_full[st], (j >> 1) & 1, a.r.status)) {
-            *abort = 1;
-            break;
-          }
+      for (int j = 0; j < steps && !*abort; ++j) {
+        const int st = j & 1;
+        bool ok = mbar_wait(&sh.k_full[st], (j >> 1) & 1, a.r.status);
+        const uint64_t kd = tc::smem_desc(base + L::K_OFF + st * L::K_BYTES, L::K_LBO, 128);
+#pragma unroll
+        for (int i = 0; i < L::RT; ++i) {
+          // S goes where the weights of step j - 2 were
+          if (j > 1) ok = ok && mbar_wait(&sh.pv_done[i][st], ((j >> 1) & 1) ^ 1u, a.r.status);
+          if (!ok) break;
           tc::fence_after_sync();
-          const uint64_t kd = tc::smem_desc(base + L::K_OFF + st * L::K_BYTES, L::K_LBO, 128);
 #pragma unroll
-          for (int i = 0; i < L::RT; ++i) {
+          for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-              for (int c = 0; c < L::QP; ++c)
-                tc::mma_f16_ss(s_col(i, st), qd + (uint64_t)((i * L::QP + c) * L::Q_BYTES + 2 * k * L::Q_LBO) / 16,
-                               kd + (uint64_t)(2 * k * L::K_LBO) / 16, tc::idesc_f16_f32(NT), k + c > 0);
-            tc::commit(&sh.s_full[i][st]);
-          }
-          tc::commit(&sh.k_empty[st]);
+            for (int c = 0; c < L::QP; ++c)
+              tc::mma_f16_ss(s_col(i, st), qd + (uint64_t)((i * L::QP + c) * L::Q_BYTES + 2 * k * L::Q_LBO) / 16,
+                             kd + (uint64_t)(2 * k * L::K_LBO) / 16, tc::idesc_f16_f32(NT), k + c > 0);
+          tc::commit(&sh.s_full[i][st]);
         }
-        if (j > 0) {
-          const int st = (j - 1) & 1;
-          const uint32_t ph = ((j - 1) >> 1) & 1;
-          if (!mbar_wait(&sh.v_full[st], ph, a.r.status)) {
-            *abort = 1;
-            break;
-          }
-          const uint64_t vd = tc::smem_desc(base + L::V_OFF + st * L::V_BYTES, L::V_LBO, L::V_SBO);
-          bool ok = true;
-#pragma unroll
-          for (int i = 0; i < L::RT; ++i) {
-            ok = ok && mbar_wait(&sh.p_full[i][st], ph, a.r.status);
-            if (!ok) break;
-            tc::fence_after_sync();
-#pragma unroll
-            for (int k = 0; k < NT / 16; ++k)
-#pragma unroll
-              for (int c = 0; c < L::WP; ++c)
-                tc::mma_bf16_ts(o_col(i), s_col(i, st) + 8 * k + NT / 2 * c, vd + (uint64_t)(2 * k * L::V_LBO) / 16,
-                                tc::idesc_f16_f32(D), k + c > 0 || (L::FOLD ? (j - 1) % L::FOLD > 0 : j > 1));
-            tc::commit(&sh.pv_done[i]);
-          }
-          if (!ok) {
-            *abort = 1;
-            break;
-          }
-          tc::commit(&sh.v_empty[st]);
+        if (!ok) {
+          *abort = 1;
+          break;
         }
+        tc::commit(&sh.k_empty[st]);
+      }
+      tc::commit(&sh.s_fin);
+      mbar_wait(&sh.s_fin, 0, a.r.status);
+    }
+  } else if (warp == W_MMA + 1) {
+    // ------------------------------------------------------------ outputs
+    if (lane == 0 && steps > 0) {
+      for (int j = 0; j < steps && !*abort; ++j) {
+        const int st = j & 1;
+        const uint32_t ph = (j >> 1) & 1;
+        bool ok = mbar_wait(&sh.v_full[st], ph, a.r.status);
+        const uint64_t vd = tc::smem_desc(base + L::V_OFF + st * L::V_BYTES, L::V_LBO, L::V_SBO);
+#pragma unroll
+        for (int i = 0; i < L::RT; ++i) {
+          ok = ok && mbar_wait(&sh.p_full[i][st], ph, a.r.status);
+          if (!ok) break;
+          tc::fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < NT / 16; ++k)
+#pragma unroll
+            for (int c = 0; c < L::WP; ++c)
+              tc::mma_bf16_ts(o_col(i), s_col(i, st) + 8 * k + NT / 2 * c, vd + (uint64_t)(2 * k * L::V_LBO) / 16,
+                              tc::idesc_f16_f32(D), k + c > 0 || (L::FOLD ? j % L::FOLD > 0 : j > 0));
+          tc::commit(&sh.pv_done[i][st]);
+        }
+        if (!ok) {
+          *abort = 1;
+          break;
+        }
+        tc::commit(&sh.v_empty[st]);
       }
       tc::commit(&sh.fin);
       mbar_wait(&sh.fin, 0, a.r.status);
@@ -413,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
           scale *= ex2(-by);
         }
         if (j > 0) {
-          ok = wait(&sh.pv_done[i], (j - 1) & 1);
+          ok = wait(&sh.pv_done[i][st ^ 1], ((j - 1) >> 1) & 1);
           if (!ok) break;
           tc::fence_after_sync();
 #pragma unroll
@@ -465,9 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       tc::fence_before_sync();
       mbar_arrive(&sh.p_full[i][st]);
     }
-    // all products are done. (Not pv_done's last phase: two of its phases may be
-    // open here, and a parity names only the latest. Inside the loop scores j
-    // imply outputs j - 2, so one is.)
+    // all outputs are done (pv_done's last phase would not do: the one before may still be open)
     if (steps > 0 && ok) wait(&sh.fin, 0);
     tc::fence_after_sync();
     float l;

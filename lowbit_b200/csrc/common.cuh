@@ -184,6 +184,33 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, int *s
   }
 }
 
+// The same without a suspend time: a time makes the compiler poll with sleeps
+// in between, whose length a pipeline of short steps feels at every wait.
+__device__ __forceinline__ bool mbar_poll(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_polling(uint64_t *bar, uint32_t parity, int *status) {
+  if (mbar_poll(bar, parity)) return true;
+  const long long t0 = clock64(), lim = wait_cycles(status);
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_poll(bar, parity)) return true;
+    if (clock64() - t0 > lim) {
+      set_status(status, LBC_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- bulk copies
 // 1-D bulk copy global -> shared (TMA engine), completion counted on `bar`.
 // No multicast: the destination is this CTA's own shared memory.
@@ -200,6 +227,13 @@ __device__ __forceinline__ void bulk_g2s(void *dst_smem, const void *src_gmem, u
 __device__ __forceinline__ uint64_t policy_evict_first() {
   uint64_t p;
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+
+// L2 policy for data that other CTAs read too
+__device__ __forceinline__ uint64_t policy_evict_normal() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
   return p;
 }
 

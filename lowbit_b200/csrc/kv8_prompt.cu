@@ -4,15 +4,16 @@
 // A CTA takes 256 rows (token t, head g of the group: row t G + g) of one
 // sequence and KV head as two tiles of 128 (fp32 at D = 128: one), and runs through the visible tokens
 // 64 at a time:
-//   warps 8-11  codes from global memory to fp16 operand tiles in shared memory
-//               (exact; keys K-major as they lie, values transposed 8 x 8 in
-//               registers), one conversion for both row tiles; block scales
-//   warp 12     S = Q K^T, both operands in shared memory, S in two buffers so that
-//               the scores of a step are ready when the weights of the last are done
-//   warp 13     O += P V, P (fp16) in tensor memory where S was
 //   warps 0-7   a thread a row: scores from tensor memory, scale, mask, running
 //               reference M, weights 2^(t - M), sums l; O is rescaled only when a
 //               row's maximum has risen by more than 2^3
+//   warps 8-11  codes to fp16 operand tiles (exact; keys K-major as they lie, values
+//               transposed 8 x 8 in registers), one conversion for both row tiles
+//   warp 12     S = Q K^T, both operands in shared memory, S in two buffers so that
+//               the scores of a step are ready when the weights of the last are done
+//   warp 13     O += P V, P (fp16) in tensor memory where S was
+//   warp 14     codes from global memory into a ring, up to 4 steps ahead (bulk copies)
+//   warp 15     block scales, 8 steps at a time
 // Scales, M, l and f are those of the few-row kernel (kv8_attention.cu); queries
 // are scaled into fp16's range per row, fp32 ones in two pieces, and weights of
 // fp32 and fp16 calls in two pieces (twice the products).
@@ -29,13 +30,17 @@ namespace {
 
 constexpr int NT = 64;        // tokens a step
 constexpr int TILE = 128;     // rows of a row tile
-constexpr int W_DEQ = 8, W_MMA = 12, THREADS = 14 * 32;
-constexpr int META = 8;       // steps whose block scales are kept
+constexpr int W_DEQ = 8, W_MMA = 12, W_COPY = 14, W_SCALE = 15, THREADS = 16 * 32;
+// registers a thread of the three kinds of warpgroups, out of 128 at launch
+constexpr int R_ROWS = 184, R_DEQ = 72, R_REST = 64;
+static_assert(256 * R_ROWS + 128 * (R_DEQ + R_REST) <= THREADS * 128, "a block's registers");
+constexpr int META = 8;       // steps whose block scales are looked up together; two such sets are kept
+constexpr int RAW = 4;        // steps whose codes are in flight or waiting
 // weights: M is the maximum (rounded up) less 12, left alone up to 2^15
 constexpr float HEAD = 12.f, SLACK = 15.f;
 
-struct StepMeta {
-  float4 g[NT / 16];  // of each 16 tokens: 2^(ek - 127), b = ev - 127, 2^(f - b), 1 if the page exists
+struct Scales {
+  float4 g[META][NT / 16];  // of each 16 tokens: 2^(ek - 127), b = ev - 127, 2^(f - b), 1 if the page exists
   int f, pad[3];
 };
 
@@ -44,10 +49,10 @@ struct StepMeta {
 // wait only tells neighbouring phases apart: every wait below follows from an
 // earlier one that its barrier is at most one phase behind.
 struct Shared {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2][2], meta_full[META], q_full, s_fin, fin;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], raw_full[RAW], raw_empty[RAW], s_full[2][2], p_full[2][2], pv_done[2][2], meta_full[2], meta_empty[2], q_full, s_fin, fin;
   uint32_t tmem;
-  int abort;
-  StepMeta meta[META];
+  int abort;  // a wait ran out
+  Scales meta[2];
 };
 
 // operand tiles, in bytes. K-major without swizzle: 8 rows x 16 bytes are one
@@ -61,14 +66,24 @@ struct Lay {
   // leaves room for one row tile.
   static constexpr int FOLD = sizeof(T) == 4 ? 4 : 0, RT = FOLD && D == 128 ? 1 : 2, ROWS = RT * TILE;
   static constexpr int QP = QUERY_PIECES<T>, WP = WEIGHT_PIECES<T>;
-  static constexpr int Q_LBO = TILE / 8 * 128, Q_BYTES = D / 8 * Q_LBO;
+  static constexpr int Q_LBO = TILE / 8 * 128 + 16, Q_BYTES = D / 8 * Q_LBO;
   static constexpr int K_LBO = NT / 8 * 128 + 16 * (128 / D), K_BYTES = D / 8 * K_LBO;
   static constexpr int V_SBO = 144, V_LBO = D / 8 * V_SBO, V_BYTES = NT / 8 * V_LBO;
-  static constexpr int K_OFF = RT * QP * Q_BYTES, V_OFF = K_OFF + 2 * K_BYTES, S_OFF = (V_OFF + 2 * V_BYTES + 127) / 128 * 128;
+  static constexpr int K_OFF = RT * QP * Q_BYTES, V_OFF = K_OFF + 2 * K_BYTES, R_BYTES = 2 * NT * D,
+                       R_OFF = (V_OFF + 2 * V_BYTES + 127) / 128 * 128, S_OFF = R_OFF + RAW * R_BYTES;
   static constexpr int SMEM = S_OFF + (int)sizeof(Shared);
   // position along K of the 8 elements from 16 c + 8 h on (the order is free, and the same in Q and K)
   __device__ static int chunk(int c, int h) { return h * (D / 16) + c; }
 };
+
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
@@ -91,13 +106,18 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       mbar_init(&sh.v_full[i], 128);
       mbar_init(&sh.k_empty[i], 1);
       mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.meta_full[i], 1);
+      mbar_init(&sh.meta_empty[i], 4 * L::RT);
       for (int j = 0; j < 2; ++j) {
         mbar_init(&sh.pv_done[i][j], 1);
         mbar_init(&sh.s_full[i][j], 1);
-        mbar_init(&sh.p_full[i][j], 128);
+        mbar_init(&sh.p_full[i][j], TILE);
       }
     }
-    for (int i = 0; i < META; ++i) mbar_init(&sh.meta_full[i], 1);
+    for (int i = 0; i < RAW; ++i) {
+      mbar_init(&sh.raw_full[i], 1);
+      mbar_init(&sh.raw_empty[i], 4);
+    }
     mbar_init(&sh.q_full, L::ROWS);
     mbar_init(&sh.s_fin, 1);
     mbar_init(&sh.fin, 1);
@@ -113,9 +133,11 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
   tc::fence_after_sync();
   const uint32_t tmem = sh.tmem, base = smem_u32(smem);
   volatile int *abort = &sh.abort;
-  // a wait of a whole warp: every lane goes on, or (time limit, recorded) none
+  // a wait of a whole warp: every lane goes on, or (time limit, recorded) none;
+  // a wait that ran out anywhere ends the ones that are not yet over
   auto wait = [&](uint64_t *bar, uint32_t parity) {
-    const bool ok = !*abort && mbar_wait(bar, parity, a.r.status);
+    if (__all_sync(0xffffffffu, mbar_poll(bar, parity))) return true;
+    const bool ok = !*abort && mbar_wait_polling(bar, parity, a.r.status);
     if (__all_sync(0xffffffffu, ok)) return true;
     *abort = 1;
     return false;
@@ -127,16 +149,17 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
 
   if (warp == W_MMA) {
     // ------------------------------------------------------------ scores
-    if (lane == 0 && steps > 0 && mbar_wait(&sh.q_full, 0, a.r.status)) {
+    reg_dec<R_REST>();
+    if (lane == 0 && steps > 0 && mbar_wait_polling(&sh.q_full, 0, a.r.status)) {
       const uint64_t qd = tc::smem_desc(base, L::Q_LBO, 128);
       for (int j = 0; j < steps && !*abort; ++j) {
         const int st = j & 1;
-        bool ok = mbar_wait(&sh.k_full[st], (j >> 1) & 1, a.r.status);
+        bool ok = mbar_wait_polling(&sh.k_full[st], (j >> 1) & 1, a.r.status);
         const uint64_t kd = tc::smem_desc(base + L::K_OFF + st * L::K_BYTES, L::K_LBO, 128);
 #pragma unroll
         for (int i = 0; i < L::RT; ++i) {
           // S goes where the weights of step j - 2 were
-          if (j > 1) ok = ok && mbar_wait(&sh.pv_done[i][st], ((j >> 1) & 1) ^ 1u, a.r.status);
+          if (j > 1) ok = ok && mbar_wait_polling(&sh.pv_done[i][st], ((j >> 1) & 1) ^ 1u, a.r.status);
           if (!ok) break;
           tc::fence_after_sync();
 #pragma unroll
@@ -154,19 +177,20 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         tc::commit(&sh.k_empty[st]);
       }
       tc::commit(&sh.s_fin);
-      mbar_wait(&sh.s_fin, 0, a.r.status);
+      mbar_wait_polling(&sh.s_fin, 0, a.r.status);
     }
   } else if (warp == W_MMA + 1) {
     // ------------------------------------------------------------ outputs
+    reg_dec<R_REST>();
     if (lane == 0 && steps > 0) {
       for (int j = 0; j < steps && !*abort; ++j) {
         const int st = j & 1;
         const uint32_t ph = (j >> 1) & 1;
-        bool ok = mbar_wait(&sh.v_full[st], ph, a.r.status);
+        bool ok = mbar_wait_polling(&sh.v_full[st], ph, a.r.status);
         const uint64_t vd = tc::smem_desc(base + L::V_OFF + st * L::V_BYTES, L::V_LBO, L::V_SBO);
 #pragma unroll
         for (int i = 0; i < L::RT; ++i) {
-          ok = ok && mbar_wait(&sh.p_full[i][st], ph, a.r.status);
+          ok = ok && mbar_wait_polling(&sh.p_full[i][st], ph, a.r.status);
           if (!ok) break;
           tc::fence_after_sync();
 #pragma unroll
@@ -184,102 +208,80 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         tc::commit(&sh.v_empty[st]);
       }
       tc::commit(&sh.fin);
-      mbar_wait(&sh.fin, 0, a.r.status);
+      mbar_wait_polling(&sh.fin, 0, a.r.status);
+    }
+  } else if (warp == W_COPY) {
+    // ------------------------------------------------------------ codes to the raw ring
+    reg_dec<R_REST>();
+    if (lane == 0 && steps > 0) {
+      const int o_lo = (int)(see0 >> a.c.lg_page), o_hi = (int)(p_last >> a.c.lg_page);  // pages that the rows see
+      const int32_t *ids = a.r.table + (size_t)b * a.r.width;
+      const long long head = (long long)kvh * a.c.page * D;
+      const int run = min(a.c.page, NT);  // tokens that lie together
+      const uint64_t keep = policy_evict_normal();
+      int j = 0;
+      for (; j < steps && !*abort; ++j) {
+        const int rs = j % RAW;
+        if (!mbar_wait_polling(&sh.raw_empty[rs], (j / RAW & 1) ^ 1u, a.r.status)) {
+          *abort = 1;
+          break;
+        }
+        uint8_t *dst = smem + L::R_OFF + rs * L::R_BYTES;
+        mbar_expect_tx(&sh.raw_full[rs], L::R_BYTES);
+        for (int k = 0; k < NT; k += run) {
+          // positions that no row sees take a neighbouring page's codes (they are masked), bad ids page 0's
+          const int pos = (t0 + j) * NT + k, id = ids[min(max(pos >> a.c.lg_page, o_lo), o_hi)];
+          const long long off = ((unsigned)id < (unsigned)a.c.pages ? id : 0) * a.c.page_stride + head + (pos & (a.c.page - 1)) * D;
+          bulk_g2s(dst + k * D, a.c.k + off, run * D, &sh.raw_full[rs], keep);
+          bulk_g2s(dst + (NT + k) * D, a.c.v + off, run * D, &sh.raw_full[rs], keep);
+        }
+      }
+      // copies in flight land before the block's shared memory goes
+      for (int k = max(0, j - RAW); k < j; ++k)
+        if (!mbar_wait_polling(&sh.raw_full[k % RAW], (k / RAW) & 1, a.r.status)) break;
+    }
+  } else if (warp == W_SCALE) {
+    // ------------------------------------------------------------ block scales, a lane 16 tokens of META steps
+    reg_dec<R_REST>();
+    const int o_lo = (int)(see0 >> a.c.lg_page), o_hi = (int)(p_last >> a.c.lg_page);
+    const int32_t *ids = a.r.table + (size_t)b * a.r.width;
+    int f = 0;  // largest value exponent so far (255 left out)
+    for (int j = 0; j < steps; j += META) {
+      const int set = j / META & 1;
+      const int id = ids[min(max(((t0 + j) * NT + lane * 16) >> a.c.lg_page, o_lo), o_hi)];
+      const bool there = (unsigned)id < (unsigned)a.c.pages;
+      if (!there) set_status(a.r.status, LBC_ERR_PAGE);
+      const int ek = there ? a.c.k_exp[id * a.c.exp_stride + kvh] : 0, ev = there ? a.c.v_exp[id * a.c.exp_stride + kvh] : 0;
+      f = max(f, __reduce_max_sync(0xffffffffu, ev == 255 ? 0 : ev));
+      const int at = max(ev, f - FAR);
+      if (!wait(&sh.meta_empty[set], (j / META >> 1 & 1) ^ 1u)) break;
+      sh.meta[set].g[lane / (NT / 16)][lane % (NT / 16)] =
+          make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(at - 127),
+                      ev == 255 ? 1.f : pow2_e8m0(127 + f - at), there ? 1.f : 0.f);
+      if (lane == 0) sh.meta[set].f = f;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.meta_full[set]);
     }
   } else if (warp >= W_DEQ) {
     // ------------------------------------------------------------ codes to operands
+    reg_dec<R_DEQ>();
     const int x = tid - W_DEQ * 32;  // 0 .. 127
-    constexpr int LR = D / 16, KP = D / 32;        // lanes a key row, 16-byte pieces a thread
-    constexpr int VB = D == 32 ? 4 : D / 16;       // bytes of a value row a thread transposes
-    constexpr int VL = D / VB, VW = VB / 4;        // lanes a value row
-    const bool v_live = x < 8 * VL;
-    const long long head = (long long)kvh * a.c.page * D;
-    // entry of the page table for the page of position j; pages outside what the rows see are not looked at
-    auto entry = [&](int j) {
-      const int o = j >> a.c.lg_page;
-      return a.r.table + (size_t)b * a.r.width + min(o, a.r.width - 1);
-    };
-    auto seen = [&](int j) {
-      const int o = j >> a.c.lg_page;
-      return ((long long)(o + 1) << a.c.lg_page) > see0 && ((long long)o << a.c.lg_page) <= p_last;
-    };
-    auto offset = [&](int id, int j) {
-      return (seen(j) && (unsigned)id < (unsigned)a.c.pages ? id : 0) * a.c.page_stride + head + (j & (a.c.page - 1)) * D;
-    };
-    // positions of the thread's key rows, value rows and (threads 0-3) scales in step j
-    auto k_pos = [&](int j, int i) { return (t0 + j) * NT + i * (128 / LR) + x / LR; };
-    auto v_pos = [&](int j) { return (t0 + j) * NT + min(x / VL, 7) * 8; };
-    auto m_pos = [&](int j) { return (t0 + j) * NT + (x & 3) * 16; };
-    // page ids of the next step but one, taken up a step later
-    int kid[KP], vid, mid, mid_j = -1, ek = 0, ev = 0, f = 0;
-    uint4 kx[KP];
-    uint32_t vx[8][VW];
-    auto look = [&](int j) {
-#pragma unroll
-      for (int i = 0; i < KP; ++i) kid[i] = __ldg(entry(k_pos(j, i)));
-      vid = __ldg(entry(v_pos(j)));
-      mid = __ldg(entry(m_pos(j)));
-    };
-    auto load_k = [&](int j) {
-#pragma unroll
-      for (int i = 0; i < KP; ++i)
-        kx[i] = __ldg(reinterpret_cast<const uint4 *>(a.c.k + offset(kid[i], k_pos(j, i)) + x % LR * 16));
-    };
-    auto load_v = [&](int j) {
-      const int8_t *src = a.c.v + offset(vid, v_pos(j)) + x % VL * VB;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (VB == 8) {
-          const uint2 y = __ldg(reinterpret_cast<const uint2 *>(src + i * D));
-          vx[i][0] = y.x;
-          vx[i][1] = y.y;
-        } else {
-          vx[i][0] = __ldg(reinterpret_cast<const uint32_t *>(src + i * D));
-        }
-      }
-    };
-    auto load_scales = [&](int j) {
-      ek = ev = 0;
-      mid_j = -1;
-      if (x < NT / 16 && seen(m_pos(j))) {
-        if ((unsigned)mid < (unsigned)a.c.pages) {
-          mid_j = mid;
-          ek = a.c.k_exp[mid * a.c.exp_stride + kvh];
-          ev = a.c.v_exp[mid * a.c.exp_stride + kvh];
-        } else {
-          set_status(a.r.status, LBC_ERR_PAGE);
-        }
-      }
-    };
-    if (steps > 0) {
-      look(0);
-      load_k(0);
-      load_v(0);
-      load_scales(0);
-      look(1);
-    }
+    constexpr int LR = D / 16, KP = D / 32, KR = 128 / LR;  // 16-byte pieces of a row, pieces a thread, rows apart
+    constexpr int VB = D == 32 ? 4 : D / 16;                // bytes of a value row a thread transposes
+    constexpr int VL = D / VB, VW = VB / 4;                 // lanes a value row
     for (int j = 0; j < steps; ++j) {
       const int st = j & 1;
       const uint32_t ph = (j >> 1) & 1;
-      if (!wait(&sh.k_empty[st], ph ^ 1u)) break;
-      if (warp == W_DEQ) {
-        // the step's block scales; f is the largest value exponent so far (255 left out)
-        int top = lane < NT / 16 && mid_j >= 0 && ev != 255 ? ev : 0;
-        f = max(f, __reduce_max_sync(0xffffffffu, top));
-        if (lane < NT / 16) {
-          const int at = max(ev, f - FAR);
-          sh.meta[j % META].g[lane] = make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(at - 127),
-                                                  ev == 255 ? 1.f : pow2_e8m0(127 + f - at), mid_j >= 0 ? 1.f : 0.f);
-          if (lane == 0) sh.meta[j % META].f = f;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.meta_full[j % META]);
-      }
+      const uint32_t raw = base + L::R_OFF + j % RAW * L::R_BYTES;
+      if (!wait(&sh.raw_full[j % RAW], (j / RAW) & 1) || !wait(&sh.k_empty[st], ph ^ 1u)) break;
       uint8_t *kt = smem + L::K_OFF + st * L::K_BYTES;
 #pragma unroll
       for (int i = 0; i < KP; ++i) {
-        const int tok = i * (128 / LR) + x / LR, c = x % LR;
-        const uint32_t w[4] = {kx[i].x ^ 0x80808080u, kx[i].y ^ 0x80808080u, kx[i].z ^ 0x80808080u, kx[i].w ^ 0x80808080u};
+        const int tok = i * KR + x / LR, c = x % LR;
+        uint32_t w[4];
+        shared_words<16>(raw + i * 2048 + x * 16, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           *reinterpret_cast<uint4 *>(kt + L::chunk(c, h) * L::K_LBO + tok / 8 * 128 + tok % 8 * 16) =
@@ -287,20 +289,23 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       }
       tc::fence_proxy_async_smem();
       mbar_arrive(&sh.k_full[st]);
-      if (j + 1 < steps) load_k(j + 1);
       if (!wait(&sh.v_empty[st], ph ^ 1u)) break;
-      if (v_live) {
+      if (x < 8 * VL) {
+        uint32_t y[8][VW];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          shared_words<VB>(raw + NT * D + (x / VL * 8 + i) * D + x % VL * VB, y[i]);
+#pragma unroll
+          for (int w = 0; w < VW; ++w) y[i][w] ^= 0x80808080u;
+        }
         uint8_t *vt = smem + L::V_OFF + st * L::V_BYTES + x / VL * L::V_LBO;
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
-          uint32_t y[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = vx[i][w] ^ 0x80808080u;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {  // elements 2 h and 2 h + 1 of the word, tokens in pairs
             uint32_t z[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = prmt(y[2 * i], y[2 * i + 1], h ? 0x7362 : 0x5140);
+            for (int i = 0; i < 4; ++i) z[i] = prmt(y[2 * i][w], y[2 * i + 1][w], h ? 0x7362 : 0x5140);
             const int d = x % VL * VB + 4 * w + 2 * h;
             uint8_t *dst = vt + d / 8 * L::V_SBO + d % 8 * 16;
             *reinterpret_cast<uint4 *>(dst) = make_uint4(half_lo(z[0]), half_lo(z[1]), half_lo(z[2]), half_lo(z[3]));
@@ -310,59 +315,69 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       }
       tc::fence_proxy_async_smem();
       mbar_arrive(&sh.v_full[st]);
-      if (j + 1 < steps) {
-        load_v(j + 1);
-        load_scales(j + 1);
-        look(j + 2);
-      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.raw_empty[j % RAW]);
     }
   } else if (warp < 4 * L::RT) {
     // ------------------------------------------------------------ rows
-    const int i = warp >> 2, r = tid & (TILE - 1), rho = rho0 + i * TILE + r;
-    const bool live = rho < s.n * a.G;
+    reg_inc<R_ROWS>();
+    const int i = warp >> 2, rho = rho0 + i * TILE + (tid & (TILE - 1)), first = rho - lane;  // first: the warp's first row
     const uint32_t quad = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
     const int p = row_pos(a, s, rho);
     const int p_min = __reduce_min_sync(0xffffffffu, p), p_max = __reduce_max_sync(0xffffffffu, p);
-    float rowf;
-    {
-      const T *src = static_cast<const T *>(a.q) + (s.r0 + min(rho, s.n * a.G - 1) / a.G) * a.ld +
-                     (size_t)(kvh * a.G + min(rho, s.n * a.G - 1) % a.G) * D;
-      float amax = 0.f;
-      for (int d = 0; d < D; d += 4) {
-        float y[4];
-        load4<T>(src + d, y);
+    // rows of q and out: LR lanes of 16 bytes (E elements) a row, RI rows an instruction
+    constexpr int E = 16 / (int)sizeof(T), LR = D / E, RI = 32 / LR;
+    uint8_t *mine = smem + i * L::QP * L::Q_BYTES;  // the row tile's query operand, at the end its output rows
+    float rowf = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) amax = y[e] == y[e] ? fmaxf(amax, fabsf(y[e])) : INFINITY;
+    for (int x0 = 0; x0 < 32 / RI; x0 += 8) {
+      constexpr int B = 32 / RI < 8 ? 32 / RI : 8;  // instructions in flight
+      uint4 raw[B];
+#pragma unroll
+      for (int x = 0; x < B; ++x) {
+        const int row = min(first + (x0 + x) * RI + lane / LR, s.n * a.G - 1);
+        raw[x] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (s.r0 + row / a.G) * a.ld +
+                                                  (size_t)(kvh * a.G + row % a.G) * D + lane % LR * E);
       }
-      const float up = fp16_range(amax);
-      rowf = a.scale_log2 / up;
-      uint8_t *qt = smem + i * L::QP * L::Q_BYTES + r / 8 * 128 + r % 8 * 16;
-#pragma unroll 2
-      for (int d = 0; d < D; d += 8) {
-        float y[8];
-        load4<T>(src + d, reinterpret_cast<float(&)[4]>(y[0]));
-        load4<T>(src + d + 4, reinterpret_cast<float(&)[4]>(y[4]));
-        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+      for (int x = 0; x < B; ++x) {
+        float y[E], amax = 0.f;
+        load4<T>(reinterpret_cast<const T *>(&raw[x]), reinterpret_cast<float(&)[4]>(y[0]));
+        if constexpr (E == 8) load4<T>(reinterpret_cast<const T *>(&raw[x]) + 4, reinterpret_cast<float(&)[4]>(y[4]));
+#pragma unroll
+        for (int e = 0; e < E; ++e) amax = y[e] == y[e] ? fmaxf(amax, fabsf(y[e])) : INFINITY;
+#pragma unroll
+        for (int d = 1; d < LR; d *= 2) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+        const float up = fp16_range(amax), back = __shfl_sync(0xffffffffu, a.scale_log2 / up, lane % RI * LR);
+        if (lane / RI == x0 + x) rowf = back;
+        uint32_t hi[E / 2], lo[E / 2];
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
           const float y0 = y[2 * e] * up, y1 = y[2 * e + 1] * up;
           hi[e] = pack_half(y0, y1);
           if (L::QP == 2) lo[e] = pack_rest(y0, y1, hi[e]);
         }
-        uint8_t *dst = qt + L::chunk(d / 16, d / 8 % 2) * L::Q_LBO;
-        *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (L::QP == 2) *reinterpret_cast<uint4 *>(dst + L::Q_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        const int r = (warp & 3) * 32 + (x0 + x) * RI + lane / LR, d = lane % LR * E;
+        uint8_t *dst = mine + L::chunk(d / 16, d / 8 % 2) * L::Q_LBO + r / 8 * 128 + r % 8 * 16 + d % 8 * 2;
+        if constexpr (E == 8) {
+          *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        } else {
+          *reinterpret_cast<uint2 *>(dst) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2 *>(dst + L::Q_BYTES) = make_uint2(lo[0], lo[1]);
+        }
+        if constexpr (E == 8 && L::QP == 2) static_assert(E == 4, "two query pieces are fp32's");
       }
-      tc::fence_proxy_async_smem();
-      mbar_arrive(&sh.q_full);
     }
+    tc::fence_proxy_async_smem();
+    mbar_arrive(&sh.q_full);
     float m = LOWEST;
     uint64_t ls[2] = {0, 0};  // the sum l, in four parts
     int f = 0;
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
-      const int st = j & 1;
-      ok = wait(&sh.meta_full[j % META], (j / META) & 1) && wait(&sh.s_full[i][st], (j >> 1) & 1);
+      const int st = j & 1, set = j / META & 1;
+      if (j % META == 0) ok = wait(&sh.meta_full[set], j / META >> 1 & 1);
+      ok = ok && wait(&sh.s_full[i][st], (j >> 1) & 1);
       if (!ok) break;
       tc::fence_after_sync();
       uint32_t sv[4][16];
@@ -371,13 +386,15 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       tc::wait_ld();
 #pragma unroll
       for (int g = 0; g < 4; ++g) tc::loaded16(sv[g]);
-      const StepMeta &meta = sh.meta[j % META];
+      const Scales &meta = sh.meta[set];
+      const float4 *scale_of = meta.g[j % META];
       const int pos0 = (t0 + j) * NT;
       const bool inside = pos0 + NT - 1 <= p_min && (a.window <= 0 || pos0 > p_max - a.window);
-      float mg[4];
+      float mg[4], back[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const float4 e = meta.g[g];
+        const float4 e = scale_of[g];
+        back[g] = e.z;
         const uint64_t c = pair(rowf * e.x, rowf * e.x), d = pair(e.y, e.y);
 #pragma unroll
         for (int k = 0; k < 16; k += 2) split(fma2(pair(u2f(sv[g][k]), u2f(sv[g][k + 1])), c, d), sv[g][k], sv[g][k + 1]);
@@ -444,34 +461,31 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
           }
         }
       }
-      // weights, and P in the place of S (every thread has read its scores)
+      // weights, and P in the place of S
       const uint64_t less = pair(-m, -m);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const uint64_t back = pair(meta.g[g].z, meta.g[g].z);
-#pragma unroll
-        for (int k = 0; k < 16; k += 2) {
-          split(add2(pair(u2f(sv[g][k]), u2f(sv[g][k + 1])), less), sv[g][k], sv[g][k + 1]);
-          sv[g][k] = __float_as_uint(ex2(u2f(sv[g][k])));
-          sv[g][k + 1] = __float_as_uint(ex2(u2f(sv[g][k + 1])));
-          ls[g & 1] = fma2(pair(u2f(sv[g][k]), u2f(sv[g][k + 1])), back, ls[g & 1]);
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int half = 0; half < 2; ++half) {
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float w0 = u2f(sv[2 * g + k / 8][2 * k % 16]), w1 = u2f(sv[2 * g + k / 8][2 * k % 16 + 1]);
+          const int g = 2 * half + k / 8, e = 2 * k % 16;
+          uint32_t x0, x1;
+          split(add2(pair(u2f(sv[g][e]), u2f(sv[g][e + 1])), less), x0, x1);
+          const float w0 = ex2(u2f(x0)), w1 = ex2(u2f(x1));
+          ls[k & 1] = fma2(pair(w0, w1), pair(back[g], back[g]), ls[k & 1]);
           hi[k] = pack_half(w0, w1);
           if (L::WP == 2) lo[k] = pack_rest(w0, w1, hi[k]);
         }
-        tc::st16(s_col(i, st) + quad + 16 * g, hi);
-        if (L::WP == 2) tc::st16(s_col(i, st) + quad + NT / 2 + 16 * g, lo);
+        tc::st16(s_col(i, st) + quad + 16 * half, hi);
+        if (L::WP == 2) tc::st16(s_col(i, st) + quad + NT / 2 + 16 * half, lo);
       }
       tc::wait_st();
       tc::fence_before_sync();
       mbar_arrive(&sh.p_full[i][st]);
+      if (j % META == META - 1) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.meta_empty[set]);
+      }
     }
     // all outputs are done (pv_done's last phase would not do: the one before may still be open)
     if (steps > 0 && ok) wait(&sh.fin, 0);
@@ -484,8 +498,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       l = (u2f(x0) + u2f(x1)) + (u2f(x2) + u2f(x3));
     }
     const float w = l == 0.f || steps == 0 ? 0.f : pow2_e8m0(f) / l;
-    T *dst = static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D;
-#pragma unroll 2
+    // the warp's rows through shared memory (16-byte pieces change places by row), then out in whole rows
+    T *stage = reinterpret_cast<T *>(mine) + (warp & 3) * 32 * D;
+#pragma unroll
     for (int c = 0; c < D; c += 16) {
       uint32_t o[16];
       if (steps > 0) {
@@ -500,15 +515,26 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         for (int k = 0; k < 16; ++k)
           if (both) o[k] = __float_as_uint(u2f(o[k]) + u2f(t[k]));
       }
-      if (live) {
 #pragma unroll
-        for (int k = 0; k < 16; k += 4) {
+      for (int k = 0; k < 16; k += E) {
+        T *dst = stage + lane * D + (((c + k) / E ^ lane) & (LR - 1)) * E;
+#pragma unroll
+        for (int h = 0; h < E; h += 4) {
           float y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = w == 0.f ? 0.f : u2f(o[k + e]) * w;
-          store4<T>(dst + c + k, y);
+          for (int e = 0; e < 4; ++e) y[e] = w == 0.f ? 0.f : u2f(o[k + h + e]) * w;
+          store4<T>(dst + h, y);
         }
       }
+    }
+    __syncwarp();
+#pragma unroll 4
+    for (int x = 0; x < 32 / RI; ++x) {
+      const int r = x * RI + lane / LR, row = first + r;
+      const uint4 v = *reinterpret_cast<const uint4 *>(stage + r * D + ((lane % LR ^ r) & (LR - 1)) * E);
+      if (row < s.n * a.G)
+        *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + ((size_t)(s.r0 + row / a.G) * a.H + kvh * a.G + row % a.G) * D +
+                                   lane % LR * E) = v;
     }
   }
   tc::fence_before_sync();

@@ -25,6 +25,11 @@ TINY = {"fp32": 2.0 ** -150, "bf16": 2.0 ** -134, "fp16": 2.0 ** -25}  # half ul
 ERR_PAGE = -8
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    torch.manual_seed(0)
+
+
 def host_pool(rng, pages, kv, page, d, spread=0.5):
     p = {}
     for n in "kv":
@@ -259,7 +264,7 @@ def test_pools_past_32_bit_offsets(new):
     dense = device_pool(pool)
     k.copy_(dense.k)
     v.copy_(dense.v)
-    far = lb.KV8Cache(k, v, dense.k_exp, dense.v_exp)
+    far = lb.KV8Cache(k, v, dense.k_exp.clone(), dense.v_exp.clone())
     table, pos = i32([[3, 0, 2, 1]]), i32([256 - new])
     q = torch.randn((new, 2, 64), device="cuda")
     assert torch.equal(lb.kv8_attention(q, far, table, pos), lb.kv8_attention(q, dense, table, pos))

@@ -41,7 +41,7 @@ constexpr float HEAD = 12.f, SLACK = 15.f;
 
 struct Scales {
   float4 g[META][NT / 16];  // of each 16 tokens: 2^(ek - 127), b = ev - 127, 2^(f - b), 1 if the page exists
-  int f, pad[3];
+  int f, all, pad[2];       // all: every page of the set exists
 };
 
 // Full / empty pairs of the rings (two stages each; phase j >> 1), S and P full
@@ -253,12 +253,15 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       if (!there) set_status(a.r.status, LBC_ERR_PAGE);
       const int ek = there ? a.c.k_exp[id * a.c.exp_stride + kvh] : 0, ev = there ? a.c.v_exp[id * a.c.exp_stride + kvh] : 0;
       f = max(f, __reduce_max_sync(0xffffffffu, ev == 255 ? 0 : ev));
-      const int at = max(ev, f - FAR);
+      const int at = max(ev, f - FAR), all = __all_sync(0xffffffffu, there);
       if (!wait(&sh.meta_empty[set], (j / META >> 1 & 1) ^ 1u)) break;
       sh.meta[set].g[lane / (NT / 16)][lane % (NT / 16)] =
           make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(at - 127),
                       ev == 255 ? 1.f : pow2_e8m0(127 + f - at), there ? 1.f : 0.f);
-      if (lane == 0) sh.meta[set].f = f;
+      if (lane == 0) {
+        sh.meta[set].f = f;
+        sh.meta[set].all = all;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.meta_full[set]);
     }
@@ -389,7 +392,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       const Scales &meta = sh.meta[set];
       const float4 *scale_of = meta.g[j % META];
       const int pos0 = (t0 + j) * NT;
-      const bool inside = pos0 + NT - 1 <= p_min && (a.window <= 0 || pos0 > p_max - a.window);
+      const bool inside = pos0 + NT - 1 <= p_min && (a.window <= 0 || pos0 > p_max - a.window) && meta.all;
       float mg[4], back[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -398,13 +401,18 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         const uint64_t c = pair(rowf * e.x, rowf * e.x), d = pair(e.y, e.y);
 #pragma unroll
         for (int k = 0; k < 16; k += 2) split(fma2(pair(u2f(sv[g][k]), u2f(sv[g][k + 1])), c, d), sv[g][k], sv[g][k + 1]);
-        if (!inside || e.w == 0.f) {
+      }
+      if (!inside) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             const int at = pos0 + 16 * g + k;
-            if (!(at <= p && (a.window <= 0 || at > p - a.window) && e.w != 0.f)) sv[g][k] = __float_as_uint(-INFINITY);
+            if (!(at <= p && (a.window <= 0 || at > p - a.window) && scale_of[g].w != 0.f)) sv[g][k] = __float_as_uint(-INFINITY);
           }
-        }
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
         float m0 = u2f(sv[g][0]), m1 = u2f(sv[g][1]);
 #pragma unroll
         for (int k = 2; k < 16; k += 4) {

@@ -77,8 +77,7 @@ __device__ __forceinline__ float block_max(float v, float *red) {
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   float m = red[0];
-#pragma unroll
-  for (int i = 1; i < THREADS / 32; ++i) m = (m != m || red[i] != red[i]) ? __uint_as_float(0x7fc00000u) : fmaxf(m, red[i]);
+  for (int i = 1; i < (int)blockDim.x / 32; ++i) m = (m != m || red[i] != red[i]) ? __uint_as_float(0x7fc00000u) : fmaxf(m, red[i]);
   return m;
 }
 
@@ -104,59 +103,144 @@ struct AppendArgs {
   void *q_out;
 };
 
-// elements [d, d + 4) and [d + D/2, d + D/2 + 4) of head `head` of a row, bias
-// added and, where `rotate`, turned by the position's angle
 template <typename T>
-__device__ __forceinline__ void load_pair(const AppendArgs &a, int row, int head, int d, int p, bool rotate, float (&x1)[4],
-                                          float (&x2)[4]) {
-  const int D = a.c.D, half = D / 2, col = head * D + d;
-  const T *src = static_cast<const T *>(a.qkv) + row * a.ld + col;
-  load4<T>(src, x1);
-  load4<T>(src + half, x2);
-  if (a.bias) {
+constexpr int VEC = 16 / (int)sizeof(T);  // elements of a 16-byte load
+
+template <typename T>
+__device__ __forceinline__ void load16(const T *p, float (&x)[VEC<T>]) {
+  const uint4 u = *reinterpret_cast<const uint4 *>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x1[i] = __fadd_rn(x1[i], a.bias[col + i]);
-      x2[i] = __fadd_rn(x2[i], a.bias[col + half + i]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      x[i] = __uint_as_float(w[i]);
+    } else {
+      const ushort2 h = make_ushort2((unsigned short)w[i], (unsigned short)(w[i] >> 16));
+      x[2 * i] = to_f<T>(reinterpret_cast<const T &>(h.x));
+      x[2 * i + 1] = to_f<T>(reinterpret_cast<const T &>(h.y));
     }
   }
-  if (rotate) {
-    float c[4], s[4];
-    load4<float>(a.cos_t + (size_t)p * half + d, c);
-    load4<float>(a.sin_t + (size_t)p * half + d, s);
+}
+template <typename T>
+__device__ __forceinline__ void store16(T *p, const float (&x)[VEC<T>]) {
+  union {
+    uint4 u;
+    T t[VEC<T>];
+  } v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float o1 = __fsub_rn(__fmul_rn(x1[i], c[i]), __fmul_rn(x2[i], s[i]));
-      const float o2 = __fadd_rn(__fmul_rn(x2[i], c[i]), __fmul_rn(x1[i], s[i]));
-      x1[i] = o1;
-      x2[i] = o2;
+  for (int i = 0; i < VEC<T>; ++i) v.t[i] = from_f<T>(x[i]);
+  *reinterpret_cast<uint4 *>(p) = v.u;
+}
+
+// V consecutive fp32 values of a table or bias (bias may lie at any float)
+template <int V>
+__device__ __forceinline__ void load_row(const float *p, float (&x)[V], bool aligned) {
+  if (aligned) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(p + i));
+      x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = __ldg(p + i);
+  }
+}
+
+// elements [d, d + V) and [d + D/2, d + D/2 + V) of head `head` of a row, bias added
+template <typename T, int D>
+__device__ __forceinline__ void load_pair(const AppendArgs &a, int row, int head, int d, float (&x1)[VEC<T>], float (&x2)[VEC<T>]) {
+  constexpr int V = VEC<T>;
+  const int col = head * D + d;
+  const T *src = static_cast<const T *>(a.qkv) + row * a.ld + col;
+  load16<T>(src, x1);
+  load16<T>(src + D / 2, x2);
+  if (a.bias) {
+    float b1[V], b2[V];
+    const bool al = (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0;
+    load_row<V>(a.bias + col, b1, al);
+    load_row<V>(a.bias + col + D / 2, b2, al);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      x1[i] = __fadd_rn(x1[i], b1[i]);
+      x2[i] = __fadd_rn(x2[i], b2[i]);
     }
   }
 }
 
-// grid: first 2 * KV * slots * B CTAs, one block (keys or values of a page and
-// head) each; then the query CTAs, one row each
-template <typename T>
-__global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
+// rotate-half by the angles whose cosines and sines are c and s
+template <int V>
+__device__ __forceinline__ void turn(float (&x1)[V], float (&x2)[V], const float (&c)[V], const float (&s)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float o1 = __fsub_rn(__fmul_rn(x1[i], c[i]), __fmul_rn(x2[i], s[i]));
+    const float o2 = __fadd_rn(__fmul_rn(x2[i], c[i]), __fmul_rn(x1[i], s[i]));
+    x1[i] = o1;
+    x2[i] = o2;
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void store_codes(int8_t *dst, const float (&x)[V], float f, float top) {
+  uint32_t w[V / 4];
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) w[i] = pack4({x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]}, f, top);
+  if constexpr (V == 8) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t *>(dst) = w[0];
+}
+
+// the sequence that owns row `row`, 32 of them compared at a time by the warp
+__device__ __forceinline__ int warp_row_seq(const Rows &r, int row) {
+  if (!r.starts) return row / (r.N / r.B);
+  int b = 0;
+  for (int i = threadIdx.x & 31; i - (int)(threadIdx.x & 31) < r.B; i += 32) {
+    const int k = __popc(__ballot_sync(0xffffffffu, i < r.B && r.starts[i + 1] <= row));
+    b += k;
+    if (k < 32) break;
+  }
+  return min(b, r.B - 1);
+}
+
+// Grid: first 2 * KV * slots * B CTAs, one block (keys or values of a page and
+// head) each; then the query CTAs, one row a warp. A thread moves 16 bytes at a
+// time; a block's rows are read twice, for the maximum and for the codes (the
+// second time from L1: keeping them in registers costs the query CTAs their
+// occupancy). blockDim is 64 when a sequence brings few rows, 256 otherwise.
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 4) append_kernel(AppendArgs a) {
+  constexpr int V = VEC<T>, half = D / 2, per = half / V;  // per: threads a head and token
   __shared__ float red[THREADS / 32];
-  const int D = a.c.D, half = D / 2, per = half / 4;  // pairs of four per head and token
   const int kv_ctas = 2 * a.c.KV * a.slots * a.r.B;
   int i = blockIdx.x;
-  if (i >= kv_ctas) {  // queries of one row
-    const int row = i - kv_ctas;
+  const int d = threadIdx.x % per * V;
+  if (i >= kv_ctas) {  // queries, one row a warp: a lane keeps its angles for all its heads
+    const int row = (i - kv_ctas) * (blockDim.x / 32) + threadIdx.x / 32, lane = threadIdx.x & 31;
+    if (row >= a.r.N) return;
     int r0, n;
-    const int b = row_seq(a.r, row);
+    const int b = warp_row_seq(a.r, row);
     seq_rows(a.r, b, r0, n);
     if (row < r0 || row >= r0 + n) return;
     const long long p = (long long)a.r.pos[b] + row - r0;
     T *out = static_cast<T *>(a.q_out) + (size_t)row * a.H * D;
-    if (p >= a.positions && threadIdx.x == 0) set_status(a.r.status, LBC_ERR_PAGE);
-    for (int e = threadIdx.x; e < a.H * per; e += THREADS) {
-      const int head = e / per, d = (e % per) * 4;
-      float x1[4] = {0.f, 0.f, 0.f, 0.f}, x2[4] = {0.f, 0.f, 0.f, 0.f};
-      if (p >= 0 && p < a.positions) load_pair<T>(a, row, head, d, (int)p, true, x1, x2);
-      store4<T>(out + head * D + d, x1);
-      store4<T>(out + head * D + d + half, x2);
+    if (p >= a.positions && lane == 0) set_status(a.r.status, LBC_ERR_PAGE);
+    if (p < 0 || p >= a.positions) {
+      float zero[V] = {};
+      for (int head = lane / per; head < a.H; head += 32 / per) {
+        store16<T>(out + head * D + d, zero);
+        store16<T>(out + head * D + d + half, zero);
+      }
+      return;
+    }
+    float c[V], s[V];
+    load_row<V>(a.cos_t + (size_t)p * half + d, c, true);
+    load_row<V>(a.sin_t + (size_t)p * half + d, s, true);
+#pragma unroll 4
+    for (int head = lane / per; head < a.H; head += 32 / per) {
+      float x1[V], x2[V];
+      load_pair<T, D>(a, row, head, d, x1, x2);
+      turn<V>(x1, x2, c, s);
+      store16<T>(out + head * D + d, x1);
+      store16<T>(out + head * D + d + half, x2);
     }
     return;
   }
@@ -174,23 +258,33 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
   const int lo = max(first, o << a.c.lg_page), hi = min(last, (o + 1) << a.c.lg_page);
   if (lo >= hi) return;
   const int id = page_id(a.c, a.r, b, o);
-  if (id < 0) return;
-  int8_t *codes = (is_v ? a.c.v : a.c.k) + id * a.c.page_stride + (size_t)kvh * a.c.page * D;
-  uint8_t *exp = (is_v ? a.c.v_exp : a.c.k_exp) + id * a.c.exp_stride + kvh;
   const int head = a.H + (is_v ? a.c.KV : 0) + kvh, s0 = lo - (o << a.c.lg_page);
-  const int work = (hi - lo) * per;
+  const int step = blockDim.x / per;  // tokens apart
+  const int t0 = threadIdx.x / per;
+  // the thread's elements of token t of the block, k turned
+  auto load = [&](int t, float (&x1)[V], float (&x2)[V]) {
+    load_pair<T, D>(a, r0 + lo - pos + t, head, d, x1, x2);
+    if (!is_v) {
+      float c[V], s[V];
+      load_row<V>(a.cos_t + (size_t)(lo + t) * half + d, c, true);
+      load_row<V>(a.sin_t + (size_t)(lo + t) * half + d, s, true);
+      turn<V>(x1, x2, c, s);
+    }
+  };
   float amax = 0.f;
-  for (int e = threadIdx.x; e < work; e += THREADS) {
-    float x1[4], x2[4];
-    const int t = e / per;
-    load_pair<T>(a, r0 + lo - pos + t, head, (e % per) * 4, lo + t, !is_v, x1, x2);
+#pragma unroll 2
+  for (int t = t0; t < hi - lo; t += step) {
+    float x1[V], x2[V];
+    load(t, x1, x2);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float m = fmaxf(fabsf(x1[j]), fabsf(x2[j]));
-      if (x1[j] != x1[j] || x2[j] != x2[j]) amax = __uint_as_float(0x7f800000u);
-      else amax = fmaxf(amax, m);
+    for (int k = 0; k < V; ++k) {
+      amax = fmaxf(amax, fmaxf(fabsf(x1[k]), fabsf(x2[k])));
+      if (x1[k] != x1[k] || x2[k] != x2[k]) amax = INFINITY;
     }
   }
+  if (id < 0) return;  // (asked only now: the rows are loaded meanwhile)
+  int8_t *codes = (is_v ? a.c.v : a.c.k) + id * a.c.page_stride + (size_t)kvh * a.c.page * D;
+  uint8_t *exp = (is_v ? a.c.v_exp : a.c.k_exp) + id * a.c.exp_stride + kvh;
   const int e_old = s0 == 0 ? 0 : *exp;
   amax = block_max(amax, red);  // its barrier also orders the read of *exp before the store below
   const int e_new = max(e_old, scale_byte(amax));
@@ -198,7 +292,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
   if (e_new > e_old && s0 > 0) {
     const float f = pow2_e8m0(max(127 + e_old - e_new, 1));  // 2^(e_old - e_new); below 2^-8 every code is 0 anyway
     uint32_t *w = reinterpret_cast<uint32_t *>(codes);
-    for (int e = threadIdx.x; e < s0 * D / 4; e += THREADS) {
+    for (int e = threadIdx.x; e < s0 * D / 4; e += blockDim.x) {
       const uint32_t u = w[e];
       float x[4];
 #pragma unroll
@@ -207,37 +301,73 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     }
   }
   const float inv = e_new == 255 ? 0.f : pow2_inverse(e_new);
-  for (int e = threadIdx.x; e < work; e += THREADS) {
-    float x1[4], x2[4];
-    const int t = e / per, d = (e % per) * 4;
-    load_pair<T>(a, r0 + lo - pos + t, head, d, lo + t, !is_v, x1, x2);
-    uint32_t *dst = reinterpret_cast<uint32_t *>(codes + (size_t)(s0 + t) * D + d);
-    dst[0] = e_new == 255 ? 0 : pack4(x1, inv, top);
-    dst[half / 4] = e_new == 255 ? 0 : pack4(x2, inv, top);
+#pragma unroll 2
+  for (int t = t0; t < hi - lo; t += step) {
+    float x1[V], x2[V];
+    load(t, x1, x2);
+    if (e_new == 255) {  // the block is NaN: its codes do not matter
+#pragma unroll
+      for (int k = 0; k < V; ++k) x1[k] = x2[k] = 0.f;
+    }
+    int8_t *dst = codes + (size_t)(s0 + t) * D + d;
+    store_codes<V>(dst, x1, inv, top);
+    store_codes<V>(dst + half, x2, inv, top);
   }
   if (threadIdx.x == 0) *exp = (uint8_t)e_new;
 }
 
-// one CTA per (page of the list, head), keys then values
+// One CTA per (page of the list, head): a thread's loads of keys and values are
+// all in flight before its first store; every store is 16 bytes, in lane order.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) read_kernel(Pool c, const int32_t *ids, T *k_out, T *v_out, int *status) {
-  const int i = blockIdx.x / c.KV, kvh = blockIdx.x % c.KV, n4 = c.page * c.D / 4;
-  const int id = ids[i];
+  constexpr int V = VEC<T>, FLY = 4;
+  const int kvh = blockIdx.x % c.KV, n = c.page * c.D / V;
+  const int id = ids[blockIdx.x / c.KV];
   const bool ok = id >= 0 && id < c.pages;
   if (!ok && threadIdx.x == 0) set_status(status, LBC_ERR_PAGE);
-  for (int s = 0; s < 2; ++s) {
-    T *out = (s ? v_out : k_out) + (size_t)blockIdx.x * c.page * c.D;
-    const size_t at = ok ? id * c.page_stride + (size_t)kvh * c.page * c.D : 0;
-    const uint32_t *w = reinterpret_cast<const uint32_t *>((s ? c.v : c.k) + at);
-    const float f = ok ? pow2_e8m0((s ? c.v_exp : c.k_exp)[id * c.exp_stride + kvh]) : 0.f;
-    for (int e = threadIdx.x; e < n4; e += THREADS) {
-      const uint32_t u = ok ? w[e] : 0;
-      float x[4];
+  const size_t at = ok ? id * c.page_stride + (size_t)kvh * c.page * c.D : 0;
+  const float f[2] = {ok ? pow2_e8m0(c.k_exp[id * c.exp_stride + kvh]) : 0.f, ok ? pow2_e8m0(c.v_exp[id * c.exp_stride + kvh]) : 0.f};
+  T *out[2] = {k_out + (size_t)blockIdx.x * c.page * c.D, v_out + (size_t)blockIdx.x * c.page * c.D};
+  for (int e0 = threadIdx.x; e0 < n; e0 += FLY * THREADS) {
+    uint32_t w[2][FLY][V / 4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = __fmul_rn((float)(int8_t)(u >> (8 * j)), f);
-      store4<T>(out + 4 * (size_t)e, x);
-    }
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int u = 0; u < FLY; ++u) {
+        const int e = e0 + u * THREADS;
+        const int8_t *src = (s ? c.v : c.k) + at + (size_t)e * V;
+        if (e < n) {
+          if constexpr (V == 8) {
+            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(src));
+            w[s][u][0] = y.x;
+            w[s][u][1] = y.y;
+          } else {
+            w[s][u][0] = __ldg(reinterpret_cast<const uint32_t *>(src));
+          }
+        }
+      }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int u = 0; u < FLY; ++u) {
+        const int e = e0 + u * THREADS;
+        if (e < n) {
+          float x[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) x[j] = ok ? __fmul_rn((float)(int8_t)(w[s][u][j / 4] >> (8 * (j % 4))), f[s]) : 0.f;
+          store16<T>(out[s] + (size_t)e * V, x);
+        }
+      }
   }
+}
+
+template <typename T>
+void launch_append(const AppendArgs &a, long long kv_ctas, cudaStream_t st) {
+  // 16 threads a token and more: up to 4 tokens need no more than 64
+  const unsigned threads = a.r.most <= 4 ? 64 : THREADS, ctas = (unsigned)(kv_ctas + (a.r.N + threads / 32 - 1) / (threads / 32));
+  if (a.c.D == 32) append_kernel<T, 32><<<ctas, threads, 0, st>>>(a);
+  else if (a.c.D == 64) append_kernel<T, 64><<<ctas, threads, 0, st>>>(a);
+  else append_kernel<T, 128><<<ctas, threads, 0, st>>>(a);
 }
 
 }  // namespace
@@ -269,12 +399,12 @@ int lbc_kv8_append(const lbc_kv8 *c, int dtype, const void *qkv, long long ld, c
   a.qkv = qkv; a.ld = ld; a.bias = bias; a.cos_t = cos_t; a.sin_t = sin_t;
   a.positions = positions; a.H = H; a.q_out = q_out;
   a.slots = (max_tokens + a.c.page - 2) / a.c.page + 1;
-  const long long ctas = 2LL * a.c.KV * a.slots * B + N;
-  if (ctas > 0x7fffffffLL) return refuse("kv8_append: too many rows");
+  const long long ctas = 2LL * a.c.KV * a.slots * B;
+  if (ctas + N > 0x7fffffffLL) return refuse("kv8_append: too many rows");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == LBC_F32) append_kernel<float><<<(unsigned)ctas, THREADS, 0, st>>>(a);
-  else if (dtype == LBC_BF16) append_kernel<__nv_bfloat16><<<(unsigned)ctas, THREADS, 0, st>>>(a);
-  else append_kernel<__half><<<(unsigned)ctas, THREADS, 0, st>>>(a);
+  if (dtype == LBC_F32) launch_append<float>(a, ctas, st);
+  else if (dtype == LBC_BF16) launch_append<__nv_bfloat16>(a, ctas, st);
+  else launch_append<__half>(a, ctas, st);
   return launched("kv8_append");
 }
 

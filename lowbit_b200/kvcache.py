@@ -34,6 +34,7 @@ import torch
 
 from .kernels import _check, _raw_stream, lib
 
+_device = torch._C._cuda_getDevice
 PAGES = (16, 32, 64, 128)
 HEAD_DIMS = (32, 64, 128)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -153,24 +154,28 @@ def kv8_append(qkv, cache: KV8Cache, table, pos, cos, sin, bias=None, starts=Non
     heads = w // d - 2 * kv
     if heads <= 0 or w % d or heads % kv:
         raise ValueError(f"qkv has {w} columns: not (H + 2*{kv}) * {d} with H a multiple of {kv}")
-    for t in (cos, sin):
-        if t.dim() != 2 or t.shape[1] != d // 2 or t.dtype != torch.float32 or not t.is_contiguous() \
-                or t.device != dev or t.shape != cos.shape or t.data_ptr() % 16:
-            raise ValueError("cos and sin must be contiguous fp32 [positions, head_dim/2] tensors on the cache's device")
-    if bias is not None and (bias.shape != (w,) or bias.dtype != torch.float32 or not bias.is_contiguous()
+    f32 = torch.float32
+    if cos.dim() != 2 or cos.shape[1] * 2 != d or cos.dtype is not f32 or not cos.is_contiguous() or cos.device != dev \
+            or sin.shape != cos.shape or sin.dtype is not f32 or not sin.is_contiguous() or sin.device != dev:
+        raise ValueError("cos and sin must be contiguous fp32 [positions, head_dim/2] tensors on the cache's device")
+    if (cos.data_ptr() | sin.data_ptr()) % 16:
+        raise ValueError("cos and sin must be 16-byte aligned")
+    if bias is not None and (bias.shape != (w,) or bias.dtype is not f32 or not bias.is_contiguous()
                              or bias.device != dev):
         raise ValueError("bias must be a contiguous fp32 tensor of qkv's width")
     width, b, most, sp = _rows(cache, n, table, pos, starts, max_tokens)
     q = qkv.new_empty((n, heads, d)) if out is None else _out(out, (n, heads, d), qkv.dtype, dev)
     if n == 0:
         return q
-    if torch.cuda.current_device() != dev.index:
+    if _device() != dev.index:
         with torch.cuda.device(dev):
             return kv8_append(qkv, cache, table, pos, cos, sin, bias, starts, max_tokens, q)
     qkv = _aligned_rows(qkv, (1,))
-    _check(lib().lbc_kv8_append(cache._ref, _DTYPES[qkv.dtype], qkv.data_ptr(), qkv.stride(0), _ptr(bias),
-                                cos.data_ptr(), sin.data_ptr(), cos.shape[0], table.data_ptr(), width, pos.data_ptr(),
-                                sp, b, n, most, heads, q.data_ptr(), _raw_stream(dev.index)), "lbc_kv8_append")
+    rc = lib().lbc_kv8_append(cache._ref, _DTYPES[qkv.dtype], qkv.data_ptr(), qkv.stride(0), _ptr(bias), cos.data_ptr(),
+                              sin.data_ptr(), cos.shape[0], table.data_ptr(), width, pos.data_ptr(), sp, b, n, most,
+                              heads, q.data_ptr(), _raw_stream(dev.index))
+    if rc < 0:
+        _check(rc, "lbc_kv8_append")
     return q
 
 
@@ -196,7 +201,7 @@ def kv8_attention(q, cache: KV8Cache, table, pos, starts=None, max_tokens: int |
         y = _out(out, (n, heads, d), q.dtype, dev)
     if n == 0:
         return y
-    if torch.cuda.current_device() != dev.index:
+    if _device() != dev.index:
         with torch.cuda.device(dev):
             return kv8_attention(q, cache, table, pos, starts, max_tokens, window, scale, y)
     q = _aligned_rows(q, (d, 1))
@@ -230,7 +235,7 @@ def kv8_read(cache: KV8Cache, pages, dtype=torch.bfloat16):
     v = torch.empty_like(k)
     if n == 0:
         return k, v
-    if torch.cuda.current_device() != dev.index:
+    if _device() != dev.index:
         with torch.cuda.device(dev):
             return kv8_read(cache, pages, dtype)
     _check(lib().lbc_kv8_read(cache._ref, _DTYPES[dtype], pages.data_ptr(), n, k.data_ptr(), v.data_ptr(),

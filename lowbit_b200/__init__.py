@@ -9,7 +9,7 @@ from .formats import (GROUP, MXBLOCK, AMXInt4Weights, Int4Weights, Int8Acts, MXF
 from .kernels import (Params, amx_available, cpu_info, gemm_mxfp4, gemm_w4a8, gemm_w4a8_amx, gemm_w4a16,
                       gpu_info, w4a8_group_acc_amx)
 
-_KVCACHE = ("KV8Cache", "kv8_append", "kv8_attention", "kv8_read")
+_KVCACHE = ("KV8Cache", "PagedKVCache", "kv8_append", "kv8_attention", "kv8_read")
 
 
 def __getattr__(name):

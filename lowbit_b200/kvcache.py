@@ -241,3 +241,80 @@ def kv8_read(cache: KV8Cache, pages, dtype=torch.bfloat16):
     _check(lib().lbc_kv8_read(cache._ref, _DTYPES[dtype], pages.data_ptr(), n, k.data_ptr(), v.data_ptr(),
                               _raw_stream(dev.index)), "lbc_kv8_read")
     return k, v
+
+
+class PagedKVCache:
+    """The model's cache over KV8Cache pools: one pool a layer, one page table
+    and one position a sequence, shared by the layers. Sequences have lengths
+    of their own. Pages are handed out from a free list as sequences grow
+    (``reserve``) and go back with ``release``.
+
+    Interface of model.KVCache: ``batch``, ``capacity``, ``pos`` (int32 [batch]
+    on the GPU), ``length`` (sequences of equal length), ``reset()``."""
+
+    def __init__(self, cfg, max_len: int, batch: int = 1, page: int = 64, pages: int | None = None):
+        if batch <= 0 or max_len <= 0:
+            raise ValueError("a cache holds at least one sequence of one token")
+        width = -(-max_len // page)
+        self.batch, self.page, self._max_len = batch, page, max_len
+        n = batch * width if pages is None else int(pages)
+        self.layers = [KV8Cache.empty(n, cfg.num_kv_heads, cfg.head_dim, page) for _ in range(cfg.num_layers)]
+        dev = self.layers[0].device
+        self.table = torch.zeros((batch, width), dtype=torch.int32, device=dev)
+        self.pos = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.lengths = [0] * batch
+        self._owned = [[] for _ in range(batch)]
+        self._free = list(range(n - 1, -1, -1))
+
+    @property
+    def capacity(self) -> int:
+        return self._max_len
+
+    @property
+    def nbytes(self) -> int:
+        return sum(c.nbytes for c in self.layers)
+
+    def reserve(self, tokens) -> None:
+        """Pages for ``tokens[b]`` tokens of every sequence (an int: the same
+        for all); raises ValueError, with nothing changed, when they do not fit."""
+        tokens = [int(tokens)] * self.batch if isinstance(tokens, int) else [int(t) for t in tokens]
+        if len(tokens) != self.batch:
+            raise ValueError(f"{len(tokens)} lengths for {self.batch} sequences")
+        if max(tokens) > self._max_len:
+            raise ValueError(f"KV cache full ({max(tokens)} > {self._max_len})")
+        more = [max(0, -(-t // self.page) - len(own)) for t, own in zip(tokens, self._owned)]
+        if sum(more) > len(self._free):
+            raise ValueError(f"KV cache out of pages ({sum(more)} needed, {len(self._free)} free)")
+        if not any(more):
+            return
+        for own, m in zip(self._owned, more):
+            own.extend(self._free.pop() for _ in range(m))
+        host = torch.zeros(self.table.shape, dtype=torch.int32)
+        for b, own in enumerate(self._owned):
+            host[b, :len(own)] = torch.tensor(own, dtype=torch.int32)
+        self.table.copy_(host)
+
+    def release(self, b: int) -> None:
+        """Empty sequence b and return its pages."""
+        self._free.extend(reversed(self._owned[b]))
+        self._owned[b] = []
+        self.lengths[b] = 0
+        self.pos[b] = 0
+
+    @property
+    def length(self) -> int:
+        if len(set(self.lengths)) > 1:
+            raise ValueError("the sequences have different lengths (see lengths)")
+        return self.lengths[0]
+
+    @length.setter
+    def length(self, n: int) -> None:
+        self.set_lengths([int(n)] * self.batch)
+
+    def set_lengths(self, lengths) -> None:
+        self.lengths = [int(n) for n in lengths]
+        self.pos.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+
+    def reset(self) -> None:
+        """Empty every sequence (pools, table and pages stay, so a captured decode graph stays valid)."""
+        self.length = 0

@@ -20,7 +20,11 @@ through the host quantizer.
 
 Beyond the reference: several sequences of equal length decode together
 (generate_batch): their rows share every GEMM, so the weights stream once
-per step for the whole batch.
+per step for the whole batch. With a paged 8-bit cache (new_cache(...,
+kind="kv8"), lowbit_b200.kvcache) the keys and values take a quarter of the
+bytes and the sequences may differ in length (generate_ragged): RoPE and the
+append run as one kernel (lbc_kv8_append), attention reads the pages
+(lbc_kv8_attention).
 """
 from __future__ import annotations
 
@@ -636,21 +640,31 @@ class Model:
         for x in self.linears():
             x.threads = threads
 
-    def new_cache(self, max_len: int, batch: int = 1) -> KVCache:
-        return KVCache(self.cfg, max_len, batch)
+    def new_cache(self, max_len: int, batch: int = 1, kind: str = "fp32", page: int = 64):
+        """A cache of `batch` sequences of up to `max_len` tokens: kind "fp32"
+        (KVCache) or "kv8" (kvcache.PagedKVCache: int8 codes in pages of `page` tokens)."""
+        if kind == "fp32":
+            return KVCache(self.cfg, max_len, batch)
+        if kind != "kv8":
+            raise ValueError(f"cache kind must be 'fp32' or 'kv8', not {kind!r}")
+        from .kvcache import PagedKVCache
+        return PagedKVCache(self.cfg, max_len, batch, page)
 
     # ------------------------------------------------------------ forward
 
-    def _run(self, tok, B: int, T: int, cache: KVCache, logits: str, head_chunk: int = 256):
+    def _run(self, tok, B: int, T: int, cache, logits: str, head_chunk: int = 256, starts=None):
         """Device forward of B sequences x T tokens (rows b*T + t) at positions
         cache.pos..; returns device logits ([B, V] last, [B*T, V] all) or the
-        final hidden states [B*T, hidden] for logits="none"."""
+        final hidden states [B*T, hidden] for logits="none". With a paged cache
+        and `starts` (int32 [B + 1] on the GPU) sequence b has rows
+        starts[b]..starts[b+1]-1, at most T."""
         torch = _torch()
         cfg = self.cfg
         lib, st = _lib(), _stream()
         H, KV, D, hid, I = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.hidden_size, cfg.intermediate_size
-        n = B * T
+        n = B * T if starts is None else int(tok.shape[0])
         eps = float(cfg.rms_norm_eps)
+        paged = not isinstance(cache, KVCache)
         S = cache.capacity
         P = self.prof
         with P.section("other"):
@@ -679,7 +693,14 @@ class Model:
                     qkv = L.qkv.mm(h)
             bias = None if L.qkv.b is None else L.qkv.b.data_ptr()
             with P.section("attention"):
-                if T == 1:  # one launch: RoPE, cache append and attention
+                if paged:
+                    from . import kvcache as KC
+                    lay = cache.layers[li]
+                    qr = KC.kv8_append(qkv, lay, cache.table, cache.pos, self.cos, self.sin, bias=L.qkv.b,
+                                       starts=starts, max_tokens=T)
+                    KC.kv8_attention(qr, lay, cache.table, cache.pos, starts=starts, max_tokens=T,
+                                     out=att.view(n, H, D))
+                elif T == 1:  # one launch: RoPE, cache append and attention
                     _check(lib.lbc_rope_attention(qkv.data_ptr(), bias, self.cos.data_ptr(), self.sin.data_ptr(),
                                                   cache.pos.data_ptr(), cache.k[li].data_ptr(),
                                                   cache.v[li].data_ptr(), att.data_ptr(), B, H, KV, D, S, st),
@@ -717,7 +738,9 @@ class Model:
             return xn
         with P.section("lm_head"):
             if logits == "last":
-                return self.lm_head(xn.view(B, T, hid)[:, T - 1].contiguous())
+                last = xn.view(B, T, hid)[:, T - 1].contiguous() if starts is None \
+                    else xn.index_select(0, starts[1:].long() - 1)
+                return self.lm_head(last)
             return torch.cat([self.lm_head(xn[i:i + head_chunk]) for i in range(0, n, head_chunk)])
 
     def forward(self, tokens, cache: KVCache | None = None, logits: str = "last",
@@ -734,6 +757,8 @@ class Model:
             raise ValueError("forward() runs one sequence; use generate_batch for several")
         if cache.length + T > cache.capacity:
             raise ValueError(f"KV cache full ({cache.length}+{T} > {cache.capacity})")
+        if not isinstance(cache, KVCache):
+            cache.reserve(cache.length + T)
         tok = torch.from_numpy(tokens).to("cuda")
         out = self._run(tok, 1, T, cache, logits, head_chunk)
         self.prof.close()
@@ -760,9 +785,11 @@ class Model:
         s = self._gstream
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):  # warm-up outside capture: workspaces, plans, cuBLAS handles
-            saved = int(cache.pos.item())
+            saved = cache.pos.clone()
+            if not isinstance(cache, KVCache):
+                cache.pos.fill_(-1)  # a padding step: a block's scale must not grow for a made-up token
             self._step(tok, cache)
-            cache.pos.fill_(saved)
+            cache.pos.copy_(saved)
         g = torch.cuda.CUDAGraph()
         self.prof.collect()  # the warm-up step's sections, before the capture
         with self.prof.capturing() as marks:
@@ -788,7 +815,10 @@ class Model:
         logit = self._run(tok, cache.batch, 1, cache, "last")
         with self.prof.section("other"):
             tok.copy_(torch.argmax(logit, dim=-1))
-            _check(_lib().lbc_advance_pos(cache.pos.data_ptr(), 1, _stream()), "lbc_advance_pos")
+            if isinstance(cache, KVCache):
+                _check(_lib().lbc_advance_pos(cache.pos.data_ptr(), 1, _stream()), "lbc_advance_pos")
+            else:
+                cache.pos.add_(1)  # one position a sequence
         self.prof.close()
 
     def generate(self, prompt, n_new: int, cache: KVCache | None = None, timings: dict | None = None,
@@ -802,7 +832,6 @@ class Model:
                        graph: bool = True) -> np.ndarray:
         """Greedy decoding of B equal-length prompts together: [B, n_new] tokens.
         Each sequence's logits equal those of decoding it alone."""
-        torch = _torch()
         prompts = np.asarray(prompts, np.int64)
         if prompts.ndim != 2:
             raise ValueError("prompts must be [B, T] (equal lengths)")
@@ -810,13 +839,50 @@ class Model:
         cache = cache or self.new_cache(T0 + n_new, batch=B)
         if cache.batch != B:
             raise ValueError(f"cache holds {cache.batch} sequences, prompts {B}")
+        if not isinstance(cache, KVCache):
+            return np.asarray(self.generate_ragged(prompts, n_new, cache, timings, graph))
         if cache.length + T0 + max(0, n_new - 1) > cache.capacity:
             raise ValueError("KV cache too short for prompt + n_new")
+        return self._generate(prompts.reshape(-1), B, T0, None, n_new, cache, timings, graph)
+
+    def generate_ragged(self, prompts, n_new: int, cache=None, timings: dict | None = None,
+                        graph: bool = True) -> list[list[int]]:
+        """Greedy decoding of prompts of any lengths together over a paged 8-bit
+        cache (a new one by default): n_new tokens each. Sequences that already
+        hold tokens in `cache` are continued."""
+        torch = _torch()
+        prompts = [np.asarray(p, np.int64).reshape(-1) for p in prompts]
+        if not prompts or any(len(p) == 0 for p in prompts):
+            raise ValueError("every prompt needs at least one token")
+        B, lens = len(prompts), [len(p) for p in prompts]
+        if cache is None:
+            cache = self.new_cache(max(lens) + max(n_new, 1), batch=B, kind="kv8")
+        if isinstance(cache, KVCache):
+            raise ValueError("prompts of different lengths need a paged cache (new_cache(kind='kv8'))")
+        if cache.batch != B:
+            raise ValueError(f"cache holds {cache.batch} sequences, prompts {B}")
+        cache.reserve([h + t + max(0, n_new - 1) for h, t in zip(cache.lengths, lens)])
+        starts = None
+        if len(set(lens)) > 1:
+            starts = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+        out = self._generate(np.concatenate(prompts), B, max(lens), starts, n_new, cache, timings, graph, lens)
+        return [[int(t) for t in row] for row in out]
+
+    def _generate(self, tokens, B: int, T0: int, starts, n_new: int, cache, timings, graph: bool, lens=None):
+        """Prefill of `tokens` (B sequences of up to T0), then n_new - 1 decode steps: [B, n_new]."""
+        torch = _torch()
+
+        def grow(k):  # k tokens more a sequence, or the prompts' own lengths
+            if isinstance(cache, KVCache):
+                cache.length = cache.length + k
+            else:
+                cache.set_lengths([a + b for a, b in zip(cache.lengths, lens if k is None else [k] * B)])
+
         hist = torch.empty((max(n_new, 1), B), dtype=torch.int64, device="cuda")
         torch.cuda.synchronize()
         t0 = time.perf_counter()
-        logit = self._run(torch.from_numpy(prompts.reshape(-1)).to("cuda"), B, T0, cache, "last")
-        cache.length = cache.length + T0
+        logit = self._run(torch.from_numpy(np.ascontiguousarray(tokens)).to("cuda"), B, T0, cache, "last", starts=starts)
+        grow(T0 if lens is None else None)
         if n_new > 0:
             with self.prof.section("other"):
                 hist[0].copy_(torch.argmax(logit, dim=-1))
@@ -840,7 +906,11 @@ class Model:
                 for i in range(1, n_new):
                     self._step(tok, cache)
                     hist[i].copy_(tok)
-            cache._length += n_new - 1  # the device position advanced inside the steps
+            # the device positions advanced inside the steps
+            if isinstance(cache, KVCache):
+                cache._length += n_new - 1
+            else:
+                cache.lengths = [n + n_new - 1 for n in cache.lengths]
         out = hist[:n_new].T.cpu().numpy()
         t2 = time.perf_counter()
         if timings is not None:

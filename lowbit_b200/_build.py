@@ -3,7 +3,9 @@
 The library is compiled in-tree with nvcc (one object per .cu, compiled in
 parallel, linked with the static CUDA runtime) and loaded with ctypes. The
 build output name does not change; a stamp file holding a hash of the sources
-and flags decides whether a rebuild is needed.
+and flags decides whether a rebuild is needed. build_torch() compiles the
+torch side of the KV-cache calls (csrc/kv8_torch.cpp, a CPython module on
+torch's C++ headers) the same way.
 
 Environment:
   NVCC               nvcc binary (default: $CUDA_HOME/bin/nvcc or nvcc on PATH)
@@ -24,6 +26,9 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB = PKG / "liblowbit_b200.so"
 STAMP = PKG / ".liblowbit_b200.stamp"
+TORCH_SRC = CSRC / "kv8_torch.cpp"
+TORCH_LIB = PKG / "_kv8_torch.so"
+TORCH_STAMP = PKG / "_build" / "kv8_torch.stamp"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # no fast-math: the activation quantizer relies on IEEE division and rint
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
@@ -96,5 +101,36 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     return LIB
 
 
+def build_torch(force: bool = False) -> Path:
+    """Compile (if needed) and return the path of the _kv8_torch module."""
+    import sysconfig
+
+    import torch
+    h = hashlib.sha256()
+    for p in (TORCH_SRC, INCLUDE / "lowbit_b200.h"):
+        h.update(p.read_bytes())
+    h.update(f"{torch.__version__} {sys.version}".encode())
+    digest = h.hexdigest()[:16]
+    if not force and TORCH_LIB.exists() and TORCH_STAMP.exists() and TORCH_STAMP.read_text().strip() == digest:
+        return TORCH_LIB
+    root = Path(torch.__file__).parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+           sysconfig.get_paths()["include"]]
+    TORCH_STAMP.parent.mkdir(exist_ok=True)
+    tmp = TORCH_LIB.with_suffix(f".so.tmp{os.getpid()}")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in inc), str(TORCH_SRC),
+           "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
+           "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{TORCH_SRC.name}: build failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+    TORCH_STAMP.write_text(digest)
+    return TORCH_LIB
+
+
 if __name__ == "__main__":
     print(build(verbose=True, force="--force" in sys.argv))
+    print(build_torch(force="--force" in sys.argv))

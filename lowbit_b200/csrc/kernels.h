@@ -1,6 +1,7 @@
 // Internal launcher declarations (not part of the public C ABI).
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -63,6 +64,18 @@ int tc_gemm(const TcCall &c, cudaStream_t st, char *err, size_t errlen);
 // 0 when the current device is sm_100 (with its status block and SM count), else a
 // negative LBC_ERR_* with the text recorded
 int device_ready(int **status, int *sms);
+
+// raises a kernel's dynamic shared memory limit to `smem` bytes, once a device
+// (`done`: a static of the kernel's launcher, a bit a device)
+template <typename K>
+inline void allow_smem(K *kernel, int smem, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess)
+    done.fetch_or(bit, std::memory_order_release);
+}
 
 // records `msg` as the text lbc_last_error() returns on this thread
 void set_last_error(const char *msg);

@@ -701,7 +701,8 @@ Plan plan_of(const Pool &c, int width, int B, int most, int H, int window, int s
 template <typename T, int D, int NQ>
 void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {
   constexpr int smem = std::max(WARPS * STAGES * HT * Warp<T, D, NQ>::STEP, (int)sizeof(float) * WARPS * 8 * NQ * (D + 4));
-  if (smem > 40 * 1024) cudaFuncSetAttribute(attention_kernel<T, D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(attention_kernel<T, D, NQ>, smem, allowed);
   cudaLaunchAttribute attr{};
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.grid);

@@ -557,7 +557,8 @@ template <typename T, int D>
 void launch(const AttnArgs &a, cudaStream_t st) {
   constexpr int smem = Lay<T, D>::SMEM;
   static_assert(smem <= 227 * 1024, "operand tiles fit an SM's shared memory");
-  cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(prompt_kernel<T, D>, smem, allowed);
   const unsigned tiles = (unsigned)(((long long)a.r.most * a.G + Lay<T, D>::ROWS - 1) / Lay<T, D>::ROWS);
   prompt_kernel<T, D><<<dim3(a.c.KV, a.r.B, tiles), THREADS, smem, st>>>(a);
 }

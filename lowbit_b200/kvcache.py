@@ -32,12 +32,30 @@ import ctypes as C
 
 import torch
 
-from .kernels import _check, _raw_stream, lib
+from .kernels import lib
 
-_device = torch._C._cuda_getDevice
 PAGES = (16, 32, 64, 128)
 HEAD_DIMS = (32, 64, 128)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_native = None  # csrc/kv8_torch.cpp, loaded on first use
+
+
+def _load():
+    """The native module (argument checks, allocation and the C ABI call), bound to the loaded library."""
+    global _native
+    from importlib.machinery import ExtensionFileLoader
+    from importlib.util import module_from_spec, spec_from_loader
+
+    from ._build import build_torch
+    loader = ExtensionFileLoader("_kv8_torch", str(build_torch()))
+    mod = module_from_spec(spec_from_loader("_kv8_torch", loader))
+    loader.exec_module(mod)
+    L = lib()
+    mod.init(*(C.cast(getattr(L, f), C.c_void_p).value
+               for f in ("lbc_kv8_append", "lbc_kv8_attention", "lbc_kv8_attention_workspace", "lbc_kv8_read",
+                         "lbc_last_error")))
+    _native = mod
+    return mod
 
 
 class _KV8(C.Structure):
@@ -53,8 +71,8 @@ class KV8Cache:
     multiple of 16 bytes, the same for k and v); within a page the layout is
     contiguous."""
 
-    __slots__ = ("k", "v", "k_exp", "v_exp", "device", "pages", "kv_heads", "page", "head_dim", "_c", "_ref",
-                 "_scratch")
+    __slots__ = ("k", "v", "k_exp", "v_exp", "device", "pages", "kv_heads", "page", "head_dim", "_c", "_at",
+                 "_index")
 
     def __init__(self, k, v, k_exp, v_exp):
         if k.dim() != 4 or v.shape != k.shape or k.dtype != torch.int8 or v.dtype != torch.int8:
@@ -80,8 +98,7 @@ class KV8Cache:
         self.device, self.pages, self.kv_heads, self.page, self.head_dim = k.device, pages, kv, page, d
         self._c = _KV8(k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), stride,
                        k_exp.stride(0) if pages > 1 else kv, pages, page, kv, d)
-        self._ref = C.byref(self._c)
-        self._scratch = {}  # workspace bytes of attention calls, by their sizes
+        self._at, self._index = C.addressof(self._c), k.device.index
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page: int = 64, device=None) -> "KV8Cache":
@@ -97,86 +114,14 @@ class KV8Cache:
         return 2 * self.pages * self.kv_heads * (self.page * self.head_dim + 1)
 
 
-def _rows(cache, n, table, pos, starts, max_tokens):
-    """Checks the row description; (width, B, max_tokens, starts pointer)."""
-    dev, i32 = cache.device, torch.int32
-    if table.dim() != 2 or table.dtype is not i32 or not table.is_contiguous() or table.device != dev:
-        raise ValueError("table must be a contiguous int32 [B, pages] tensor on the cache's device")
-    b, width = table.shape
-    if pos.dim() != 1 or len(pos) != b or pos.dtype is not i32 or not pos.is_contiguous() or pos.device != dev:
-        raise ValueError("pos must be a contiguous int32 [B] tensor on the cache's device")
-    if b == 0 or width == 0:
-        raise ValueError("table must hold at least one sequence and one page")
-    if starts is None:
-        if n % b:
-            raise ValueError(f"{n} rows do not divide over {b} sequences; give starts")
-        most = n // b
-        if max_tokens is not None and max_tokens < most:
-            raise ValueError(f"max_tokens {max_tokens} is below the {most} rows of a sequence")
-        return width, b, most, None
-    if starts.shape != (b + 1,) or starts.dtype != torch.int32 or not starts.is_contiguous() or starts.device != dev:
-        raise ValueError("starts must be a contiguous int32 [B + 1] tensor on the cache's device")
-    most = n if max_tokens is None else min(int(max_tokens), n)
-    if most < 0:
-        raise ValueError("max_tokens must not be negative")
-    return width, b, most, starts.data_ptr()
-
-
-def _out(out, shape, dtype, device):
-    if out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous() \
-            or out.data_ptr() % 16:
-        raise ValueError(f"out must be a contiguous, 16-byte aligned {dtype} tensor of shape {tuple(shape)}")
-    return out
-
-
-def _aligned_rows(x, inner: tuple):
-    """x with its dimensions after the first contiguous and 16-byte aligned rows."""
-    if x.stride()[1:] == inner and x.data_ptr() % 16 == 0 and x.stride(0) * x.element_size() % 16 == 0 \
-            and x.stride(0) >= inner[0] * x.shape[1]:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
 def kv8_append(qkv, cache: KV8Cache, table, pos, cos, sin, bias=None, starts=None, max_tokens: int | None = None,
                out=None):
     """Append the k and v of fused rows ``qkv`` [N, (H + 2*KV)*D] (fp32, bf16 or
-    fp16; + ``bias`` fp32) to the cache and return q rotated [N, H, D] in
-    qkv's type. cos, sin: fp32 [positions, D/2] (model.rope_tables).
-    ``max_tokens`` bounds the rows of a sequence when ``starts`` is given."""
-    kv, d, dev = cache.kv_heads, cache.head_dim, cache.device
-    if qkv.dim() != 2 or qkv.dtype not in _DTYPES or qkv.device != dev:
-        raise ValueError("qkv must be an fp32, bf16 or fp16 [N, (H + 2*KV)*D] tensor on the cache's device")
-    n, w = qkv.shape
-    heads = w // d - 2 * kv
-    if heads <= 0 or w % d or heads % kv:
-        raise ValueError(f"qkv has {w} columns: not (H + 2*{kv}) * {d} with H a multiple of {kv}")
-    f32 = torch.float32
-    if cos.dim() != 2 or cos.shape[1] * 2 != d or cos.dtype is not f32 or not cos.is_contiguous() or cos.device != dev \
-            or sin.shape != cos.shape or sin.dtype is not f32 or not sin.is_contiguous() or sin.device != dev:
-        raise ValueError("cos and sin must be contiguous fp32 [positions, head_dim/2] tensors on the cache's device")
-    if (cos.data_ptr() | sin.data_ptr()) % 16:
-        raise ValueError("cos and sin must be 16-byte aligned")
-    if bias is not None and (bias.shape != (w,) or bias.dtype is not f32 or not bias.is_contiguous()
-                             or bias.device != dev):
-        raise ValueError("bias must be a contiguous fp32 tensor of qkv's width")
-    width, b, most, sp = _rows(cache, n, table, pos, starts, max_tokens)
-    q = qkv.new_empty((n, heads, d)) if out is None else _out(out, (n, heads, d), qkv.dtype, dev)
-    if n == 0:
-        return q
-    if _device() != dev.index:
-        with torch.cuda.device(dev):
-            return kv8_append(qkv, cache, table, pos, cos, sin, bias, starts, max_tokens, q)
-    qkv = _aligned_rows(qkv, (1,))
-    rc = lib().lbc_kv8_append(cache._ref, _DTYPES[qkv.dtype], qkv.data_ptr(), qkv.stride(0), _ptr(bias), cos.data_ptr(),
-                              sin.data_ptr(), cos.shape[0], table.data_ptr(), width, pos.data_ptr(), sp, b, n, most,
-                              heads, q.data_ptr(), _raw_stream(dev.index))
-    if rc < 0:
-        _check(rc, "lbc_kv8_append")
-    return q
+    fp16; + ``bias`` fp32; rows may lie apart) to the cache and return q rotated
+    [N, H, D] in qkv's type. cos, sin: fp32 [positions, D/2] (model.rope_tables).
+    ``max_tokens`` bounds the rows of a sequence when ``starts`` is given.
+    Arguments of the wrong shape, type or device raise ValueError."""
+    return (_native or _load()).append(cache._at, cache._index, qkv, table, pos, cos, sin, bias, starts, max_tokens, out)
 
 
 def kv8_attention(q, cache: KV8Cache, table, pos, starts=None, max_tokens: int | None = None, window: int = 0,
@@ -185,62 +130,17 @@ def kv8_attention(q, cache: KV8Cache, table, pos, starts=None, max_tokens: int |
     apart), whose k and v are already appended, over the cache: [N, H, D] in
     q's type. The row at position p sees positions p - window + 1 .. p (all up
     to p without a window); scale defaults to 1/sqrt(D). Rows that see nothing
-    are 0."""
-    kv, d, dev, L = cache.kv_heads, cache.head_dim, cache.device, lib()
-    if q.dim() != 3 or q.dtype not in _DTYPES or q.device != dev or q.shape[2] != d:
-        raise ValueError(f"q must be an fp32, bf16 or fp16 [N, H, {d}] tensor on the cache's device")
-    n, heads, _ = q.shape
-    if heads == 0 or heads % kv:
-        raise ValueError(f"{heads} query heads are not a multiple of {kv} KV heads")
-    if window < 0:
-        raise ValueError("window must not be negative")
-    width, b, most, sp = _rows(cache, n, table, pos, starts, max_tokens)
-    if out is None:
-        y = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, heads, d))
-    else:
-        y = _out(out, (n, heads, d), q.dtype, dev)
-    if n == 0:
-        return y
-    if _device() != dev.index:
-        with torch.cuda.device(dev):
-            return kv8_attention(q, cache, table, pos, starts, max_tokens, window, scale, y)
-    q = _aligned_rows(q, (d, 1))
-    dt = _DTYPES[q.dtype]
-    sizes = (width, b, most, heads, window)
-    nb = cache._scratch.get(sizes)
-    if nb is None:
-        nb = cache._scratch[sizes] = L.lbc_kv8_attention_workspace(cache._ref, dt, width, b, n, most, heads, window)
-    # from torch's allocator: private to this call in stream order, and to a graph when captured
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-    rc = L.lbc_kv8_attention(cache._ref, dt, q.data_ptr(), q.stride(0), table.data_ptr(), width, pos.data_ptr(), sp,
-                             b, n, most, heads, window, d ** -0.5 if scale is None else scale, y.data_ptr(),
-                             _ptr(ws), nb, _raw_stream(dev.index))
-    if rc < 0:
-        _check(rc, "lbc_kv8_attention")
-    return y
+    are 0. Arguments of the wrong shape, type or device raise ValueError."""
+    return (_native or _load()).attention(cache._at, cache._index, q, table, pos, starts, max_tokens, window, scale, out)
 
 
 def kv8_read(cache: KV8Cache, pages, dtype=torch.bfloat16):
     """Keys and values of the pages ``pages`` (int32 ids on the GPU), each
     [len(pages), kv_heads, page, head_dim]: exact in bf16 and fp32; fp16 rounds
     what lies outside its range."""
-    dev = cache.device
-    if pages.dim() != 1 or pages.dtype != torch.int32 or not pages.is_contiguous() or pages.device != dev:
-        raise ValueError("pages must be a contiguous int32 tensor of ids on the cache's device")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be torch.float32, bfloat16 or float16")
-    n = pages.shape[0]
-    shape = (n, cache.kv_heads, cache.page, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=dev)
-    v = torch.empty_like(k)
-    if n == 0:
-        return k, v
-    if _device() != dev.index:
-        with torch.cuda.device(dev):
-            return kv8_read(cache, pages, dtype)
-    _check(lib().lbc_kv8_read(cache._ref, _DTYPES[dtype], pages.data_ptr(), n, k.data_ptr(), v.data_ptr(),
-                              _raw_stream(dev.index)), "lbc_kv8_read")
-    return k, v
+    return (_native or _load()).read(cache._at, cache._index, pages, _DTYPES[dtype])
 
 
 class PagedKVCache:

@@ -39,20 +39,10 @@ namespace lbc {
 namespace kv8 {
 namespace {
 
-#ifndef HT
-#define HT 1
-#endif
-#ifndef STAGES
-#define STAGES 2
-#endif
-#ifndef RES1
-#define RES1 4
-#endif
-#ifndef RES2
-#define RES2 2
-#endif
+// CTAs an SM that the registers allow
+constexpr int resident(bool fp32, int D, int nq) { return nq > 1 ? 2 : fp32 && D == 128 ? 3 : 4; }
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int WTOK = 16 * HT;       // tokens of a warp in a unit
+constexpr int WTOK = 16;            // tokens of a warp in a unit
 constexpr int UNIT = WARPS * WTOK;
 constexpr int META = 128;           // pages looked up at a time
 // weights 2^(t - M) fill fp16's range: M is the maximum (rounded up) less 14,
@@ -65,6 +55,12 @@ struct Meta {
   float4 s[META];       // 2^(ek - 127), b = ev - 127, 2^(f - b), 1 if the page exists
   int f;                // largest value exponent so far (255 left out)
 };
+
+// Ring steps of a warp: more where they are smaller. Measured 2 / 3 / 4 / 6 at
+// D = 64 (13 sequences to 39520 tokens): 75.7 / 67.8 / 67.9 / 71.9 us; 2 / 3 at
+// D = 128 (64 to 8192): 122 / 130.
+template <int D>
+constexpr int STAGES = D == 128 ? 2 : D == 64 ? 3 : 4;
 
 template <typename T, int D, int NQ>
 struct Warp {
@@ -139,77 +135,64 @@ struct Warp {
     }
   }
 
-  __device__ __forceinline__ void scores(float (&z)[HT][NQ][4], const uint32_t (&step)[HT], int lane) {
+  // scores of the step's 16 tokens, in units of rowf * 2^(ek - 127)
+  __device__ __forceinline__ void scores(float (&z)[NQ][4], uint32_t step, int lane) {
+    uint32_t k[2][KW];
 #pragma unroll
-    for (int h = 0; h < HT; ++h) {
+    for (int n = 0; n < NQ; ++n) z[n][0] = z[n][1] = z[n][2] = z[n][3] = 0.f;
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) z[h][n][0] = z[h][n][1] = z[h][n][2] = z[h][n][3] = 0.f;
-      uint32_t k[2][KW];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = (lane >> 2) + 8 * i, t = lane & 3;
-        if constexpr (D == 32) shared_words<8>(step[h] + place(r, t >> 1) + (t & 1) * 8, k[i]);
-        if constexpr (D == 64) shared_words<16>(step[h] + place(r, t), k[i]);
-        if constexpr (D == 128) {
-          shared_words<16>(step[h] + place(r, 2 * t), k[i]);
-          shared_words<16>(step[h] + place(r, 2 * t + 1), k[i] + 4);
-        }
+    for (int i = 0; i < 2; ++i) {
+      const int r = (lane >> 2) + 8 * i, t = lane & 3;
+      if constexpr (D == 32) shared_words<8>(step + place(r, t >> 1) + (t & 1) * 8, k[i]);
+      if constexpr (D == 64) shared_words<16>(step + place(r, t), k[i]);
+      if constexpr (D == 128) {
+        shared_words<16>(step + place(r, 2 * t), k[i]);
+        shared_words<16>(step + place(r, 2 * t + 1), k[i] + 4);
       }
+    }
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        const uint32_t x0 = k[0][w] ^ 0x80808080u, x1 = k[1][w] ^ 0x80808080u;
-        const uint32_t op[4] = {half_lo(x0), half_lo(x1), half_hi(x0), half_hi(x1)};
+    for (int w = 0; w < KW; ++w) {
+      const uint32_t x0 = k[0][w] ^ 0x80808080u, x1 = k[1][w] ^ 0x80808080u;
+      const uint32_t op[4] = {half_lo(x0), half_lo(x1), half_hi(x0), half_hi(x1)};
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+      for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int c = 0; c < QP; ++c) mma16816(z[h][n], op, q[n][c][w][0], q[n][c][w][1]);
-      }
+        for (int c = 0; c < QP; ++c) mma16816(z[n], op, q[n][c][w][0], q[n][c][w][1]);
     }
   }
 
-  // z: scores to weights (in place); j: position of the warp's first token; e: its tiles' pages
-  __device__ __forceinline__ void weights(const AttnArgs &a, const float4 (&e)[HT], float (&z)[HT][NQ][4], int j, int lane,
-                                          int p_min, int p_max) {
-    float mx[NQ][2];
-    bool rise = false;
-#pragma unroll
-    for (int h = 0; h < HT; ++h) {
-      const int j0 = j + 16 * h;
-      const bool whole = j0 + 15 <= p_min && (a.window <= 0 || j0 > p_max - a.window) && e[h].w != 0.f;
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) z[h][n][i] = fmaf(z[h][n][i], rowf[n][i & 1] * e[h].x, e[h].y);
-      if (!whole) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int at = j0 + (lane >> 2) + 8 * (i >> 1), pr = p[n][i & 1];
-            const bool seen = at <= pr && (a.window <= 0 || at > pr - a.window) && e[h].w != 0.f;
-            z[h][n][i] = seen ? z[h][n][i] : -INFINITY;
-          }
-      }
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float y = fmaxf(z[h][n][i], z[h][n][i + 2]);
-          mx[n][i] = h ? fmaxf(mx[n][i], y) : y;
-        }
-    }
+  // scores to weights, in place; j: position of the step's first token; e: its block's scales
+  __device__ __forceinline__ void weights(const AttnArgs &a, const float4 e, float (&z)[NQ][4], int j, int lane, int p_min,
+                                          int p_max) {
+    const bool whole = j + 15 <= p_min && (a.window <= 0 || j > p_max - a.window) && e.w != 0.f;
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) rise |= mx[n][i] > m[n][i] + SLACK;
+      for (int i = 0; i < 4; ++i) z[n][i] = fmaf(z[n][i], rowf[n][i & 1] * e.x, e.y);
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = j + (lane >> 2) + 8 * (i >> 1), pr = p[n][i & 1];
+          const bool seen = at <= pr && (a.window <= 0 || at > pr - a.window) && e.w != 0.f;
+          z[n][i] = seen ? z[n][i] : -INFINITY;
+        }
+    }
+    bool rise = false;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) rise |= fmaxf(z[n][i], z[n][i + 2]) > m[n][i] + SLACK;
     if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          float mx = fmaxf(z[n][i], z[n][i + 2]);
 #pragma unroll
-          for (int d = 4; d <= 16; d *= 2) mx[n][i] = fmaxf(mx[n][i], __shfl_xor_sync(0xffffffffu, mx[n][i], d));
-          const float to = fmaxf(m[n][i], ceilf(mx[n][i]) - HEAD), f = ex2(m[n][i] - to);
+          for (int d = 4; d <= 16; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const float to = fmaxf(m[n][i], ceilf(mx) - HEAD), f = ex2(m[n][i] - to);
           m[n][i] = to;
           l[n][i] *= f;
 #pragma unroll
@@ -220,48 +203,43 @@ struct Warp {
         }
     }
 #pragma unroll
-    for (int h = 0; h < HT; ++h)
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          z[h][n][i] = ex2(z[h][n][i] - m[n][i & 1]);
-          l[n][i & 1] = fmaf(z[h][n][i], e[h].z, l[n][i & 1]);
-        }
-  }
-
-  __device__ __forceinline__ void outputs(const float (&z)[HT][NQ][4], const uint32_t (&step)[HT], int lane) {
-#pragma unroll
-    for (int h = 0; h < HT; ++h) {
-      uint32_t b[NQ][WP][2], v[4][VW];
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        constexpr int VB = D / 8;  // bytes of a token's row that a lane needs
-        const int r = 2 * (lane & 3) + (i & 1) + 8 * (i >> 1), at = (lane >> 2) * VB;
-        shared_words<VB>(step[h] + 16 * D + place(r, at >> 4) + (at & 15), v[i]);
+        z[n][i] = ex2(z[n][i] - m[n][i & 1]);
+        l[n][i & 1] = fmaf(z[n][i], e.z, l[n][i & 1]);
+      }
+  }
+
+  __device__ __forceinline__ void outputs(const float (&z)[NQ][4], uint32_t step, int lane) {
+    uint32_t b[NQ][WP][2], v[4][VW];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      constexpr int VB = D / 8;  // bytes of a token's row that a lane needs
+      const int r = 2 * (lane & 3) + (i & 1) + 8 * (i >> 1), at = (lane >> 2) * VB;
+      shared_words<VB>(step + 16 * D + place(r, at >> 4) + (at & 15), v[i]);
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t hi = pack_half(z[n][2 * i], z[n][2 * i + 1]);
+        b[n][0][i] = transpose8(hi);
+        if constexpr (WP == 2) b[n][1][i] = transpose8(pack_rest(z[n][2 * i], z[n][2 * i + 1], hi));
       }
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
+    for (int w = 0; w < VW; ++w) {
+      // four tokens' words -> for each element the pairs (token 2t, 2t + 1) and (2t + 8, 2t + 9)
+      const uint32_t x0 = v[0][w] ^ 0x80808080u, x1 = v[1][w] ^ 0x80808080u;
+      const uint32_t x2 = v[2][w] ^ 0x80808080u, x3 = v[3][w] ^ 0x80808080u;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t hi = pack_half(z[h][n][2 * i], z[h][n][2 * i + 1]);
-          b[n][0][i] = transpose8(hi);
-          if constexpr (WP == 2) b[n][1][i] = transpose8(pack_rest(z[h][n][2 * i], z[h][n][2 * i + 1], hi));
-        }
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t y0 = prmt(x0, x1, c ? 0x7362 : 0x5140), y1 = prmt(x2, x3, c ? 0x7362 : 0x5140);
+        const uint32_t op[4] = {half_lo(y0), half_hi(y0), half_lo(y1), half_hi(y1)};
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        // four tokens' words -> for each element the pairs (token 2t, 2t + 1) and (2t + 8, 2t + 9)
-        const uint32_t x0 = v[0][w] ^ 0x80808080u, x1 = v[1][w] ^ 0x80808080u;
-        const uint32_t x2 = v[2][w] ^ 0x80808080u, x3 = v[3][w] ^ 0x80808080u;
+        for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t y0 = prmt(x0, x1, c ? 0x7362 : 0x5140), y1 = prmt(x2, x3, c ? 0x7362 : 0x5140);
-          const uint32_t op[4] = {half_lo(y0), half_hi(y0), half_lo(y1), half_hi(y1)};
-#pragma unroll
-          for (int n = 0; n < NQ; ++n)
-#pragma unroll
-            for (int r = 0; r < WP; ++r) mma16816(o[n][2 * w + c], op, b[n][r][0], b[n][r][1]);
-        }
+          for (int r = 0; r < WP; ++r) mma16816(o[n][2 * w + c], op, b[n][r][0], b[n][r][1]);
       }
     }
   }
@@ -344,7 +322,7 @@ __device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, in
 }
 
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(THREADS, resident(sizeof(T) == 4, D, NQ)) attention_kernel(AttnArgs a) {
   constexpr int R = 8 * NQ, PAD = D + 4;
   __shared__ Meta meta;
   __shared__ long long total_s, scan[WARPS];
@@ -352,7 +330,9 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
   __shared__ long long found_at;
   __shared__ Seq found_seq;
   __shared__ float sm[WARPS][R], sl[WARPS][R];
-  extern __shared__ __align__(16) uint8_t ring[];  // [WARPS][STAGES][HT] steps; then the warps' O [WARPS][R][PAD]
+  extern __shared__ __align__(16) uint8_t ring[];  // [WARPS][STAGES] steps; then the warps' O [WARPS][R][PAD]
+  after_previous_kernel();
+  if (!a.split) next_kernel_may_start();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const long long cta = blockIdx.x;
 
@@ -417,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
 
   using W = Warp<T, D, NQ>;
   W w;
-  const uint32_t mine = smem_u32(ring) + warp * (STAGES * HT * W::STEP);
+  const uint32_t mine = smem_u32(ring) + warp * (STAGES<D> * W::STEP);
   float *so = reinterpret_cast<float *>(ring);
   long long at = lo;
   do {
@@ -443,20 +423,17 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
         meta.off[tid] = max(id, 0) * a.c.page_stride + head;
       }
       __syncthreads();
-      // fetches the warp's tiles of unit c, if the chunk has it, into their ring steps
+      // fetches the warp's 16 tokens of unit c, if the chunk has it, into their ring step
+      auto ring_step = [&](int c) { return mine + (c - c0) % STAGES<D> * W::STEP; };
       auto fetch = [&](int c) {
         if (c < c1) {
-#pragma unroll
-          for (int h = 0; h < HT; ++h) {
-            const int j = (s.u0 + c) * UNIT + warp * WTOK + 16 * h;
-            w.fetch(a, mine + ((c - c0) % STAGES * HT + h) * W::STEP,
-                    meta.off[(j >> a.c.lg_page) - o0] + (j & (a.c.page - 1)) * D, lane);
-          }
+          const int j = (s.u0 + c) * UNIT + warp * WTOK;
+          w.fetch(a, ring_step(c), meta.off[(j >> a.c.lg_page) - o0] + (j & (a.c.page - 1)) * D, lane);
         }
         copy_commit();
       };
 #pragma unroll
-      for (int i = 0; i < STAGES - 1; ++i) fetch(c0 + i);
+      for (int i = 0; i < STAGES<D> - 1; ++i) fetch(c0 + i);
       int ek = 0, ev = 0;
       if (id >= 0) {
         ek = a.c.k_exp[id * a.c.exp_stride + kvh];
@@ -487,19 +464,14 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? RES1 : RES2) attention_kern
         p_max = __reduce_max_sync(0xffffffffu, p_max);
       }
       for (int c = c0; c < c1; ++c) {
-        float z[HT][NQ][4];
-        float4 e[HT];
-        uint32_t step[HT];
+        float z[NQ][4];
         const int j = (s.u0 + c) * UNIT + warp * WTOK;
-#pragma unroll
-        for (int h = 0; h < HT; ++h) {
-          e[h] = meta.s[((j + 16 * h) >> a.c.lg_page) - o0];
-          step[h] = mine + ((c - c0) % STAGES * HT + h) * W::STEP;
-        }
-        copy_wait<STAGES - 2>();
+        const float4 e = meta.s[(j >> a.c.lg_page) - o0];
+        const uint32_t step = ring_step(c);
+        copy_wait<STAGES<D> - 2>();
         __syncwarp();  // every lane's copies of this step are there, and its reads of the last one done
         w.scores(z, step, lane);
-        fetch(c + STAGES - 1);  // into the step that the last iteration read
+        fetch(c + STAGES<D> - 1);  // into the step that the last iteration read
         w.weights(a, e, z, j, lane, p_min, p_max);
         w.outputs(z, step, lane);
       }
@@ -597,7 +569,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
   __shared__ float red[2][WARPS], wo[THREADS];
   __shared__ float4 part[SLICES][C];
   __shared__ float den[WARPS];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  after_previous_kernel();
   const int r = blockIdx.x % R, kvh = blockIdx.x / R % a.c.KV, tile = blockIdx.x / R / a.c.KV, b = blockIdx.y;
   const int tid = threadIdx.x, col = tid % C, slice = tid / C, rho = tile * R + r;
   const Seq s = seq_of<UNIT, 8 * NQ>(a, b);
@@ -667,31 +639,41 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
   store4<T>(dst, out);
 }
 
-#ifndef PROMPT_ROWS
-#define PROMPT_ROWS 128
-#endif
 struct Plan {
   int prompt, nq, tiles, split, cluster, grid;
   size_t desc, bytes;
 };
 
-// row tile: 8 rows, or 16 when a sequence has more (32 spill registers).
-// A cluster an item where one wave holds every item's CTAs and a CTA has at
-// most 16 units (1024 tokens) to go through; the even cut with its second
-// kernel otherwise.
-Plan plan_of(const Pool &c, int width, int B, int most, int H, int window, int sms) {
+// rows of a tile: 8 or 16; 24 where that saves a tile and the registers suffice
+int row_tiles(long long rows, int dtype, int D, int &nq) {
+  nq = rows <= 8 ? 1 : 2;
+  if (nq == 2 && !(dtype == LBC_F32 && D == 128) && (rows + 23) / 24 < (rows + 15) / 16) nq = 3;
+  return (int)((rows + 8 * nq - 1) / (8 * nq));
+}
+
+// Which kernel, and how its work is cut.
+//   prompt      Measured at D = 128: the prompt kernel takes 1.35 us a wave of
+//               its CTAs and 64 tokens, this one 1.3 us for 2 SMs' worth of
+//               units; so it takes over when its waves are the fewer.
+//   cluster     a CTA goes through at most 16 units (1024 tokens), and a wave
+//               holds the clusters of every item where there is more than one CTA
+//   split       otherwise
+Plan plan_of(const Pool &c, int dtype, int width, int B, int most, int H, int window, int sms) {
   Plan p{};
   const long long rows = (long long)most * (H / c.KV);
-  p.prompt = rows >= PROMPT_ROWS;
+  p.tiles = row_tiles(rows, dtype, c.D, p.nq);
+  const long long items = (long long)B * c.KV * p.tiles;
+  const int high = prompt_rows(dtype, c.D);
+  const long long waves = ((long long)B * c.KV * ((rows + high - 1) / high) + sms - 1) / sms;
+  p.prompt = rows > 24 && waves * 2 * sms <= items;
   if (p.prompt) return p;
-  p.nq = rows <= 8 ? 1 : 2;
-  p.tiles = (int)((rows + 8 * p.nq - 1) / (8 * p.nq));
   long long len = (long long)width << c.lg_page;
   if (window > 0) len = std::min(len, (long long)window + most + UNIT);
-  const long long units = (len + UNIT - 1) / UNIT, items = (long long)B * c.KV * p.tiles;
-  const long long wave = (long long)(p.nq == 1 ? RES1 : RES2) * sms;
-  p.cluster = units >= 8 ? 8 : units >= 4 ? 4 : units >= 2 ? 2 : 1;
-  p.split = p.cluster > 1 && (items * p.cluster > wave || units > 16 * p.cluster);
+  const long long units = (len + UNIT - 1) / UNIT;
+  const long long wave = (long long)resident(dtype == LBC_F32, c.D, p.nq) * sms;
+  p.cluster = 1;
+  while (p.cluster < 8 && 2 * p.cluster <= units && 2 * p.cluster * items <= wave) p.cluster *= 2;
+  p.split = units > 16 * p.cluster;
   p.grid = (int)std::min<long long>(p.split ? std::min(items * units, wave) : items * p.cluster, 0x7fffffff);
   p.desc = p.split ? ((size_t)items * sizeof(int2) + 255) / 256 * 256 : 0;
   p.bytes = p.split ? p.desc + (size_t)p.grid * 2 * 8 * p.nq * (c.D + 3) * sizeof(float) : 0;
@@ -700,36 +682,17 @@ Plan plan_of(const Pool &c, int width, int B, int most, int H, int window, int s
 
 template <typename T, int D, int NQ>
 void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {
-  constexpr int smem = std::max(WARPS * STAGES * HT * Warp<T, D, NQ>::STEP, (int)sizeof(float) * WARPS * 8 * NQ * (D + 4));
+  constexpr int smem = std::max(WARPS * STAGES<D> * Warp<T, D, NQ>::STEP, (int)sizeof(float) * WARPS * 8 * NQ * (D + 4));
   static std::atomic<uint64_t> allowed{0};
   allow_smem(attention_kernel<T, D, NQ>, smem, allowed);
-  cudaLaunchAttribute attr{};
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.grid);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  if (!p.split && p.cluster > 1) {
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = p.cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.numAttrs = 1;
-  }
-  cudaLaunchKernelEx(&cfg, attention_kernel<T, D, NQ>, a);
-  if (!p.split) return;
-  // started while the last CTAs of the first kernel run; it waits for their records
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(8 * NQ * a.c.KV * a.tiles, a.r.B);
-  cfg.dynamicSmemBytes = 0;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, join_kernel<T, D, NQ>, a);
+  launch_chained(attention_kernel<T, D, NQ>, dim3(p.grid), THREADS, smem, p.split ? 1 : p.cluster, st, a);
+  if (p.split) launch_chained(join_kernel<T, D, NQ>, dim3(8 * NQ * a.c.KV * a.tiles, a.r.B), THREADS, 0, 1, st, a);
 }
 template <typename T, int D>
 void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {
   if (p.nq == 1) launch<T, D, 1>(a, p, st);
-  else launch<T, D, 2>(a, p, st);
+  else if (p.nq == 2) launch<T, D, 2>(a, p, st);
+  else if constexpr (!(sizeof(T) == 4 && D == 128)) launch<T, D, 3>(a, p, st);
 }
 template <typename T>
 void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {
@@ -753,7 +716,7 @@ size_t lbc_kv8_attention_workspace(const lbc_kv8 *c, int dtype, int table_width,
   int *status = nullptr, sms = 0;
   if (check_pool(c, p) || device_ready(&status, &sms) || table_width <= 0 || B <= 0 || H <= 0 || H % p.KV || max_tokens < 0)
     return 0;
-  return plan_of(p, table_width, B, max_tokens, H, window, sms).bytes;
+  return plan_of(p, dtype, table_width, B, max_tokens, H, window, sms).bytes;
 }
 
 int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, const int32_t *table, int table_width,
@@ -775,7 +738,7 @@ int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, 
     return refuse("kv8_attention: q and out must be 16-byte aligned");
   a.q = q; a.ld = ld; a.out = out; a.H = H; a.G = H / a.c.KV; a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const Plan p = plan_of(a.c, table_width, B, max_tokens, H, window, sms);
+  const Plan p = plan_of(a.c, dtype, table_width, B, max_tokens, H, window, sms);
   if (p.bytes && (!workspace || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return refuse("kv8_attention: workspace too small or not 256-byte aligned");
   a.tiles = p.tiles;

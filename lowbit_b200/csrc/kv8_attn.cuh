@@ -66,7 +66,8 @@ __device__ __forceinline__ int row_pos(const AttnArgs &a, const Seq &s, int rho)
   return p >= ((long long)a.r.width << a.c.lg_page) ? -1 : (int)p;
 }
 
-// prompt chunks (kv8_prompt.cu)
+// prompt chunks (kv8_prompt.cu), and the rows that one of its CTAs takes
+int prompt_rows(int dtype, int D);
 void launch_prompt(const AttnArgs &a, int dtype, cudaStream_t st);
 
 }  // namespace kv8

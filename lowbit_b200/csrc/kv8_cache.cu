@@ -138,12 +138,12 @@ __device__ __forceinline__ void load_row(const float *p, float (&x)[V], bool ali
   if (aligned) {
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
-      const float4 v = __ldg(reinterpret_cast<const float4 *>(p + i));
+      const float4 v = *reinterpret_cast<const float4 *>(p + i);
       x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = __ldg(p + i);
+    for (int i = 0; i < V; ++i) x[i] = p[i];
   }
 }
 
@@ -210,6 +210,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 4) append_kernel(AppendArgs a) {
   constexpr int V = VEC<T>, half = D / 2, per = half / V;  // per: threads a head and token
   __shared__ float red[THREADS / 32];
+  after_previous_kernel();
+  next_kernel_may_start();
   const int kv_ctas = 2 * a.c.KV * a.slots * a.r.B;
   int i = blockIdx.x;
   const int d = threadIdx.x % per * V;
@@ -320,6 +322,8 @@ __global__ void __launch_bounds__(THREADS, 4) append_kernel(AppendArgs a) {
 // all in flight before its first store; every store is 16 bytes, in lane order.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) read_kernel(Pool c, const int32_t *ids, T *k_out, T *v_out, int *status) {
+  after_previous_kernel();
+  next_kernel_may_start();
   constexpr int V = VEC<T>, FLY = 4;
   const int kvh = blockIdx.x % c.KV, n = c.page * c.D / V;
   const int id = ids[blockIdx.x / c.KV];
@@ -338,11 +342,11 @@ __global__ void __launch_bounds__(THREADS) read_kernel(Pool c, const int32_t *id
         const int8_t *src = (s ? c.v : c.k) + at + (size_t)e * V;
         if (e < n) {
           if constexpr (V == 8) {
-            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(src));
+            const uint2 y = *reinterpret_cast<const uint2 *>(src);
             w[s][u][0] = y.x;
             w[s][u][1] = y.y;
           } else {
-            w[s][u][0] = __ldg(reinterpret_cast<const uint32_t *>(src));
+            w[s][u][0] = *reinterpret_cast<const uint32_t *>(src);
           }
         }
       }
@@ -365,9 +369,9 @@ template <typename T>
 void launch_append(const AppendArgs &a, long long kv_ctas, cudaStream_t st) {
   // 16 threads a token and more: up to 4 tokens need no more than 64
   const unsigned threads = a.r.most <= 4 ? 64 : THREADS, ctas = (unsigned)(kv_ctas + (a.r.N + threads / 32 - 1) / (threads / 32));
-  if (a.c.D == 32) append_kernel<T, 32><<<ctas, threads, 0, st>>>(a);
-  else if (a.c.D == 64) append_kernel<T, 64><<<ctas, threads, 0, st>>>(a);
-  else append_kernel<T, 128><<<ctas, threads, 0, st>>>(a);
+  if (a.c.D == 32) launch_chained(append_kernel<T, 32>, dim3(ctas), threads, 0, 1, st, a);
+  else if (a.c.D == 64) launch_chained(append_kernel<T, 64>, dim3(ctas), threads, 0, 1, st, a);
+  else launch_chained(append_kernel<T, 128>, dim3(ctas), threads, 0, 1, st, a);
 }
 
 }  // namespace
@@ -422,12 +426,12 @@ int lbc_kv8_read(const lbc_kv8 *c, int dtype, const int32_t *ids, int n, void *k
   const unsigned ctas = (unsigned)n * p.KV;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == LBC_F32)
-    read_kernel<float><<<ctas, THREADS, 0, st>>>(p, ids, static_cast<float *>(k_out), static_cast<float *>(v_out), status);
+    launch_chained(read_kernel<float>, dim3(ctas), THREADS, 0, 1, st, p, ids, static_cast<float *>(k_out), static_cast<float *>(v_out), status);
   else if (dtype == LBC_BF16)
-    read_kernel<__nv_bfloat16><<<ctas, THREADS, 0, st>>>(p, ids, static_cast<__nv_bfloat16 *>(k_out),
-                                                         static_cast<__nv_bfloat16 *>(v_out), status);
+    launch_chained(read_kernel<__nv_bfloat16>, dim3(ctas), THREADS, 0, 1, st, p, ids, static_cast<__nv_bfloat16 *>(k_out),
+                   static_cast<__nv_bfloat16 *>(v_out), status);
   else
-    read_kernel<__half><<<ctas, THREADS, 0, st>>>(p, ids, static_cast<__half *>(k_out), static_cast<__half *>(v_out), status);
+    launch_chained(read_kernel<__half>, dim3(ctas), THREADS, 0, 1, st, p, ids, static_cast<__half *>(k_out), static_cast<__half *>(v_out), status);
   return launched("kv8_read");
 }
 

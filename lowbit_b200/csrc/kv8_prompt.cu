@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
   using L = Lay<T, D>;
   extern __shared__ __align__(128) uint8_t smem[];
   Shared &sh = *reinterpret_cast<Shared *>(smem + L::S_OFF);
+  after_previous_kernel();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.x, b = blockIdx.y, tile = gridDim.z - 1 - blockIdx.z;  // late rows, the longest, first
   const Seq s = seq_of<NT, L::ROWS>(a, b);
@@ -560,7 +561,7 @@ void launch(const AttnArgs &a, cudaStream_t st) {
   static std::atomic<uint64_t> allowed{0};
   allow_smem(prompt_kernel<T, D>, smem, allowed);
   const unsigned tiles = (unsigned)(((long long)a.r.most * a.G + Lay<T, D>::ROWS - 1) / Lay<T, D>::ROWS);
-  prompt_kernel<T, D><<<dim3(a.c.KV, a.r.B, tiles), THREADS, smem, st>>>(a);
+  launch_chained(prompt_kernel<T, D>, dim3(a.c.KV, a.r.B, tiles), THREADS, smem, 1, st, a);
 }
 template <typename T>
 void launch(const AttnArgs &a, cudaStream_t st) {
@@ -570,6 +571,8 @@ void launch(const AttnArgs &a, cudaStream_t st) {
 }
 
 }  // namespace
+
+int prompt_rows(int dtype, int D) { return dtype == LBC_F32 && D == 128 ? Lay<float, 128>::ROWS : 2 * TILE; }
 
 void launch_prompt(const AttnArgs &a, int dtype, cudaStream_t st) {
   if (dtype == LBC_F32) launch<float>(a, st);

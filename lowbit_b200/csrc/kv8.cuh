@@ -21,7 +21,7 @@ struct Pool {
 // the sequences of one call
 struct Rows {
   const int32_t *table, *pos, *starts;
-  int width, B, N, most;  // table width (pages), sequences, rows, max_tokens
+  int width, B, N, most;  // table width (pages), sequences, rows; max_tokens (without starts: the rows of each)
   int *status;
 };
 
@@ -29,7 +29,7 @@ struct Rows {
 // call's limits keeps the rows that do, and the status word says so
 __device__ __forceinline__ void seq_rows(const Rows &r, int b, int &r0, int &n) {
   if (!r.starts) {
-    n = r.N / r.B;
+    n = r.most;
     r0 = b * n;
     return;
   }
@@ -44,7 +44,7 @@ __device__ __forceinline__ void seq_rows(const Rows &r, int b, int &r0, int &n) 
 
 // the sequence that owns row `row`: the last one that starts at or before it
 __device__ __forceinline__ int row_seq(const Rows &r, int row) {
-  if (!r.starts) return row / (r.N / r.B);
+  if (!r.starts) return row / r.most;
   int lo = 0, hi = r.B;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;

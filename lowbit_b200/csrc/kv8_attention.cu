@@ -75,24 +75,40 @@ struct Warp {
   // first element of the four that lane t's word s of a key row holds
   __device__ static int key_dim(int t, int s) { return t * (D / 4) + 4 * s; }
 
-  __device__ __forceinline__ void start(const AttnArgs &a, const Seq &s, int tile, int kvh, int lane) {
+  // the lane's query elements, row 8 n + g of the tile, four at a time as they lie in memory; taken up by start()
+  struct Query {
+    struct alignas(4 * sizeof(T)) Four {
+      T e[4];
+    } x[NQ][KW];
+  };
+  __device__ __forceinline__ void load_query(Query &y, const AttnArgs &a, const Seq &s, int tile, int kvh, int lane) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int rho = (tile * NQ + n) * 8 + g;
-      const bool live = rho < s.n * a.G;
-      const T *src = static_cast<const T *>(a.q) + (s.r0 + rho / a.G) * a.ld + (size_t)(kvh * a.G + rho % a.G) * D;
-      float x[KW][4], amax = 0.f;
+      if (rho < s.n * a.G) {
+        const int tok = rho < a.G ? 0 : rho / a.G, h = rho - tok * a.G;  // (one token: no division)
+        const T *src = static_cast<const T *>(a.q) + (s.r0 + tok) * a.ld + (size_t)(kvh * a.G + h) * D;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        if (live) {
-          load4<T>(src + key_dim(t, w), x[w]);
-        } else {
-          x[w][0] = x[w][1] = x[w][2] = x[w][3] = 0.f;
-        }
+        for (int w = 0; w < KW; ++w) y.x[n][w] = *reinterpret_cast<const typename Query::Four *>(src + key_dim(t, w));
+      } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) amax = x[w][i] == x[w][i] ? fmaxf(amax, fabsf(x[w][i])) : INFINITY;
+        for (int w = 0; w < KW; ++w) y.x[n][w].e[0] = y.x[n][w].e[1] = y.x[n][w].e[2] = y.x[n][w].e[3] = from_f<T>(0.f);
       }
+    }
+  }
+  __device__ __forceinline__ void start(const Query &y, const AttnArgs &a, const Seq &s, int tile, int lane) {
+    const int t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float amax = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = to_f<T>(y.x[n][w].e[i]);
+          amax = x == x ? fmaxf(amax, fabsf(x)) : INFINITY;
+        }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       const float f = fp16_range(amax);
@@ -100,7 +116,7 @@ struct Warp {
       for (int w = 0; w < KW; ++w)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float x0 = x[w][2 * h] * f, x1 = x[w][2 * h + 1] * f;
+          const float x0 = to_f<T>(y.x[n][w].e[2 * h]) * f, x1 = to_f<T>(y.x[n][w].e[2 * h + 1]) * f;
           q[n][0][w][h] = pack_half(x0, x1);
           if constexpr (QP == 2) q[n][1][w][h] = pack_rest(x0, x1, q[n][0][w][h]);
         }
@@ -262,12 +278,6 @@ struct Warp {
   }
 };
 
-__device__ __forceinline__ int cluster_size() {
-  uint32_t n;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
-  return (int)n;
-}
-
 // joins the sums of a cluster's CTAs (each the four warps' O in `so`, M and l in
 // sm and sl) and writes the item's rows; the formula is join_kernel's
 template <typename T, int D, int NQ>
@@ -275,7 +285,7 @@ __device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, in
                                              float (*sm)[8 * NQ], float (*sl)[8 * NQ]) {
   constexpr int R = 8 * NQ, PAD = D + 4;
   __shared__ float mine[3][R];  // M, M - f, l
-  const int tid = threadIdx.x, size = cluster_size(), rank = (int)cluster_ctarank();
+  const int tid = threadIdx.x, size = gridDim.x, rank = blockIdx.x;
   for (int x = tid; x < R * (D / 4); x += THREADS) {  // the four warps' O into the first one's place
     float4 *y = reinterpret_cast<float4 *>(so + x / (D / 4) * PAD + x % (D / 4) * 4);
     constexpr int Q = R * PAD / 4;
@@ -297,21 +307,32 @@ __device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, in
   for (int x = x0 + tid; x < x1; x += THREADS) {
     const int r = x / (D / 4), d = x % (D / 4) * 4, rho = tile * R + r;
     if (rho >= s.n * a.G) continue;
-    float mg = LOWEST, ag = LOWEST, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < size; ++c) {
-      mg = fmaxf(mg, ld_dsmem_f32(dsmem_addr(&mine[0][r], c)));
-      ag = fmaxf(ag, ld_dsmem_f32(dsmem_addr(&mine[1][r], c)));
+    // all CTAs' values at once: one remote latency (a rank past the size reads its own again, and is left out)
+    float m[8], af[8], lc[8], mg = LOWEST, ag = LOWEST, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    uint4 v[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const uint32_t from = c < size ? c : rank;
+      m[c] = ld_dsmem_f32(dsmem_addr(&mine[0][r], from));
+      af[c] = ld_dsmem_f32(dsmem_addr(&mine[1][r], from));
+      lc[c] = ld_dsmem_f32(dsmem_addr(&mine[2][r], from));
+      v[c] = ld_dsmem_v4(dsmem_addr(so + r * PAD + d, from));
     }
-#pragma unroll 2
-    for (int c = 0; c < size; ++c) {
-      const float m = ld_dsmem_f32(dsmem_addr(&mine[0][r], c)), af = ld_dsmem_f32(dsmem_addr(&mine[1][r], c));
-      const uint4 v = ld_dsmem_v4(dsmem_addr(so + r * PAD + d, c));
-      const float w = ex2(m - mg);
-      l = fmaf(ld_dsmem_f32(dsmem_addr(&mine[2][r], c)), m > LOWEST ? ex2(af - ag) : 1.f, l);
-      y[0] = fmaf(u2f(v.x), w, y[0]);
-      y[1] = fmaf(u2f(v.y), w, y[1]);
-      y[2] = fmaf(u2f(v.z), w, y[2]);
-      y[3] = fmaf(u2f(v.w), w, y[3]);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      mg = fmaxf(mg, m[c]);
+      ag = fmaxf(ag, af[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      if (c < size) {
+        const float w = ex2(m[c] - mg);
+        l = fmaf(lc[c], m[c] > LOWEST ? ex2(af[c] - ag) : 1.f, l);
+        y[0] = fmaf(u2f(v[c].x), w, y[0]);
+        y[1] = fmaf(u2f(v[c].y), w, y[1]);
+        y[2] = fmaf(u2f(v[c].z), w, y[2]);
+        y[3] = fmaf(u2f(v[c].w), w, y[3]);
+      }
     }
     const float w = l == 0.f ? 0.f : (mg > LOWEST ? ex2(mg - ag) : 1.f) / l;
 #pragma unroll
@@ -384,15 +405,16 @@ __global__ void __launch_bounds__(THREADS, resident(sizeof(T) == 4, D, NQ)) atte
     kvh = (int)(item % a.c.KV);
     tile = (int)(item / a.c.KV);
   } else {
-    const int size = cluster_size(), item = (int)(cta / size), rank = (int)(cta % size);
-    kvh = item % a.c.KV;
-    tile = item / a.c.KV % a.tiles;
-    b = item / a.c.KV / a.tiles;
+    // grid: (cluster, KV head and tile, sequence); the cluster's size is a power of two
+    const int shift = 31 - __clz(gridDim.x), rank = blockIdx.x;
+    tile = blockIdx.y / a.c.KV;
+    kvh = blockIdx.y - tile * a.c.KV;
+    b = blockIdx.z;
     s = seq_of<UNIT, 8 * NQ>(a, b);
     if (tile >= s.tiles) return;  // the whole cluster
-    lo = (long long)rank * s.units / size;
-    hi = (long long)(rank + 1) * s.units / size;
-    u = (int)lo;
+    u = (int)(((long long)rank * s.units) >> shift);
+    lo = u;
+    hi = ((long long)(rank + 1) * s.units) >> shift;
   }
 
   using W = Warp<T, D, NQ>;
@@ -416,7 +438,11 @@ __global__ void __launch_bounds__(THREADS, resident(sizeof(T) == 4, D, NQ)) atte
       const int c1 = min(u1, c0 + chunk);
       const int o0 = (s.u0 + c0) * UNIT >> a.c.lg_page, pages = (((s.u0 + c1) * UNIT - 1) >> a.c.lg_page) - o0 + 1;
       int id = -1;
+      typename W::Query query;
       if (c0 > u) __syncthreads();  // every warp is done with the entries before
+      // on its way while the pages are looked up, where the registers allow it
+      constexpr bool EARLY = NQ == 1 && D < 128;
+      if (c0 == u && EARLY) w.load_query(query, a, s, tile, kvh, lane);
       if (tid < pages) {
         const int o = o0 + tid;
         if ((o + 1) << a.c.lg_page > see0 && o << a.c.lg_page <= see1) id = page_id(a.c, a.r, b, o);
@@ -439,7 +465,10 @@ __global__ void __launch_bounds__(THREADS, resident(sizeof(T) == 4, D, NQ)) atte
         ek = a.c.k_exp[id * a.c.exp_stride + kvh];
         ev = a.c.v_exp[id * a.c.exp_stride + kvh];
       }
-      if (c0 == u) w.start(a, s, tile, kvh, lane);
+      if (c0 == u) {
+        if (!EARLY) w.load_query(query, a, s, tile, kvh, lane);
+        w.start(query, a, s, tile, lane);
+      }
       if (id >= 0 && ev != 255) atomicMax(&meta.f, ev);
       __syncthreads();
       const int f_old = f;
@@ -477,7 +506,10 @@ __global__ void __launch_bounds__(THREADS, resident(sizeof(T) == 4, D, NQ)) atte
       }
       copy_wait<0>();
     }
-    if (u == u1) w.start(a, s, tile, kvh, lane);  // an item without units: rows of zeros
+    if (u == u1) {  // no units: nothing to add, or an item of zeros
+      typename W::Query none = {};
+      w.start(none, a, s, tile, lane);
+    }
     // the warps' sums, brought to a common M
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
@@ -503,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, resident(sizeof(T) == 4, D, NQ)) atte
               make_float2(w.o[n][c][i] * f, w.o[n][c][i + 2] * f);
       }
     __syncthreads();
-    if (!a.split && cluster_size() > 1) {
+    if (!a.split && gridDim.x > 1) {
       join_cluster<T, D, NQ>(a, s, tile, kvh, b, f, so, sm, sl);
       return;
     }
@@ -685,7 +717,8 @@ void launch(const AttnArgs &a, const Plan &p, cudaStream_t st) {
   constexpr int smem = std::max(WARPS * STAGES<D> * Warp<T, D, NQ>::STEP, (int)sizeof(float) * WARPS * 8 * NQ * (D + 4));
   static std::atomic<uint64_t> allowed{0};
   allow_smem(attention_kernel<T, D, NQ>, smem, allowed);
-  launch_chained(attention_kernel<T, D, NQ>, dim3(p.grid), THREADS, smem, p.split ? 1 : p.cluster, st, a);
+  launch_chained(attention_kernel<T, D, NQ>, p.split ? dim3(p.grid) : dim3(p.cluster, a.c.KV * p.tiles, a.r.B), THREADS, smem,
+                 p.split ? 1 : p.cluster, st, a);
   if (p.split) launch_chained(join_kernel<T, D, NQ>, dim3(8 * NQ * a.c.KV * a.tiles, a.r.B), THREADS, 0, 1, st, a);
 }
 template <typename T, int D>

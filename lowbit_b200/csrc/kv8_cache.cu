@@ -45,7 +45,7 @@ int check_rows(const Pool &c, const int32_t *table, int width, const int32_t *po
     return LBC_ERR_SHAPE;
   }
   o.table = table; o.pos = pos; o.starts = starts;
-  o.width = width; o.B = B; o.N = N; o.most = most;
+  o.width = width; o.B = B; o.N = N; o.most = starts ? most : N / B;
   o.status = status;
   return 0;
 }
@@ -191,7 +191,7 @@ __device__ __forceinline__ void store_codes(int8_t *dst, const float (&x)[V], fl
 
 // the sequence that owns row `row`, 32 of them compared at a time by the warp
 __device__ __forceinline__ int warp_row_seq(const Rows &r, int row) {
-  if (!r.starts) return row / (r.N / r.B);
+  if (!r.starts) return row / r.most;
   int b = 0;
   for (int i = threadIdx.x & 31; i - (int)(threadIdx.x & 31) < r.B; i += 32) {
     const int k = __popc(__ballot_sync(0xffffffffu, i < r.B && r.starts[i + 1] <= row));

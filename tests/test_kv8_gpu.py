@@ -114,6 +114,134 @@ def test_prompts(dt, heads, kv, d, page, new):
     attention_case(3, dt, heads, kv, d, page, [0, 70, 1, -5], new)
 
 
+def kernels_of(call):
+    """Names of the kernels a call launches."""
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA], acc_events=True) as prof:
+        call()
+        torch.cuda.synchronize()
+    return " ".join(e.name for e in prof.events())
+
+
+def test_many_rows_take_the_prompt_kernel():
+    """Few rows stay on the few-row kernel, whatever the lengths; a batch of prompts goes to the other one."""
+    cache = lb.KV8Cache.empty(64, 4, 64, page=32)
+    for b, new, want, other in ((12, 1, "attention_kernel", "prompt_kernel"), (1, 100, "attention_kernel", "prompt_kernel"),
+                                (12, 100, "prompt_kernel", "attention_kernel")):
+        q, table, pos = torch.zeros((b * new, 8, 64), device="cuda"), i32(np.zeros((b, 8))), i32([0] * b)
+        lb.kv8_attention(q, cache, table, pos)
+        names = kernels_of(lambda: lb.kv8_attention(q, cache, table, pos))  # noqa: B023
+        assert want in names and other not in names, names
+
+
+# twelve sequences, so that the calls reach the prompt kernel
+LONG = dict(pos=[0, 70, 1, -5, 200, 31, 0, 64, 127, 128, 300, 5], new=[150, 1, 0, 61, 149, 64, 150, 150, 33, 128, 90, 150])
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("heads,kv,d,page", [(8, 4, 32, 16), (8, 4, 64, 32), (8, 4, 128, 64), (12, 3, 32, 128), (7, 1, 128, 16),
+                                             (30, 2, 64, 128)])
+def test_batches_of_prompts(dt, heads, kv, d, page):
+    attention_case(13, dt, heads, kv, d, page, **LONG)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("d,page", [(32, 32), (64, 16), (128, 128)])
+@pytest.mark.parametrize("window", [1, 40, 64, 129, 1000])
+def test_batches_of_prompts_with_windows(dt, d, page, window):
+    attention_case(14, dt, 8, 4, d, page, window=window, **LONG)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_batches_of_prompts_long(dt):
+    attention_case(15, dt, 8, 4, 64, 64, [1500] * 10 + [0, 1300], 70)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_batches_of_prompts_nothing_leaks(dt):
+    """As test_nothing_leaks_from_masked_places, on the prompt kernel."""
+    rng = np.random.default_rng(16)
+    b, new, window, page, p0 = 12, 100, 40, 16, 110
+    width = -(-(p0 + new) // page) + 2
+    pool = host_pool(rng, b * width, 4, page, 64)
+    table = rng.permutation(b * width).reshape(b, width)
+    first = (p0 - window + 1) // page
+    q = torch.from_numpy(rng.standard_normal((b * new, 8, 64)).astype(np.float32)).to(TYPES[dt])
+    ref, mag, size = R.attention(pool, q.double().numpy(), table, [p0] * b, window=window)
+    bad = {n: a.copy() for n, a in pool.items()}
+    for n in ("k_exp", "v_exp"):
+        bad[n][table[:, :first]] = 255
+        bad[n][table[:, -2:]] = 255
+    junk = table.copy()
+    junk[:, :first], junk[:, -2:] = 10 ** 6, -3
+    K.device_status(reset=True)
+    for t in (table, junk):
+        out = lb.kv8_attention(q.cuda(), device_pool(bad), i32(t), i32([p0] * b), window=window)
+        check(out, ref, mag, size, dt, 64, p0 + new)
+    assert K.device_status(reset=True) == 0
+    o, row = p0 // page + 2, 3  # a NaN block inside sequence 3: exactly the rows that see it
+    for n in ("k_exp", "v_exp"):
+        one = {m: a.copy() for m, a in bad.items()}
+        one[n][table[row, o], 1] = 255
+        out = lb.kv8_attention(q.cuda(), device_pool(one), i32(table), i32([p0] * b), window=window).float().cpu().numpy()
+        p = np.arange(p0, p0 + new)
+        sees = np.zeros((b, new, 8), bool)
+        sees[row, :, 2:4] = ((p >= o * page) & (p - window + 1 < (o + 1) * page))[:, None]
+        sees = sees.reshape(b * new, 8)
+        assert np.isnan(out[sees]).all() and np.isfinite(out[~sees]).all()
+    q[5 * new + 1, 2], q[7 * new, 0, 5] = float("nan"), float("inf")
+    out = lb.kv8_attention(q.cuda(), device_pool(bad), i32(table), i32([p0] * b), window=window).float().cpu().numpy()
+    hit = np.zeros((b * new, 8), bool)
+    hit[5 * new + 1, 2] = hit[7 * new, 0] = True
+    assert np.isnan(out[hit]).any(-1).all() and np.isfinite(out[~hit]).all()
+
+
+def test_batches_of_prompts_out_of_range():
+    rng = np.random.default_rng(17)
+    b, new = 12, 100
+    pool = host_pool(rng, 4 * b, 4, 64, 64)
+    cache, q = device_pool(pool), torch.randn((b * new, 8, 64), device="cuda")
+    table = i32(np.arange(4 * b).reshape(b, 4))
+    K.device_status(reset=True)
+    good = lb.kv8_attention(q, cache, table, i32([100] * b))
+    assert K.device_status(reset=True) == 0
+    bad = table.clone()
+    bad[0, 0], bad[0, 1] = 4 * b, -1
+    out = lb.kv8_attention(q, cache, bad, i32([100] * b))
+    assert K.device_status(reset=True) == ERR_PAGE
+    assert torch.equal(out[new:], good[new:]) and torch.isfinite(out).all()
+    out = lb.kv8_attention(q, cache, table, i32([2 ** 31 - 200] + [100] * (b - 1)))
+    assert K.device_status(reset=True) == ERR_PAGE
+    assert torch.equal(out[new:], good[new:]) and not out[:new].any()
+    st = i32(np.arange(b + 1) * new)
+    out = lb.kv8_attention(q, cache, table, i32([100] * b), starts=st, max_tokens=new - 1, out=torch.full_like(good, 7.0))
+    assert K.device_status(reset=True) == ERR_PAGE
+    ref, mag, size = (a.reshape(b, new, *a.shape[1:])[:, :-1]
+                      for a in R.attention(pool, q.cpu().numpy(), table.cpu().numpy(), [100] * b))
+    out = out.view(b, new, 8, 64)
+    check(out[:, :-1], ref, mag, size, "fp32", 64, 200)
+    assert (out[:, -1] == 7).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("b,new", [(1, 1), (9, 1), (3, 40), (12, 150)])
+def test_same_bits_every_time(dt, b, new):
+    """No result depends on the order in which blocks run; calls on two streams do not disturb each other."""
+    rng = np.random.default_rng(18)
+    pool = device_pool(host_pool(rng, 20 * b, 4, 64, 64))
+    table, pos = i32(rng.permutation(20 * b).reshape(b, 20)), i32([1280 - new - 13 * i for i in range(b)])
+    q = torch.randn((b * new, 8, 64), device="cuda").to(TYPES[dt])
+    first = lb.kv8_attention(q, pool, table, pos)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(lb.kv8_attention(q, pool, table, pos))
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o, first)
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("window", [1, 2, 15, 64, 100, 5000])
 @pytest.mark.parametrize("new", [1, 4, 150])
@@ -225,6 +353,17 @@ def test_out_of_range_is_recorded_and_skipped(new):
                                out=torch.full_like(good, 7.0))
         assert K.device_status(reset=True) == ERR_PAGE
         assert torch.isfinite(out[:new - 1]).all() and torch.equal(out[new - 1], torch.full_like(out[0], 7.0))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_batches_of_prompts_strided(dt):
+    """q as a slice of fused rows, on the prompt kernel: the same bits."""
+    rng = np.random.default_rng(19)
+    cache = device_pool(host_pool(rng, 48, 4, 64, 64))
+    table, pos = i32(rng.permutation(48).reshape(12, 4)), i32([100] * 12)
+    q = torch.randn((1200, 16 * 64), device="cuda").to(TYPES[dt])[:, 256:768].unflatten(1, (8, 64))
+    assert not q.is_contiguous()
+    assert torch.equal(lb.kv8_attention(q, cache, table, pos), lb.kv8_attention(q.contiguous(), cache, table, pos))
 
 
 @pytest.mark.parametrize("dt", TYPES)

@@ -42,18 +42,6 @@ __device__ __forceinline__ void seq_rows(const Rows &r, int b, int &r0, int &n) 
   }
 }
 
-// the sequence that owns row `row`: the last one that starts at or before it
-__device__ __forceinline__ int row_seq(const Rows &r, int row) {
-  if (!r.starts) return row / r.most;
-  int lo = 0, hi = r.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (r.starts[mid] <= row) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
 // id of the page that holds positions [o * page, (o + 1) * page) of sequence
 // b, or -1 (recorded) when the table or the pool has no such page
 __device__ __forceinline__ int page_id(const Pool &c, const Rows &r, int b, int o) {

@@ -256,6 +256,31 @@ def test_long(dt, new, pos):
     attention_case(6, dt, 4, 1, 128, 16, pos, new)
 
 
+@pytest.mark.parametrize("new", [1, 2, 40])
+@pytest.mark.parametrize("kv,g,d", [(8, 1, 128), (8, 4, 64), (4, 16, 32)])
+def test_long_sums_do_not_drift(new, kv, g, d):
+    """Positive values, so that sums cut off instead of rounded would all come out small. Rounding to nearest
+    has mean 0; what tensor cores cut off stays within a step: two additions to its sum (2 * 2^-23), and as
+    much again for the weights' two pieces. So the mean relative error is at most 2^-21."""
+    rng = np.random.default_rng(30)
+    b, length, page = 64, 8192, 64
+    pool = host_pool(rng, length // page, kv, page, d)
+    pool["v"] = np.abs(pool["v"])
+    table = np.broadcast_to(np.arange(length // page), (b, length // page))  # one prefix for all
+    q = torch.from_numpy(rng.standard_normal((b * new, kv * g, d)).astype(np.float32)).cuda()
+    out = lb.kv8_attention(q, device_pool(pool), i32(table), i32([length - new] * b))
+    k, v = (torch.from_numpy((pool[n] * R.pow2(pool[n + "_exp"])[..., None, None]).transpose(1, 0, 2, 3).reshape(kv, length, d)).cuda()
+            for n in "kv")
+    worst = []
+    for i in range(0, b * new, 8 * new):
+        x = q[i:i + 8 * new].double().view(8, new, kv, g, d)
+        s = torch.einsum("btkgd,kld->btkgl", x, k) / d ** 0.5
+        seen = torch.arange(length, device="cuda") <= torch.arange(length - new, length, device="cuda")[:, None]
+        ref = torch.einsum("btkgl,kld->btkgd", s.masked_fill(~seen[None, :, None, None], -torch.inf).softmax(-1), v)
+        worst.append(((out[i:i + 8 * new].double().view_as(ref) - ref) / ref).mean().item())
+    assert abs(np.mean(worst)) <= 2.0 ** -21, np.mean(worst)
+
+
 @pytest.mark.parametrize("new", [1, 140])
 def test_block_scales_far_apart(new):
     """Blocks 2^20 apart in scale, and an all-zero block (exponent 0) whose tokens still count."""

@@ -39,8 +39,15 @@ namespace lbc {
 namespace kv8 {
 namespace {
 
-// CTAs an SM that the registers allow
-constexpr int resident(bool fp32, int D, int nq) { return nq > 1 ? 2 : fp32 && D == 128 ? 3 : 4; }
+// CTAs an SM that the registers allow. bf16 tiles of 16 rows fit three times at
+// D <= 64: 9 sequences to 64000 tokens, 8 KV heads, 116 -> 110 us (D = 64), 88 ->
+// 79 (D = 32); 15 to 11600, 1 KV head, 16.6 -> 17.5. fp16's second weight piece
+// leaves it at two (19.8 -> 20.3).
+constexpr int resident(int dtype, int D, int nq) {
+  return nq == 2 && D < 128 && dtype == LBC_BF16 ? 3 : nq > 1 ? 2 : dtype == LBC_F32 && D == 128 ? 3 : 4;
+}
+template <typename T>
+constexpr int DTYPE = sizeof(T) == 4 ? LBC_F32 : is_bf16<T> ? LBC_BF16 : LBC_F16;
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int WTOK = 16;            // tokens of a warp in a unit
 constexpr int UNIT = WARPS * WTOK;
@@ -353,7 +360,7 @@ __device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, in
 }
 
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(THREADS, resident(sizeof(T) == 4, D, NQ)) attention_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_kernel(AttnArgs a) {
   constexpr int R = 8 * NQ, PAD = D + 4;
   __shared__ Meta meta;
   __shared__ long long total_s, scan[WARPS];
@@ -699,7 +706,13 @@ int row_tiles(long long rows, int dtype, int D, int &nq) {
 //               units; so it takes over when its waves are the fewer.
 //   cluster     a CTA goes through at most 16 units (1024 tokens), and a wave
 //               holds the clusters of every item where there is more than one CTA
-//   split       otherwise
+//   split       otherwise; more CTAs than SMs only where each gets THIN units of
+//               the longest possible sequences: below, a CTA's start and the
+//               records that it adds to the join cost more than it saves.
+//               Measured with 1 / 3 / 5 / 7: one sequence of 30000 tokens, 2 KV
+//               heads 19.8 / 15.6 / 15.1 / 13.5 us; two of up to 16000, 8 KV
+//               heads 21.1 / 21.2 / 21.2 / 23.0
+constexpr int THIN = 6;
 Plan plan_of(const Pool &c, int dtype, int width, int B, int most, int H, int window, int sms) {
   Plan p{};
   const long long rows = (long long)most * (H / c.KV);
@@ -712,11 +725,11 @@ Plan plan_of(const Pool &c, int dtype, int width, int B, int most, int H, int wi
   long long len = (long long)width << c.lg_page;
   if (window > 0) len = std::min(len, (long long)window + most + UNIT);
   const long long units = (len + UNIT - 1) / UNIT;
-  const long long wave = (long long)resident(dtype == LBC_F32, c.D, p.nq) * sms;
+  const long long wave = (long long)resident(dtype, c.D, p.nq) * sms;
   p.cluster = 1;
   while (p.cluster < 8 && 2 * p.cluster <= units && 2 * p.cluster * items <= wave) p.cluster *= 2;
   p.split = units > 16 * p.cluster;
-  p.grid = (int)std::min<long long>(p.split ? std::min(items * units, wave) : items * p.cluster, 0x7fffffff);
+  p.grid = (int)std::min<long long>(p.split ? std::min(wave, std::max<long long>(items * units / THIN, sms)) : items * p.cluster, 0x7fffffff);
   p.desc = p.split ? ((size_t)items * sizeof(int2) + 255) / 256 * 256 : 0;
   p.bytes = p.split ? p.desc + (size_t)p.grid * 2 * 8 * p.nq * (c.D + 3) * sizeof(float) : 0;
   return p;

@@ -5,6 +5,7 @@
 // exponent and codes are written without atomics and do not depend on the
 // order in which CTAs run. Products and sums of the rotation are rounded
 // separately (as lbc_qkv_rope does).
+#include <algorithm>
 #include <cstdio>
 
 #include "kernels.h"
@@ -318,33 +319,62 @@ __global__ void __launch_bounds__(THREADS, 4) append_kernel(AppendArgs a) {
   if (threadIdx.x == 0) *exp = (uint8_t)e_new;
 }
 
-// One CTA per (page of the list, head): a thread's loads of keys and values are
-// all in flight before its first store; every store is 16 bytes, in lane order.
-template <typename T>
-__global__ void __launch_bounds__(THREADS) read_kernel(Pool c, const int32_t *ids, T *k_out, T *v_out, int *status) {
+// A block (page of the list and head) is 2^lg pieces of VEC elements. A thread
+// has FLY pieces of keys and of values in flight before its first store; every
+// store is 16 bytes, in lane order. A CTA reads one block, or, where there are
+// many that hold fewer pieces than its threads can fly, `take` of them (MANY):
+// 97 MB of pages of 16 tokens, D = 64, 31.1 -> 17.1 us. Looking the block up for
+// every piece costs large ones time (pages of 64, D = 128: 64 -> 73 us), and few
+// ones latency (8.2 -> 10.2 us from an idle GPU), so both keep one block a CTA.
+// Bound by HBM: 402 MB of pages of 64, D = 128, to bf16 in 64 us, 6.3 TB/s.
+constexpr int FLY = 4;
+template <typename T, bool MANY>
+__global__ void __launch_bounds__(THREADS) read_kernel(Pool c, const int32_t *ids, unsigned blocks, int lg, int take, T *k_out, T *v_out,
+                                                       int *status) {
   after_previous_kernel();
   next_kernel_may_start();
-  constexpr int V = VEC<T>, FLY = 4;
-  const int kvh = blockIdx.x % c.KV, n = c.page * c.D / V;
-  const int id = ids[blockIdx.x / c.KV];
-  const bool ok = id >= 0 && id < c.pages;
-  if (!ok && threadIdx.x == 0) set_status(status, LBC_ERR_PAGE);
-  const size_t at = ok ? id * c.page_stride + (size_t)kvh * c.page * c.D : 0;
-  const float f[2] = {ok ? pow2_e8m0(c.k_exp[id * c.exp_stride + kvh]) : 0.f, ok ? pow2_e8m0(c.v_exp[id * c.exp_stride + kvh]) : 0.f};
-  T *out[2] = {k_out + (size_t)blockIdx.x * c.page * c.D, v_out + (size_t)blockIdx.x * c.page * c.D};
-  for (int e0 = threadIdx.x; e0 < n; e0 += FLY * THREADS) {
+  constexpr int V = VEC<T>;
+  struct Block {
+    long long at;  // bytes to its codes (a page that does not exist: any)
+    float f[2];
+    bool ok;
+  };
+  auto look_up = [&](unsigned block, bool record) {
+    const unsigned page = block / c.KV, kvh = block - page * c.KV;
+    const int id = ids[page];
+    Block y;
+    y.ok = id >= 0 && id < c.pages;
+    if (!y.ok && record) set_status(status, LBC_ERR_PAGE);
+    y.at = y.ok ? id * c.page_stride + (long long)kvh * c.page * c.D : 0;
+    const long long scale = y.ok ? id * c.exp_stride + kvh : 0;
+    y.f[0] = y.ok ? pow2_e8m0(c.k_exp[scale]) : 0.f;
+    y.f[1] = y.ok ? pow2_e8m0(c.v_exp[scale]) : 0.f;
+    return y;
+  };
+  const unsigned first = blockIdx.x * take, n = (MANY ? min((unsigned)take, blocks - first) : 1u) << lg;
+  Block y[MANY ? FLY : 1];
+  if constexpr (!MANY) y[0] = look_up(first, threadIdx.x == 0);
+  T *out[2] = {k_out + ((size_t)first << lg) * V, v_out + ((size_t)first << lg) * V};
+  for (unsigned e0 = threadIdx.x; e0 < n; e0 += FLY * THREADS) {
     uint32_t w[2][FLY][V / 4];
+    if constexpr (MANY) {
+#pragma unroll
+      for (int u = 0; u < FLY; ++u) {
+        const unsigned e = e0 + u * THREADS;
+        if (e < n) y[u] = look_up(first + (e >> lg), (e & ((1u << lg) - 1)) == 0);
+      }
+    }
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int u = 0; u < FLY; ++u) {
-        const int e = e0 + u * THREADS;
-        const int8_t *src = (s ? c.v : c.k) + at + (size_t)e * V;
+        const unsigned e = e0 + u * THREADS;
+        const int8_t *src = (s ? c.v : c.k) + y[MANY ? u : 0].at + (MANY ? e & ((1u << lg) - 1) : e) * V;
         if (e < n) {
           if constexpr (V == 8) {
-            const uint2 y = *reinterpret_cast<const uint2 *>(src);
-            w[s][u][0] = y.x;
-            w[s][u][1] = y.y;
+            const uint2 x = *reinterpret_cast<const uint2 *>(src);
+            w[s][u][0] = x.x;
+            w[s][u][1] = x.y;
           } else {
             w[s][u][0] = *reinterpret_cast<const uint32_t *>(src);
           }
@@ -354,15 +384,26 @@ __global__ void __launch_bounds__(THREADS) read_kernel(Pool c, const int32_t *id
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int u = 0; u < FLY; ++u) {
-        const int e = e0 + u * THREADS;
+        const unsigned e = e0 + u * THREADS;
         if (e < n) {
+          const Block &z = y[MANY ? u : 0];
           float x[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) x[j] = ok ? __fmul_rn((float)(int8_t)(w[s][u][j / 4] >> (8 * (j % 4))), f[s]) : 0.f;
+          for (int j = 0; j < V; ++j) x[j] = z.ok ? __fmul_rn((float)(int8_t)(w[s][u][j / 4] >> (8 * (j % 4))), z.f[s]) : 0.f;
           store16<T>(out[s] + (size_t)e * V, x);
         }
       }
   }
+}
+
+template <typename T>
+void launch_read(const Pool &c, const int32_t *ids, int n, void *k_out, void *v_out, int *status, int sms, cudaStream_t st) {
+  const unsigned blocks = (unsigned)n * c.KV;
+  int lg = 0;
+  while (VEC<T> << lg < c.page * c.D) ++lg;
+  const int take = blocks / 8 < (unsigned)sms ? 1 : std::max(1, FLY * THREADS >> lg);
+  launch_chained(take > 1 ? read_kernel<T, true> : read_kernel<T, false>, dim3((blocks - 1) / take + 1), THREADS, 0, 1, st, c, ids,
+                 blocks, lg, take, static_cast<T *>(k_out), static_cast<T *>(v_out), status);
 }
 
 template <typename T>
@@ -423,15 +464,10 @@ int lbc_kv8_read(const lbc_kv8 *c, int dtype, const int32_t *ids, int n, void *k
   if (!ids || !k_out || !v_out) return refuse("kv8_read: NULL argument");
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15)
     return refuse("kv8_read: outputs must be 16-byte aligned");
-  const unsigned ctas = (unsigned)n * p.KV;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == LBC_F32)
-    launch_chained(read_kernel<float>, dim3(ctas), THREADS, 0, 1, st, p, ids, static_cast<float *>(k_out), static_cast<float *>(v_out), status);
-  else if (dtype == LBC_BF16)
-    launch_chained(read_kernel<__nv_bfloat16>, dim3(ctas), THREADS, 0, 1, st, p, ids, static_cast<__nv_bfloat16 *>(k_out),
-                   static_cast<__nv_bfloat16 *>(v_out), status);
-  else
-    launch_chained(read_kernel<__half>, dim3(ctas), THREADS, 0, 1, st, p, ids, static_cast<__half *>(k_out), static_cast<__half *>(v_out), status);
+  if (dtype == LBC_F32) launch_read<float>(p, ids, n, k_out, v_out, status, sms, st);
+  else if (dtype == LBC_BF16) launch_read<__nv_bfloat16>(p, ids, n, k_out, v_out, status, sms, st);
+  else launch_read<__half>(p, ids, n, k_out, v_out, status, sms, st);
   return launched("kv8_read");
 }
 

@@ -557,6 +557,26 @@ def test_read(d, page, kv):
     assert [t.shape[0] for t in lb.kv8_read(cache, i32([]))] == [0, 0]
 
 
+@pytest.mark.parametrize("d,page,kv,n", [(32, 16, 3, 701), (64, 16, 5, 333), (32, 64, 1, 1500), (128, 64, 3, 450)])
+def test_read_many_blocks(d, page, kv, n):
+    rng = np.random.default_rng(25)
+    pool = host_pool(rng, 9, kv, page, d)
+    pool["v_exp"][4, 0] = 255
+    cache, ids = device_pool(pool), rng.integers(0, 9, n)
+    bad = ids.copy()
+    bad[[0, n // 2, n - 1]] = [9, -1, 2 ** 31 - 1]
+    K.device_status(reset=True)
+    for dt in TYPES.values():
+        for want in (ids, bad):
+            got = lb.kv8_read(cache, i32(want), dtype=dt)
+            there = (want >= 0) & (want < 9)
+            for name, g in zip("kv", got):
+                ref = pool[name][want * there] * R.pow2(pool[name + "_exp"][want * there])[..., None, None]
+                ref[~there] = 0
+                assert torch.equal(g.cpu().nan_to_num(1.25), torch.from_numpy(ref).float().to(dt).nan_to_num(1.25))
+            assert K.device_status(reset=True) == (0 if there.all() else ERR_PAGE)
+
+
 # ---------------------------------------------------------------- streams, graphs, refusals
 
 def test_another_stream_and_graph_replay():

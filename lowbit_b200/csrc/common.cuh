@@ -184,8 +184,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, int *s
   }
 }
 
-// The same without a suspend time: a time makes the compiler poll with sleeps
-// in between, whose length a pipeline of short steps feels at every wait.
+// The same without a suspend time, for pipelines of short steps.
 __device__ __forceinline__ bool mbar_poll(uint64_t *bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(

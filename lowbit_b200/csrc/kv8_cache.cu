@@ -207,6 +207,9 @@ __device__ __forceinline__ int warp_row_seq(const Rows &r, int row) {
 // time; a block's rows are read twice, for the maximum and for the codes (the
 // second time from L1: keeping them in registers costs the query CTAs their
 // occupancy). blockDim is 64 when a sequence brings few rows, 256 otherwise.
+// Bound by latency: one token 5.0 us, 64 sequences 7.5 us (launch, then table,
+// rows, maximum, codes in turn); 6255 rows of 48 heads of 128, bf16, 38 us, 3.7
+// TB/s of the 141 MB that it has to move.
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 4) append_kernel(AppendArgs a) {
   constexpr int V = VEC<T>, half = D / 2, per = half / V;  // per: threads a head and token

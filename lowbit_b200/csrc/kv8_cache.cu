@@ -67,7 +67,7 @@ int launched(const char *what) {
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, APPEND = 128;  // of the read and append kernels
 
 __device__ __forceinline__ float block_max(float v, float *red) {
 #pragma unroll
@@ -202,25 +202,27 @@ __device__ __forceinline__ int warp_row_seq(const Rows &r, int row) {
   return min(b, r.B - 1);
 }
 
-// Grid: first 2 * KV * slots * B CTAs, one block (keys or values of a page and
-// head) each; then the query CTAs, one row a warp. A thread moves 16 bytes at a
-// time; a block's rows are read twice, for the maximum and for the codes (the
-// second time from L1: keeping them in registers costs the query CTAs their
-// occupancy). blockDim is 64 when a sequence brings few rows, 256 otherwise.
-// Bound by latency: one token 5.0 us, 64 sequences 7.5 us (launch, then table,
-// rows, maximum, codes in turn); 6255 rows of 48 heads of 128, bf16, 38 us, 3.7
+// Grid: first the query CTAs, one row a warp; then 2 * KV * slots * B CTAs, one
+// block (keys or values of a page and head) each, whose work is shorter. A
+// thread moves 16 bytes at a time; a block's rows are read twice, for the
+// maximum and for the codes (the second time from L1: keeping them in registers
+// costs the query CTAs their occupancy). 128 threads, so that more CTAs are in
+// different phases of this (256: 37.1 us for 35.1; blocks first: 37.7), 64 when
+// a sequence brings few rows.
+// Bound by latency: one token 4.4 us, 64 sequences 6 us (launch, then table,
+// rows, maximum, codes in turn); 6255 rows of 48 heads of 128, bf16, 35.1 us, 4.0
 // TB/s of the 141 MB that it has to move.
 template <typename T, int D>
-__global__ void __launch_bounds__(THREADS, 4) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(APPEND, 8) append_kernel(AppendArgs a) {
   constexpr int V = VEC<T>, half = D / 2, per = half / V;  // per: threads a head and token
-  __shared__ float red[THREADS / 32];
+  __shared__ float red[APPEND / 32];
   after_previous_kernel();
   next_kernel_may_start();
-  const int kv_ctas = 2 * a.c.KV * a.slots * a.r.B;
+  const int q_ctas = (a.r.N + blockDim.x / 32 - 1) / (blockDim.x / 32);
   int i = blockIdx.x;
   const int d = threadIdx.x % per * V;
-  if (i >= kv_ctas) {  // queries, one row a warp: a lane keeps its angles for all its heads
-    const int row = (i - kv_ctas) * (blockDim.x / 32) + threadIdx.x / 32, lane = threadIdx.x & 31;
+  if (i < q_ctas) {  // queries, one row a warp: a lane keeps its angles for all its heads
+    const int row = i * (blockDim.x / 32) + threadIdx.x / 32, lane = threadIdx.x & 31;
     if (row >= a.r.N) return;
     int r0, n;
     const int b = warp_row_seq(a.r, row);
@@ -250,6 +252,7 @@ __global__ void __launch_bounds__(THREADS, 4) append_kernel(AppendArgs a) {
     }
     return;
   }
+  i -= q_ctas;
   const bool is_v = i & 1;
   i >>= 1;
   const int kvh = i % a.c.KV;
@@ -412,7 +415,7 @@ void launch_read(const Pool &c, const int32_t *ids, int n, void *k_out, void *v_
 template <typename T>
 void launch_append(const AppendArgs &a, long long kv_ctas, cudaStream_t st) {
   // 16 threads a token and more: up to 4 tokens need no more than 64
-  const unsigned threads = a.r.most <= 4 ? 64 : THREADS, ctas = (unsigned)(kv_ctas + (a.r.N + threads / 32 - 1) / (threads / 32));
+  const unsigned threads = a.r.most <= 4 ? 64 : APPEND, ctas = (unsigned)(kv_ctas + (a.r.N + threads / 32 - 1) / (threads / 32));
   if (a.c.D == 32) launch_chained(append_kernel<T, 32>, dim3(ctas), threads, 0, 1, st, a);
   else if (a.c.D == 64) launch_chained(append_kernel<T, 64>, dim3(ctas), threads, 0, 1, st, a);
   else launch_chained(append_kernel<T, 128>, dim3(ctas), threads, 0, 1, st, a);

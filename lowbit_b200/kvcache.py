@@ -21,7 +21,7 @@ Rows at negative positions are padding (nothing stored, output 0): a fixed
 batch marks its free places with ``pos`` -1. All of it is read on the device,
 so a captured CUDA graph replays with new positions and tables. Ids or
 positions out of range are skipped on the device and recorded in
-``kernels.device_status()``.
+``kernels.device_status()``; output rows that no sequence owns are not written.
 
 The reference has no counterpart: its cache is one fp32 array per layer
 (src/lowbit/model.py:216-230).

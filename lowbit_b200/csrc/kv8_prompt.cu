@@ -501,7 +501,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       }
     }
     // all outputs are done (pv_done's last phase would not do: the one before may still be open)
-    if (steps > 0 && ok) wait(&sh.fin, 0);
+    // (they follow every store of the query operand, in whose place the rows are staged; without a step a barrier
+    // of the row tile's warps orders the two)
+    if (steps == 0) named_bar_sync(1 + i, TILE);
+    else if (ok) wait(&sh.fin, 0);
     tc::fence_after_sync();
     float l;
     {

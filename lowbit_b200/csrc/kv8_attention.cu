@@ -18,8 +18,9 @@
 // 2^b_j: t_j = z_j + b_j, M about max t_j - 14 the running reference,
 //   O = sum_j 2^(t_j - M) code_j,  l = sum_j 2^(t_j - M) 2^(f - b_j),
 //   out = 2^f O / l,  f = max b_j,
-// so weights stay within fp16 whatever the scales, and all rescaling is by
-// powers of two (M is a whole number).
+// so weights stay within fp16, and all rescaling is by powers of two (M is a
+// whole number). f is the largest b looked up, seen by a row or not; where they
+// lie more than 2^60 apart, rows are computed one by one (kv8_attn.cuh: far_row).
 //
 // Work: an item is (sequence, tile of 8 NQ rows, KV head); its visible tokens
 // are cut into units of 64 (16 a warp). The units of all items form one line
@@ -284,21 +285,13 @@ struct Warp {
     }
   }
 
-  // f grew by d: keeps M - f, so that l and its bound stay, when d is large
+  // f grew by d <= RISE
   __device__ __forceinline__ void raise(int d) {
-    const float by = (float)max(0, d - 40), f = ex2(-by), fl = ex2((float)d - by);
+    const float f = ex2((float)d);
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (m[n][i] > LOWEST) m[n][i] += by;
-        l[n][i] *= fl;
-#pragma unroll
-        for (int c = 0; c < MT; ++c) {
-          o[n][c][i] *= f;
-          o[n][c][i + 2] *= f;
-        }
-      }
+      for (int i = 0; i < 2; ++i) l[n][i] *= f;
   }
 };
 
@@ -358,9 +351,9 @@ __device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, in
         y[3] = fmaf(u2f(v[c].w), w, y[3]);
       }
     }
-    const float w = l == 0.f ? 0.f : (mg > LOWEST ? ex2(mg - ag) : 1.f) / l;
+    const float w = l == 0.f ? 0.f : 1.f / l, top = mg > LOWEST ? whole_pow2(mg - ag) : 1.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] *= w;
+    for (int i = 0; i < 4; ++i) y[i] = y[i] * w * top;
     store4<T>(static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D + d, y);
   }
   cluster_sync();  // this CTA's sums are read until here
@@ -456,7 +449,8 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
     const int see1 = min((long long)s.p0 + s.n - 1, (long long)cap - 1);
     const int chunk = ((META - 1) << a.c.lg_page) / UNIT;  // units whose pages are looked up together
     const long long head = (long long)kvh * a.c.page * D;
-    int f = 0;
+    int f = 0, f_first = 0;
+    bool far = false;
     if (tid == 0) meta.f = 0;
     for (int c0 = u; c0 < u1; c0 += chunk) {
       const int c1 = min(u1, c0 + chunk);
@@ -497,12 +491,15 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
       __syncthreads();
       const int f_old = f;
       f = meta.f;
-      if (tid < pages) {
-        const int at = max(ev, f - FAR);
-        meta.s[tid] = make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(at - 127),
-                                  ev == 255 ? 1.f : pow2_e8m0(127 + f - at), id >= 0 ? 1.f : 0.f);
+      if (c0 == u) f_first = f;
+      if (tid < pages)
+        meta.s[tid] = make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(ev - 127),
+                                  ev == 255 ? 1.f : pow2_e8m0(min(127 + f - ev, 254)), id >= 0 ? 1.f : 0.f);
+      far = __syncthreads_or(id >= 0 && ev < f - FAR) || f > f_first + RISE;
+      if (far) {  // (copies on their way land before the ring's memory is used otherwise)
+        copy_wait<0>();
+        break;
       }
-      __syncthreads();
       if (c0 > u && f > f_old) w.raise(f - f_old);
       if (c0 == u) {
         p_min = p_max = w.p[0][0];  // of the tile's rows
@@ -534,30 +531,49 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
       typename W::Query none = {};
       w.start(none, a, s, tile, lane);
     }
-    // the warps' sums, brought to a common M
+    if (far) {  // the segment anew, a row a warp; the other warps' places hold nothing
+      __syncthreads();
+      const int j0 = (s.u0 + u) * UNIT, j1 = (s.u0 + u1) * UNIT, lift = far_lift(a, b, kvh, j0, j1, lane);
+      f = 127 + lift;
+      for (int r = warp; r < R && first_rho + r < s.n * a.G; r += WARPS) {
+        const int rho = first_rho + r;
+        float m, l, o[D / 32];
+        far_row<T, D>(a, b, kvh, static_cast<const T *>(a.q) + (s.r0 + rho / a.G) * a.ld + (size_t)(kvh * a.G + rho % a.G) * D,
+                      row_pos(a, s, rho), j0, j1, lift, lane, m, l, o);
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+        for (int i = 0; i < WARPS; ++i) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int d = 4; d <= 16; d *= 2) w.l[n][i] += __shfl_xor_sync(0xffffffffu, w.l[n][i], d);
-        if (g == 0) {
-          sm[warp][8 * n + 2 * t + i] = w.m[n][i];
-          sl[warp][8 * n + 2 * t + i] = w.l[n][i];
+          for (int d = 0; d < D / 32; ++d) so[(i * R + r) * PAD + lane * (D / 32) + d] = i ? 0.f : o[d];
+          sm[i][r] = i ? LOWEST : m;
+          sl[i][r] = i ? 0.f : l;
         }
       }
-    __syncthreads();
+    } else {
+      // the warps' sums, brought to a common M
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+      for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = 8 * n + 2 * t + i;
-        const float f = ex2(w.m[n][i] - fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])));
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int c = 0; c < W::MT; ++c)
-          *reinterpret_cast<float2 *>(so + (warp * R + r) * PAD + g * (D / 8) + 2 * c) =
-              make_float2(w.o[n][c][i] * f, w.o[n][c][i + 2] * f);
-      }
+          for (int d = 4; d <= 16; d *= 2) w.l[n][i] += __shfl_xor_sync(0xffffffffu, w.l[n][i], d);
+          if (g == 0) {
+            sm[warp][8 * n + 2 * t + i] = w.m[n][i];
+            sl[warp][8 * n + 2 * t + i] = w.l[n][i];
+          }
+        }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = 8 * n + 2 * t + i;
+          const float f = ex2(w.m[n][i] - fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r])));
+#pragma unroll
+          for (int c = 0; c < W::MT; ++c)
+            *reinterpret_cast<float2 *>(so + (warp * R + r) * PAD + g * (D / 8) + 2 * c) =
+                make_float2(w.o[n][c][i] * f, w.o[n][c][i + 2] * f);
+        }
+    }
     __syncthreads();
     if (!a.split && gridDim.x > 1) {
       join_cluster<T, D, NQ>(a, s, tile, kvh, b, f, so, sm, sl);
@@ -690,8 +706,8 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
     y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
   }
   l = den[0] + den[1] + den[2] + den[3];
-  const float f = l == 0.f ? 0.f : (mg > LOWEST ? ex2(mg - ag) : 1.f) / l;
-  const float out[4] = {y.x * f, y.y * f, y.z * f, y.w * f};
+  const float f = l == 0.f ? 0.f : 1.f / l, top = mg > LOWEST ? whole_pow2(mg - ag) : 1.f;
+  const float out[4] = {y.x * f * top, y.y * f * top, y.z * f * top, y.w * f * top};
   store4<T>(dst, out);
 }
 

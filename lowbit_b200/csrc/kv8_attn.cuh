@@ -9,9 +9,13 @@ namespace lbc {
 namespace kv8 {
 
 constexpr float LOWEST = -3e38f;  // M before any visible token
-// blocks whose value scale is 2^60 below the largest count with 2^(f - 60): they
-// only matter to l (an all-zero block has exponent 0)
-constexpr int FAR = 60;
+// Both kernels add block j's weights to l with 2^(f - b_j), f the largest value
+// exponent looked up so far. That, and a weight that underflows while its share of
+// l does not, is sound while the exponents looked up together lie within FAR and
+// f grows by at most RISE after that (l <= 2^(15 + FAR + RISE) a token; a lost
+// weight is below 2^-50 of l). Where they lie farther apart, the rows are computed
+// by far_row.
+constexpr int FAR = 60, RISE = 30;
 
 // fp16 pieces of queries and of weights: fp32 needs 22 bits of both; bf16 and
 // fp16 queries are exact in one; fp16 outputs (11 bits) would show weights
@@ -65,6 +69,66 @@ __device__ __forceinline__ int row_pos(const AttnArgs &a, const Seq &s, int rho)
   const long long p = (long long)s.p0 + min(rho, s.n * a.G - 1) / a.G;
   return p >= ((long long)a.r.width << a.c.lg_page) ? -1 : (int)p;
 }
+
+// One row over the tokens [j0, j1) by one warp, for value scales of any spread: in
+// fp32 with the values themselves, o = 2^-lift sum 2^(z_j - m) v_j and l = sum
+// 2^(z_j - m), m the largest z_j rounded up. A lane holds D / 32 elements. Not
+// fast, and seldom run: a token at a time, with few registers, so that the
+// kernels around it keep theirs.
+template <typename T, int D>
+__device__ __forceinline__ void far_row(const AttnArgs &a, int b, int kvh, const T *q, int p, int j0, int j1, int lift, int lane,
+                                        float &m, float &l, float (&o)[D / 32]) {
+  constexpr int E = D / 32;  // elements a lane
+  const int lo = max(j0, a.window > 0 ? max(0, p - a.window + 1) : 0), hi = min(j1, p + 1);
+  float x[E], amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    x[i] = to_f<T>(q[lane * E + i]);
+    amax = x[i] == x[i] ? fmaxf(amax, fabsf(x[i])) : INFINITY;
+  }
+#pragma unroll
+  for (int d = 16; d >= 1; d /= 2) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+  const float up = fp16_range(amax), back = a.scale_log2 / up, down = lift ? ex2(-(float)lift) : 1.f;
+  m = LOWEST;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    x[i] *= up;
+    o[i] = 0.f;
+  }
+#pragma unroll 1
+  for (int j = lo; j < hi; ++j) {
+    const int id = a.r.table[(size_t)b * a.r.width + (j >> a.c.lg_page)];
+    if ((unsigned)id >= (unsigned)a.c.pages) continue;
+    const long long off = id * a.c.page_stride + ((long long)kvh * a.c.page + (j & (a.c.page - 1))) * D + lane * E;
+    const long long at = id * a.c.exp_stride + kvh;
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) z = fmaf(x[i], (float)a.c.k[off + i], z);
+#pragma unroll
+    for (int d = 16; d >= 1; d /= 2) z += __shfl_xor_sync(0xffffffffu, z, d);
+    z *= back * pow2_e8m0(a.c.k_exp[at]);
+    const float to = fmaxf(m, ceilf(z)), f = ex2(m - to), w = ex2(z - to), value = pow2_e8m0(a.c.v_exp[at]) * down;
+    m = to;
+    l = fmaf(l, f, w);
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = fmaf(w, (float)a.c.v[off + i] * value, o[i] * f);
+  }
+}
+
+// far_row's `lift` for the tokens [j0, j1) of sequence b: 20 where sums of the largest values could pass fp32's range
+__device__ __forceinline__ int far_lift(const AttnArgs &a, int b, int kvh, int j0, int j1, int lane) {
+  int top = 0;
+  for (int i = (j0 >> a.c.lg_page) + lane; i < a.r.width && i <= (j1 - 1) >> a.c.lg_page; i += 32) {
+    const int id = a.r.table[(size_t)b * a.r.width + i];
+    const int ev = (unsigned)id < (unsigned)a.c.pages ? a.c.v_exp[id * a.c.exp_stride + kvh] : 255;
+    if (ev != 255) top = max(top, ev);
+  }
+  return __any_sync(0xffffffffu, top > 220) ? 20 : 0;
+}
+
+// 2^x of a whole number (the exponential unit would make 2^-127, of a block of exponent 0, a zero)
+__device__ __forceinline__ float whole_pow2(float x) { return x == -127.f ? pow2_e8m0(0) : ex2(x); }
 
 // prompt chunks (kv8_prompt.cu), and the rows that one of its CTAs takes
 int prompt_rows(int dtype, int D);

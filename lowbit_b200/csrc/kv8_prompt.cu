@@ -44,12 +44,14 @@ constexpr int R_ROWS = 184, R_DEQ = 72, R_REST = 64;
 static_assert(256 * R_ROWS + 128 * (R_DEQ + R_REST) <= THREADS * 128, "a block's registers");
 constexpr int META = 8;       // steps whose block scales are looked up together; two such sets are kept
 constexpr int RAW = 4;        // steps whose codes are in flight or waiting
+// added to a set's f from where the value exponents lie farther apart than the row warps' sums allow (kv8_attn.cuh: FAR)
+constexpr int APART = 1024;
 // weights: M is the maximum (rounded up) less 12, left alone up to 2^15
 constexpr float HEAD = 12.f, SLACK = 15.f;
 
 struct Scales {
   float4 g[META][NT / 16];  // of each 16 tokens: 2^(ek - 127), b = ev - 127, 2^(f - b), 1 if the page exists
-  int f, all, pad[2];       // all: every page of the set exists
+  int f, all, pad[2];       // f: largest value exponent so far; all: every page of the set exists
 };
 
 // Full / empty pairs of the rings (two stages each; phase j >> 1), S and P full
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
     reg_dec<R_REST>();
     const int o_lo = (int)(see0 >> a.c.lg_page), o_hi = (int)(p_last >> a.c.lg_page);
     const int32_t *ids = a.r.table + (size_t)b * a.r.width;
-    int f = 0;  // largest value exponent so far (255 left out)
+    int f = 0, f_first = 0, far = 0;  // largest value exponent so far (255 left out), and of the first set
     for (int j = 0; j < steps; j += META) {
       const int set = j / META & 1;
       const int id = ids[min(max(((t0 + j) * NT + lane * 16) >> a.c.lg_page, o_lo), o_hi)];
@@ -264,13 +266,15 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       if (!there) set_status(a.r.status, LBC_ERR_PAGE);
       const int ek = there ? a.c.k_exp[id * a.c.exp_stride + kvh] : 0, ev = there ? a.c.v_exp[id * a.c.exp_stride + kvh] : 0;
       f = max(f, __reduce_max_sync(0xffffffffu, ev == 255 ? 0 : ev));
-      const int at = max(ev, f - FAR), all = __all_sync(0xffffffffu, there);
+      if (j == 0) f_first = f;
+      const int all = __all_sync(0xffffffffu, there);
+      if (__any_sync(0xffffffffu, there && ev < f - FAR) || f > f_first + RISE) far = APART;
       if (!wait(&sh.meta_empty[set], (j / META >> 1 & 1) ^ 1u)) break;
       sh.meta[set].g[lane / (NT / 16)][lane % (NT / 16)] =
-          make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(at - 127),
-                      ev == 255 ? 1.f : pow2_e8m0(127 + f - at), there ? 1.f : 0.f);
+          make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(ev - 127),
+                      ev == 255 ? 1.f : pow2_e8m0(min(127 + f - ev, 254)), there ? 1.f : 0.f);
       if (lane == 0) {
-        sh.meta[set].f = f;
+        sh.meta[set].f = f + far;
         sh.meta[set].all = all;
       }
       __syncwarp();
@@ -433,27 +437,23 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         mg[g] = fmaxf(m0, m1);
       }
       const float mx = fmaxf(fmaxf(mg[0], mg[1]), fmaxf(mg[2], mg[3]));
-      // a larger f scales l; a much larger one also moves M (kv8_attention.cu: raise)
-      float by = 0.f;
-      if (meta.f > f) {
+      if (meta.f > f) {  // a larger f scales l
         if (j > 0) {
-          by = (float)max(0, meta.f - f - 40);
-          const float w = ex2((float)(meta.f - f) - by);
+          const float w = ex2((float)(meta.f - f));
           ls[0] = mul2(ls[0], pair(w, w));
           ls[1] = mul2(ls[1], pair(w, w));
         }
         f = meta.f;
       }
-      const bool rise = __any_sync(0xffffffffu, mx > m + SLACK) || by > 0.f;
+      const bool rise = __any_sync(0xffffffffu, mx > m + SLACK);
       if (rise || (L::FOLD && j > 0)) {
         float scale = 1.f;
         if (rise) {
-          const float to = m > LOWEST ? m + by : m;
-          m = fmaxf(to, ceilf(mx) - HEAD);
-          scale = ex2(to - m);
+          const float to = fmaxf(m, ceilf(mx) - HEAD);
+          scale = ex2(m - to);
+          m = to;
           ls[0] = mul2(ls[0], pair(scale, scale));
           ls[1] = mul2(ls[1], pair(scale, scale));
-          scale *= ex2(-by);
         }
         if (j > 0) {
           ok = wait(&sh.pv_done[i][st ^ 1], ((j - 1) >> 1) & 1);
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       split(ls[1], x2, x3);
       l = (u2f(x0) + u2f(x1)) + (u2f(x2) + u2f(x3));
     }
-    const float w = l == 0.f || steps == 0 ? 0.f : pow2_e8m0(f) / l;
+    const float w = l == 0.f || steps == 0 ? 0.f : 1.f / l, top = pow2_e8m0(f);  // (2^f / l can be too small for fp32)
     // the warp's rows through shared memory (16-byte pieces change places by row), then out in whole rows
     T *stage = reinterpret_cast<T *>(mine) + (warp & 3) * 32 * D;
 #pragma unroll
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         for (int h = 0; h < E; h += 4) {
           float y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = w == 0.f ? 0.f : u2f(o[k + h + e]) * w;
+          for (int e = 0; e < 4; ++e) y[e] = w == 0.f ? 0.f : u2f(o[k + h + e]) * w * top;
           store4<T>(dst + h, y);
         }
       }
@@ -551,6 +551,20 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       if (row < s.n * a.G)
         *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + ((size_t)(s.r0 + row / a.G) * a.H + kvh * a.G + row % a.G) * D +
                                    lane % LR * E) = v;
+    }
+    // the rows anew, one after another, where the scales lie too far apart (kv8_attn.cuh: FAR)
+    if (steps > 0 && ok && f >= APART) {
+      __syncwarp();  // behind the stores above
+      const int lift = f > APART + 220 ? 20 : 0;
+      for (int row = first; row < min(first + 32, s.n * a.G); ++row) {
+        const size_t at = (size_t)(s.r0 + row / a.G);
+        float m, l, o[D / 32];
+        far_row<T, D>(a, b, kvh, static_cast<const T *>(a.q) + at * a.ld + (size_t)(kvh * a.G + row % a.G) * D,
+                      __shfl_sync(0xffffffffu, p, row - first), 0, 0x7fffffff, lift, lane, m, l, o);
+        T *dst = static_cast<T *>(a.out) + (at * a.H + kvh * a.G + row % a.G) * D + lane * (D / 32);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) dst[d] = from_f<T>(l == 0.f ? 0.f : o[d] / l * (lift ? ex2((float)lift) : 1.f));
+      }
     }
   }
   tc::fence_before_sync();

@@ -23,7 +23,7 @@ def seeded():
 @pytest.mark.parametrize("d", [32, 64, 128])
 def test_tiles_of_padding_are_zero(dt, d):
     """Prompts whose whole row tiles see nothing (before position 0, or past the table under a window): exact
-    zeros every time, and the other rows are right."""
+    zeros every time, and the other rows are right. (Twelve such sequences take the prompt kernel.)"""
     rng = np.random.default_rng(40)
     b, new, page = 12, 150, 64
     pool = G.host_pool(rng, 5 * b, 4, page, d)
@@ -49,8 +49,153 @@ def test_tiles_of_padding_are_zero(dt, d):
     assert K.device_status(reset=True) == G.ERR_PAGE
 
 
-def test_tiles_of_padding_take_the_prompt_kernel():
-    cache = lb.KV8Cache.empty(60, 4, 64, page=64)
-    q, table, pos = torch.ones((12 * 150, 8, 64), device="cuda"), G.i32(np.arange(60).reshape(12, 5)), G.i32([-150] * 12)
-    lb.kv8_attention(q, cache, table, pos)
-    assert "prompt_kernel" in G.kernels_of(lambda: lb.kv8_attention(q, cache, table, pos))
+# ---------------------------------------------------------------- value scales far apart
+
+def check(out, pool, q, table, pos, window, dt, d):
+    """test_kv8_gpu.check with what weights held in fp16 lose at their lower end: half a subnormal step, 2^-25, where the
+    row's largest p_i 2^b_i (b: the value exponent) stands for 2^13 or more: at most 2^-38 of it a code."""
+    ref, mag, size = R.attention(pool, q, table, pos, window=window)
+    kv, page = pool["k"].shape[1:3]
+    n, heads = q.shape[:2]
+    floor, new = np.zeros((n, heads, 1)), n // len(pos)
+    for i in range(n):
+        p = pos[i // new] + i % new
+        lo = max(0, p - window + 1) if window else 0
+        ids = table[i // new, :-(-(p + 1) // page)]
+        for h in range(heads):
+            g = h // (heads // kv)
+            k = (pool["k"][ids, g] * R.pow2(pool["k_exp"][ids, g])[:, None, None]).reshape(-1, d)[lo:p + 1]
+            s = k @ q[i, h] / d ** 0.5
+            w = np.exp(s - s.max())
+            floor[i, h] = (w / w.sum() * R.pow2(pool["v_exp"][ids, g]).repeat(page)[lo:p + 1]).max() * 127 * len(w)
+    u, longest = 2.0 ** -22, max(pos) + new
+    tol = mag * ((2 * (d + 8) * size[..., None] + longest + 16) * u + G.R_P[dt]) + floor * 2.0 ** -38
+    err = np.abs(out.double().cpu().numpy() - ref)
+    assert np.isfinite(err).all()
+    assert (err <= tol + np.maximum(G.R_OUT[dt] * np.abs(ref), G.TINY[dt])).all()
+
+
+def far_case(dt, pos, new, low, gap, page, d, window=0, steer=False, b=1):
+    """Value blocks of the pages `low` (a table slot, or a list of them) 2^gap below the others. `steer`: keys and
+    queries that put the weight on those."""
+    rng = np.random.default_rng(41)
+    width = -(-(max(pos) + new) // page)
+    pool = G.host_pool(rng, b * width, 2, page, d, 0.0)
+    table = rng.permutation(b * width).reshape(b, width)
+    pool["v_exp"] = (pool["v_exp"].astype(int) + 60 * (gap > 110)).astype(np.uint8)
+    ids = table[:, np.atleast_1d(low)]
+    pool["v_exp"][ids] -= gap
+    q = rng.standard_normal((b * new, 4, d))
+    if steer:
+        pool["k"] = -np.abs(pool["k"])
+        pool["k"][ids] = np.abs(pool["k"][ids])
+        q = np.abs(q) * 4
+    q = torch.from_numpy(q.astype(np.float32)).to(G.TYPES[dt])
+    out = lb.kv8_attention(q.cuda(), G.device_pool(pool), G.i32(table), G.i32(pos), window=window)
+    check(out, pool, q.double().numpy(), table, pos, window, dt, d)
+    assert K.device_status(reset=True) == 0
+
+
+GAPS = [40, 59, 62, 75, 110, 170]
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("page,d", [(16, 32), (32, 64), (64, 128)])
+def test_rows_that_see_small_values_only(dt, gap, page, d):
+    """Later, larger tokens do not change a row that does not see them: few rows, prompts, windows."""
+    far_case(dt, [page - 2], 5, 0, gap, page, d)                # the first rows end inside the small block
+    far_case(dt, [2 * page - 3], 6, 1, gap, page, d, window=2)  # some rows' windows hold small tokens only
+    far_case(dt, [0] * 12, 100, 0, gap, page, d, b=12)
+    far_case(dt, [3] * 12, 140, [1, 2], gap, page, d, window=9, b=12)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("new,b", [(1, 1), (5, 3), (100, 12)])
+def test_weight_on_small_values(dt, gap, new, b):
+    """Large values are seen, but the weight lies on small ones."""
+    far_case(dt, [150] * b, new, [1, 3], gap, 32, 64, steer=True, b=b)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("new", [1, 2, 3])
+@pytest.mark.parametrize("page,step", [(16, 10), (16, 4), (64, 1)])
+def test_scales_that_rise_along_a_long_context(dt, new, page, step):
+    """Each `step` pages twice the last ones' values, over enough sequences that a block of the grid looks pages up
+    several times; windows that end anywhere. Within the bound of test_kv8_gpu.check, which is relative to the row."""
+    rng = np.random.default_rng(42)
+    kv, d, b, length, window = 8, 32, 64, 8192, 700
+    n = length // page
+    pool = G.host_pool(rng, n, kv, page, d, 0.0)
+    pool["v_exp"] = (20 + np.arange(n)[:, None] // step + 0 * pool["v_exp"]).astype(np.uint8)
+    table = np.broadcast_to(np.arange(n), (b, n))
+    pos = np.linspace(window, length - new, b).astype(int)
+    q = torch.randn((b * new, kv, d), device="cuda").to(G.TYPES[dt])
+    k, v = (torch.from_numpy((pool[m] * R.pow2(pool[m + "_exp"])[..., None, None]).transpose(1, 0, 2, 3).reshape(kv, length, d)).cuda()
+            for m in "kv")
+    at = (torch.from_numpy(pos).cuda()[:, None] + torch.arange(new, device="cuda")).view(-1, 1)
+    j = torch.arange(length, device="cuda")
+    s = torch.einsum("rhd,hld->rhl", q.double(), k) / d ** 0.5
+    size = torch.einsum("rhd,hld->rhl", q.double().abs(), k.abs()).amax(-1) / d ** 0.5
+    for win in (0, window):
+        seen = (j <= at) & ((j > at - win) if win else True)
+        p = s.masked_fill(~seen[:, None], -torch.inf).softmax(-1)
+        ref, mag = torch.einsum("rhl,hld->rhd", p, v), torch.einsum("rhl,hld->rhd", p, v.abs())
+        out = lb.kv8_attention(q, G.device_pool(pool), G.i32(table), G.i32(pos), window=win)
+        G.check(out, ref.cpu().numpy(), mag.cpu().numpy(), size.cpu().numpy(), dt, d, length)
+
+
+@pytest.mark.parametrize("new,b", [(1, 1), (100, 12)])
+def test_largest_and_smallest_values_together(new, b):
+    """Values near the type's end beside ones 2^200 below: sums stay finite."""
+    rng = np.random.default_rng(43)
+    pool = G.host_pool(rng, 8 * b, 2, 32, 64, 0.0)
+    pool["v"] = np.clip(pool["v"], -63, 63)
+    table = rng.permutation(8 * b).reshape(b, 8)
+    pool["v_exp"][:] = 249
+    pool["v_exp"][table[:, ::2]] = 49
+    q = rng.standard_normal((b * new, 4, 64)).astype(np.float32)
+    pos = [256 - new] * b
+    out = lb.kv8_attention(torch.from_numpy(q).cuda(), G.device_pool(pool), G.i32(table), G.i32(pos))
+    G.check(out, *R.attention(pool, q, table, pos), "fp32", 64, 256)
+
+
+@pytest.mark.parametrize("dt", G.TYPES)
+@pytest.mark.parametrize("new,b", [(3, 2), (100, 12)])
+def test_far_scales_with_bad_places(dt, new, b):
+    """Where the scales are far apart too: a NaN block spoils the rows that see it, a missing page is left out."""
+    rng = np.random.default_rng(44)
+    page, d, w = 16, 64, 10
+    pool = G.host_pool(rng, b * w, 2, page, d, 0.0)
+    table = rng.permutation(b * w).reshape(b, w)
+    pool["v_exp"][table[:, 1]] -= 80
+    pool["v_exp"][table[0, 4], 1] = 255
+    p0 = 5 * page - new // 2
+    pos = [p0] * b
+    q = torch.randn((b * new, 4, d), device="cuda").to(G.TYPES[dt])
+    cache = G.device_pool(pool)
+    out = lb.kv8_attention(q, cache, G.i32(table), G.i32(pos), window=200).float().cpu().numpy().reshape(b, new, 4, d)
+    sees = p0 + np.arange(new) >= 4 * page
+    assert np.isnan(out[0, sees, 2:]).all() and np.isfinite(out[0, ~sees]).all()
+    assert np.isfinite(out[0, :, :2]).all() and np.isfinite(out[1:]).all()
+    clean = {n: a.copy() for n, a in pool.items()}
+    clean["v_exp"][table[0, 4], 1] = 121
+    K.device_status(reset=True)
+    bad = table.copy()
+    bad[1, 3] = -1
+    out = lb.kv8_attention(q, G.device_pool(clean), G.i32(bad), G.i32(pos))
+    assert K.device_status(reset=True) == G.ERR_PAGE
+    # leaving page 3 out is a row over the remaining tokens
+    keep = np.r_[0:3 * page, 4 * page:w * page]
+    k, v = (torch.from_numpy((clean[n][table[1]] * R.pow2(clean[n + "_exp"][table[1]])[..., None, None])
+                             .transpose(1, 0, 2, 3).reshape(2, w * page, d)).cuda() for n in "kv")
+    x = q.double().view(b, new, 2, 2, d)[1]
+    s = torch.einsum("tkgd,kld->tkgl", x, k) / d ** 0.5
+    size = torch.einsum("tkgd,kld->tkgl", x.abs(), k.abs()).amax(-1) / d ** 0.5
+    at = p0 + torch.arange(new, device="cuda")[:, None]
+    j = torch.arange(w * page, device="cuda")
+    seen = (j <= at) & torch.isin(j, torch.from_numpy(keep).cuda())
+    p = s.masked_fill(~seen[:, None, None], -torch.inf).softmax(-1)
+    ref, mag = torch.einsum("tkgl,kld->tkgd", p, v), torch.einsum("tkgl,kld->tkgd", p, v.abs())
+    G.check(out.view(b, new, 4, d)[1], *(t.reshape(new, 4, -1).squeeze(-1).cpu().numpy() for t in (ref, mag, size)), dt, d, w * page)

@@ -213,7 +213,7 @@ struct Warp {
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) rise |= fmaxf(z[n][i], z[n][i + 2]) > m[n][i] + SLACK;
+      for (int i = 0; i < 2; ++i) rise |= fmaxf(z[n][i], z[n][i + 2]) - m[n][i] > SLACK;
     if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
@@ -222,7 +222,7 @@ struct Warp {
           float mx = fmaxf(z[n][i], z[n][i + 2]);
 #pragma unroll
           for (int d = 4; d <= 16; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-          const float to = fmaxf(m[n][i], ceilf(mx) - HEAD), f = ex2(m[n][i] - to);
+          const float to = fmaxf(m[n][i], reference(mx, HEAD, SLACK)), f = ex2(m[n][i] - to);
           m[n][i] = to;
           l[n][i] *= f;
 #pragma unroll
@@ -301,7 +301,7 @@ template <typename T, int D, int NQ>
 __device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, int tile, int kvh, int b, int f, float *so,
                                              float (*sm)[8 * NQ], float (*sl)[8 * NQ]) {
   constexpr int R = 8 * NQ, PAD = D + 4;
-  __shared__ float mine[3][R];  // M, M - f, l
+  __shared__ float mine[3][R];  // M, f, l
   const int tid = threadIdx.x, size = gridDim.x, rank = blockIdx.x;
   for (int x = tid; x < R * (D / 4); x += THREADS) {  // the four warps' O into the first one's place
     float4 *y = reinterpret_cast<float4 *>(so + x / (D / 4) * PAD + x % (D / 4) * 4);
@@ -316,7 +316,7 @@ __device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, in
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) l = fmaf(sl[i][tid], ex2(sm[i][tid] - m), l);
     mine[0][tid] = m;
-    mine[1][tid] = m > LOWEST ? m - (float)(f - 127) : LOWEST;
+    mine[1][tid] = (float)(f - 127);
     mine[2][tid] = l;
   }
   cluster_sync();
@@ -325,26 +325,26 @@ __device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, in
     const int r = x / (D / 4), d = x % (D / 4) * 4, rho = tile * R + r;
     if (rho >= s.n * a.G) continue;
     // all CTAs' values at once: one remote latency (a rank past the size reads its own again, and is left out)
-    float m[8], af[8], lc[8], mg = LOWEST, ag = LOWEST, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    float m[8], fc[8], lc[8], mg = LOWEST, ag = LOWEST, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
     uint4 v[8];
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       const uint32_t from = c < size ? c : rank;
       m[c] = ld_dsmem_f32(dsmem_addr(&mine[0][r], from));
-      af[c] = ld_dsmem_f32(dsmem_addr(&mine[1][r], from));
+      fc[c] = ld_dsmem_f32(dsmem_addr(&mine[1][r], from));
       lc[c] = ld_dsmem_f32(dsmem_addr(&mine[2][r], from));
       v[c] = ld_dsmem_v4(dsmem_addr(so + r * PAD + d, from));
     }
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       mg = fmaxf(mg, m[c]);
-      ag = fmaxf(ag, af[c]);
+      if (m[c] > LOWEST) ag = fmaxf(ag, m[c] - fc[c]);
     }
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       if (c < size) {
         const float w = ex2(m[c] - mg);
-        l = fmaf(lc[c], m[c] > LOWEST ? ex2(af[c] - ag) : 1.f, l);
+        l = fmaf(lc[c], m[c] > LOWEST ? ex2((m[c] - ag) - fc[c]) : 1.f, l);  // (M - f alone rounds where scores pass 2^24)
         y[0] = fmaf(u2f(v[c].x), w, y[0]);
         y[1] = fmaf(u2f(v[c].y), w, y[1]);
         y[2] = fmaf(u2f(v[c].z), w, y[2]);
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
     if (tid < n) {
       const float *q = record(c0 + tid) + R * D + r;
       wo[tid] = ex2(q[0] - mg);
-      l = fmaf(q[R], q[0] > LOWEST ? ex2(q[0] - q[2 * R] - ag) : 1.f, l);
+      l = fmaf(q[R], q[0] > LOWEST ? ex2((q[0] - ag) - q[2 * R]) : 1.f, l);
     }
     __syncthreads();
 #pragma unroll 4

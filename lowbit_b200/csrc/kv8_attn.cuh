@@ -70,6 +70,13 @@ __device__ __forceinline__ int row_pos(const AttnArgs &a, const Seq &s, int rho)
   return p >= ((long long)a.r.width << a.c.lg_page) ? -1 : (int)p;
 }
 
+// M for the largest t: `head` below it, rounded up; t itself where floats are too
+// sparse for that (from 2^25 on `head` rounds to more than fp16 weights allow)
+__device__ __forceinline__ float reference(float t, float head, float slack) {
+  const float m = ceilf(t) - head;
+  return t - m > slack ? t : m;
+}
+
 // One row over the tokens [j0, j1) by one warp, for value scales of any spread: in
 // fp32 with the values themselves, o = 2^-lift sum 2^(z_j - m) v_j and l = sum
 // 2^(z_j - m), m the largest z_j rounded up. A lane holds D / 32 elements. Not

@@ -445,11 +445,11 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         }
         f = meta.f;
       }
-      const bool rise = __any_sync(0xffffffffu, mx > m + SLACK);
+      const bool rise = __any_sync(0xffffffffu, mx - m > SLACK);
       if (rise || (L::FOLD && j > 0)) {
         float scale = 1.f;
         if (rise) {
-          const float to = fmaxf(m, ceilf(mx) - HEAD);
+          const float to = fmaxf(m, reference(mx, HEAD, SLACK));
           scale = ex2(m - to);
           m = to;
           ls[0] = mul2(ls[0], pair(scale, scale));

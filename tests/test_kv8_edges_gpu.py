@@ -199,3 +199,22 @@ def test_far_scales_with_bad_places(dt, new, b):
     p = s.masked_fill(~seen[:, None, None], -torch.inf).softmax(-1)
     ref, mag = torch.einsum("tkgl,kld->tkgd", p, v), torch.einsum("tkgl,kld->tkgd", p, v.abs())
     G.check(out.view(b, new, 4, d)[1], *(t.reshape(new, 4, -1).squeeze(-1).cpu().numpy() for t in (ref, mag, size)), dt, d, w * page)
+
+
+@pytest.mark.parametrize("dt", G.TYPES)
+@pytest.mark.parametrize("new,b,length", [(1, 1, 500), (1, 1, 60000), (3, 40, 900), (100, 12, 300)])
+def test_scores_past_2_to_24(dt, new, b, length):
+    """Scores so large that whole numbers are no longer exact in fp32: a row stays between its smallest and largest
+    visible value (a factor 2 of the softmax's references would leave that range)."""
+    rng = np.random.default_rng(45)
+    page = 64
+    width = -(-length // page)
+    pool = G.host_pool(rng, width, 2, page, 64)
+    pool["v"] = np.maximum(np.abs(pool["v"]), 32).astype(np.int8)  # a block's values lie within a factor 4
+    table = np.broadcast_to(np.arange(width), (b, width))
+    q = torch.randn((b * new, 4, 64), device="cuda").to(G.TYPES[dt])
+    cache, v = G.device_pool(pool), pool["v"] * R.pow2(pool["v_exp"])[..., None, None]
+    lo, hi = v.min((0, 2)).repeat(2, 0), v.max((0, 2)).repeat(2, 0)  # by query head
+    for scale in 2.0 ** np.arange(16, 64, 1.5):
+        out = lb.kv8_attention(q, cache, G.i32(table), G.i32([length - new] * b), scale=scale).double().cpu().numpy()
+        assert (out >= lo * (1 - 2.0 ** -8)).all() and (out <= hi * (1 + 2.0 ** -8)).all(), scale

@@ -147,7 +147,10 @@ class PagedKVCache:
     """The model's cache over KV8Cache pools: one pool a layer, one page table
     and one position a sequence, shared by the layers. Sequences have lengths
     of their own. Pages are handed out from a free list as sequences grow
-    (``reserve``) and go back with ``release``.
+    (``reserve``) and go back with ``release``. Table entries without a page
+    are -1: a token past its sequence's pages is not stored, and recorded
+    (kernels.device_status()). A released place is padding (``pos`` -1) until
+    tokens are reserved for it.
 
     Interface of model.KVCache: ``batch``, ``capacity``, ``pos`` (int32 [batch]
     on the GPU), ``length`` (sequences of equal length), ``reset()``."""
@@ -160,10 +163,11 @@ class PagedKVCache:
         n = batch * width if pages is None else int(pages)
         self.layers = [KV8Cache.empty(n, cfg.num_kv_heads, cfg.head_dim, page) for _ in range(cfg.num_layers)]
         dev = self.layers[0].device
-        self.table = torch.zeros((batch, width), dtype=torch.int32, device=dev)
+        self.table = torch.full((batch, width), -1, dtype=torch.int32, device=dev)
         self.pos = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.lengths = [0] * batch
         self._owned = [[] for _ in range(batch)]
+        self._released = set()
         self._free = list(range(n - 1, -1, -1))
 
     @property
@@ -176,30 +180,38 @@ class PagedKVCache:
 
     def reserve(self, tokens) -> None:
         """Pages for ``tokens[b]`` tokens of every sequence (an int: the same
-        for all); raises ValueError, with nothing changed, when they do not fit."""
-        tokens = [int(tokens)] * self.batch if isinstance(tokens, int) else [int(t) for t in tokens]
+        for all); raises ValueError, with nothing changed, when they do not fit.
+        A released place starts again at position 0; None leaves a place as it is."""
+        tokens = [tokens] * self.batch if isinstance(tokens, int) else list(tokens)
         if len(tokens) != self.batch:
             raise ValueError(f"{len(tokens)} lengths for {self.batch} sequences")
+        started = [b for b in sorted(self._released) if tokens[b] is not None]
+        tokens = [0 if t is None else int(t) for t in tokens]
         if max(tokens) > self._max_len:
             raise ValueError(f"KV cache full ({max(tokens)} > {self._max_len})")
         more = [max(0, -(-t // self.page) - len(own)) for t, own in zip(tokens, self._owned)]
         if sum(more) > len(self._free):
             raise ValueError(f"KV cache out of pages ({sum(more)} needed, {len(self._free)} free)")
+        for b in started:
+            self.pos[b] = 0
+        self._released.difference_update(started)
         if not any(more):
             return
         for own, m in zip(self._owned, more):
             own.extend(self._free.pop() for _ in range(m))
-        host = torch.zeros(self.table.shape, dtype=torch.int32)
+        host = torch.full(self.table.shape, -1, dtype=torch.int32)
         for b, own in enumerate(self._owned):
             host[b, :len(own)] = torch.tensor(own, dtype=torch.int32)
         self.table.copy_(host)
 
     def release(self, b: int) -> None:
-        """Empty sequence b and return its pages."""
+        """Empty sequence b and return its pages; its place is padding from here on."""
         self._free.extend(reversed(self._owned[b]))
         self._owned[b] = []
+        self._released.add(b)
         self.lengths[b] = 0
-        self.pos[b] = 0
+        self.table[b] = -1
+        self.pos[b] = -1
 
     @property
     def length(self) -> int:
@@ -212,8 +224,10 @@ class PagedKVCache:
         self.set_lengths([int(n)] * self.batch)
 
     def set_lengths(self, lengths) -> None:
+        """Sets the sequences' lengths; a released place of length 0 stays padding."""
         self.lengths = [int(n) for n in lengths]
-        self.pos.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+        self._released = {b for b in self._released if self.lengths[b] == 0}
+        self.pos.copy_(torch.tensor([-1 if b in self._released else n for b, n in enumerate(self.lengths)], dtype=torch.int32))
 
     def reset(self) -> None:
         """Empty every sequence (pools, table and pages stay, so a captured decode graph stays valid)."""

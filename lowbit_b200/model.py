@@ -818,7 +818,7 @@ class Model:
             if isinstance(cache, KVCache):
                 _check(_lib().lbc_advance_pos(cache.pos.data_ptr(), 1, _stream()), "lbc_advance_pos")
             else:
-                cache.pos.add_(1)  # one position a sequence
+                cache.pos.add_(cache.pos >= 0)  # one position a sequence; places of padding (-1) stay
         self.prof.close()
 
     def generate(self, prompt, n_new: int, cache: KVCache | None = None, timings: dict | None = None,

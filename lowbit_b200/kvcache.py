@@ -159,7 +159,7 @@ class PagedKVCache:
         if batch <= 0 or max_len <= 0:
             raise ValueError("a cache holds at least one sequence of one token")
         width = -(-max_len // page)
-        self.batch, self.page, self._max_len = batch, page, max_len
+        self.batch, self.page, self._max_len, self._positions = batch, page, max_len, cfg.max_position
         n = batch * width if pages is None else int(pages)
         self.layers = [KV8Cache.empty(n, cfg.num_kv_heads, cfg.head_dim, page) for _ in range(cfg.num_layers)]
         dev = self.layers[0].device
@@ -189,6 +189,8 @@ class PagedKVCache:
         tokens = [0 if t is None else int(t) for t in tokens]
         if max(tokens) > self._max_len:
             raise ValueError(f"KV cache full ({max(tokens)} > {self._max_len})")
+        if max(tokens) > self._positions:  # the append would store nothing past the rotation tables
+            raise ValueError(f"{max(tokens)} tokens pass the model's max_position ({self._positions})")
         more = [max(0, -(-t // self.page) - len(own)) for t, own in zip(tokens, self._owned)]
         if sum(more) > len(self._free):
             raise ValueError(f"KV cache out of pages ({sum(more)} needed, {len(self._free)} free)")

@@ -99,3 +99,21 @@ def test_a_place_is_used_again(graph):
         # the last token of the six was not appended, the sixth step's input was: the histories agree
         assert one.length == len(prompts[b]) + 5
         assert m.generate(turn[b], 4, cache=one, graph=graph) == got[b]
+
+
+def test_lengths_stop_at_the_rotation_tables():
+    """A cache may be longer than the model's positions, its sequences may not."""
+    cfg = PM.tiny_config(max_position=40)
+    m = PM.Model(cfg, PM.random_weights(cfg, seed=6), backend="fp32")
+    K.device_status(reset=True)
+    c = m.new_cache(100, batch=2, kind="kv8", page=16)
+    got = m.generate_ragged([[1, 2, 3], [4] * 36], 5, cache=c)  # the fifth token is not appended
+    assert c.lengths == [7, 40] and len(got[1]) == 5
+    for call in (lambda: m.generate_ragged([[1], [2]], 1, cache=c), lambda: c.reserve([1, 41]),
+                 lambda: m.generate_ragged([[1] * 38], 4), lambda: m.generate([1] * 38, 4, cache=m.new_cache(64, kind="kv8")),
+                 lambda: m.forward([1] * 41, m.new_cache(64, kind="kv8"))):
+        with pytest.raises(ValueError, match="max_position"):
+            call()
+    assert c.lengths == [7, 40] and K.device_status(reset=True) == 0
+    m.forward([1] * 40, m.new_cache(64, kind="kv8"))
+    assert K.device_status(reset=True) == 0

@@ -77,10 +77,12 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
 
 // a power of two that brings |x| <= amax to at most 2^14 (its top to 2^13 and
 // more), so that two fp16 pieces hold 22 bits of everything down to 2^-16 of
-// the largest; 1 for non-finite rows, whose fp16 form then stays non-finite
+// the largest; NaN for non-finite rows: an infinite query makes every score
+// infinite or NaN, so a row that sees anything is NaN (scores of -inf alone would
+// look like a row that sees nothing)
 __device__ __forceinline__ float fp16_range(float amax) {
   const int e = (int)(__float_as_uint(amax) >> 23) & 255;
-  if (e == 255) return 1.f;
+  if (e == 255) return __uint_as_float(0x7fc00000u);
   return __uint_as_float((uint32_t)(min(13 + 127 - e, 126) + 127) << 23);
 }
 

@@ -218,3 +218,33 @@ def test_scores_past_2_to_24(dt, new, b, length):
     for scale in 2.0 ** np.arange(16, 64, 1.5):
         out = lb.kv8_attention(q, cache, G.i32(table), G.i32([length - new] * b), scale=scale).double().cpu().numpy()
         assert (out >= lo * (1 - 2.0 ** -8)).all() and (out <= hi * (1 + 2.0 ** -8)).all(), scale
+
+
+@pytest.mark.parametrize("dt", G.TYPES)
+@pytest.mark.parametrize("new,b", [(1, 1), (1, 40), (3, 2), (100, 12)])
+def test_infinite_queries(dt, new, b):
+    """softmax of infinite scores is NaN, whatever their signs; a row that sees nothing is 0 whatever its query;
+    other rows are as without them."""
+    rng = np.random.default_rng(46)
+    pool = G.host_pool(rng, 8, 2, 64, 64)
+    table = np.broadcast_to(np.arange(8), (b, 8))
+    q = torch.randn((b * new, 4, 64), device="cuda").to(G.TYPES[dt])
+    for sign in (1, -1):  # keys that are all positive make scores of one sign
+        pool["k"] = (sign * np.maximum(np.abs(pool["k"]), 1)).astype(np.int8)
+        cache = G.device_pool(pool)
+        for p0 in (0, 300, -1, -new):
+            pos = G.i32([p0] * b)
+            ref = lb.kv8_attention(q, cache, G.i32(table), pos)
+            for bad in (float("inf"), float("-inf"), float("nan")):
+                x = q.clone()
+                x[0, 1, 5] = x[-1, 3, 63] = bad
+                for scale in (None, 0.0):
+                    out = lb.kv8_attention(x, cache, G.i32(table), pos, scale=scale)
+                    base = ref if scale is None else lb.kv8_attention(q, cache, G.i32(table), pos, scale=scale)
+                    hit = torch.zeros((b * new, 4), dtype=torch.bool, device="cuda")
+                    hit[0, 1] = hit[-1, 3] = True
+                    sees = torch.from_numpy((p0 + np.arange(new) >= 0)[None].repeat(b, 0).reshape(-1)).cuda()
+                    nan = hit & sees[:, None]
+                    assert torch.isnan(out[nan]).all() and not out[~sees].any()
+                    # (a row's references follow votes of rows beside it: other roundings, the same value)
+                    torch.testing.assert_close(out[~nan].float(), base[~nan].float(), rtol=2 * G.R_OUT[dt] + 2.0 ** -10, atol=2.0 ** -10)

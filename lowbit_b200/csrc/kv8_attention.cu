@@ -738,7 +738,7 @@ int row_tiles(long long rows, int dtype, int D, int &nq) {
 constexpr int THIN = 6;
 Plan plan_of(const Pool &c, int dtype, int width, int B, int most, int H, int window, int sms) {
   Plan p{};
-  const long long rows = (long long)most * (H / c.KV);
+  const long long rows = (long long)std::max(most, 1) * (H / c.KV);  // (max_tokens 0: one CTA a sequence records the rows left out)
   p.tiles = row_tiles(rows, dtype, c.D, p.nq);
   const long long items = (long long)B * c.KV * p.tiles;
   const int high = prompt_rows(dtype, c.D);
@@ -810,7 +810,7 @@ int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, 
   if (H <= 0 || H % a.c.KV || H > 65535 || (long long)max_tokens * H > 0x7fffffff)
     return refuse("kv8_attention: H must be a multiple of the KV heads");
   if ((long long)max_tokens * (H / a.c.KV) > 128LL * 65535) return refuse("kv8_attention: too many rows a sequence");
-  if (N == 0 || max_tokens == 0) return 0;
+  if (N == 0) return 0;
   if (!q || !out) return refuse("kv8_attention: NULL argument");
   if (ld < (long long)H * a.c.D || ld * (dtype == LBC_F32 ? 4 : 2) % 16) return refuse("kv8_attention: bad row stride");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)

@@ -581,7 +581,7 @@ void launch(const AttnArgs &a, cudaStream_t st) {
   static_assert(smem <= 227 * 1024, "operand tiles fit an SM's shared memory");
   static std::atomic<uint64_t> allowed{0};
   allow_smem(prompt_kernel<T, D>, smem, allowed);
-  const unsigned tiles = (unsigned)(((long long)a.r.most * a.G + Lay<T, D>::ROWS - 1) / Lay<T, D>::ROWS);
+  const unsigned tiles = (unsigned)(((long long)std::max(a.r.most, 1) * a.G + Lay<T, D>::ROWS - 1) / Lay<T, D>::ROWS);
   launch_chained(prompt_kernel<T, D>, dim3(a.c.KV, a.r.B, tiles), THREADS, smem, 1, st, a);
 }
 template <typename T>

@@ -248,3 +248,30 @@ def test_infinite_queries(dt, new, b):
                     assert torch.isnan(out[nan]).all() and not out[~sees].any()
                     # (a row's references follow votes of rows beside it: other roundings, the same value)
                     torch.testing.assert_close(out[~nan].float(), base[~nan].float(), rtol=2 * G.R_OUT[dt] + 2.0 ** -10, atol=2.0 ** -10)
+
+
+@pytest.mark.parametrize("heads", [4, 128])
+@pytest.mark.parametrize("b", [2, 40])
+def test_rows_left_out_by_max_tokens_are_recorded(heads, b):
+    """max_tokens below the rows of a sequence, 0 included: the rows left out are not written, and recorded."""
+    rng = np.random.default_rng(47)
+    pool = G.host_pool(rng, 8, 2, 64, 64)
+    table, pos = G.i32(np.broadcast_to(np.arange(8), (b, 8))), G.i32([100] * b)
+    q = torch.randn((2 * b, heads, 64), device="cuda")
+    cos, sin = (torch.from_numpy(t).cuda() for t in G.rope_tables(64, 512, 1e4))
+    qkv = torch.randn((2 * b, (heads + 4) * 64), device="cuda")
+    starts, none = G.i32(np.arange(b + 1) * 2), G.i32([0] * (b + 1))
+    for most in (0, 1):
+        cache = G.device_pool(pool)
+        out = lb.kv8_attention(q, cache, table, pos, starts=starts, max_tokens=most, out=torch.full_like(q, 7.0))
+        assert K.device_status(reset=True) == G.ERR_PAGE
+        left = out.view(b, 2, heads, 64)[:, most:]
+        assert (left == 7).all() and torch.isfinite(out).all()
+        lb.kv8_append(qkv, cache, table, pos, cos, sin, starts=starts, max_tokens=most)
+        assert K.device_status(reset=True) == G.ERR_PAGE
+        if most == 0:
+            G.same_pool(cache, pool)
+        # no sequence has rows: nothing to leave out
+        lb.kv8_attention(q, cache, table, pos, starts=none, max_tokens=most)
+        lb.kv8_append(qkv, cache, table, pos, cos, sin, starts=none, max_tokens=most)
+        assert K.device_status(reset=True) == 0

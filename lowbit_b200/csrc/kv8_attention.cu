@@ -285,6 +285,26 @@ struct Warp {
     }
   }
 
+  // O so far to a total in global memory (this thread's, THREADS floats from element to element, M last), and begun
+  // anew; or, at a segment's end, back to registers
+  __device__ __forceinline__ void fold(float *total, bool begun, bool last) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float *at = total + (size_t)((n * 2 + i) * (2 * MT + 1)) * THREADS;
+        const float f = begun ? ex2(at[2 * MT * THREADS] - m[n][i]) : 0.f;
+        at[2 * MT * THREADS] = m[n][i];
+#pragma unroll
+        for (int c = 0; c < 2 * MT; ++c) {
+          float &x = o[n][c / 2][i + 2 * (c % 2)];
+          const float y = begun ? fmaf(at[c * THREADS], f, x) : x;
+          at[c * THREADS] = y;
+          x = last ? y : 0.f;
+        }
+      }
+  }
+
   // f grew by d <= RISE
   __device__ __forceinline__ void raise(int d) {
     const float f = ex2((float)d);
@@ -449,6 +469,9 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
     const int see1 = min((long long)s.p0 + s.n - 1, (long long)cap - 1);
     const int chunk = ((META - 1) << a.c.lg_page) / UNIT;  // units whose pages are looked up together
     const long long head = (long long)kvh * a.c.page * D;
+    // 16-bit calls: units after which O is added to its total, a whole number of chunks with FOLD / 2 tokens a warp
+    const int spell = (FOLD / 2 / WTOK + chunk - 1) / chunk * chunk;
+    auto place = [&]() { return a.total + (size_t)cta * (THREADS * NQ * (D / 4 + 2)) + tid; };
     int f = 0, f_first = 0;
     bool far = false;
     if (tid == 0) meta.f = 0;
@@ -458,6 +481,7 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
       int id = -1;
       typename W::Query query;
       if (c0 > u) __syncthreads();  // every warp is done with the entries before
+      if (sizeof(T) == 2 && a.total && c0 > u && (c0 - u) % spell == 0) w.fold(place(), c0 - u > spell, false);
       // on its way while the pages are looked up, where the registers allow it
       constexpr bool EARLY = NQ == 1 && D < 128;
       if (c0 == u && EARLY) w.load_query(query, a, s, tile, kvh, lane);
@@ -527,6 +551,7 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
       }
       copy_wait<0>();
     }
+    if (sizeof(T) == 2 && a.total && !far && u1 - u > spell) w.fold(place(), true, true);
     if (u == u1) {  // no units: nothing to add, or an item of zeros
       typename W::Query none = {};
       w.start(none, a, s, tile, lane);
@@ -713,7 +738,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
 
 struct Plan {
   int prompt, nq, tiles, split, cluster, grid;
-  size_t desc, bytes;
+  size_t desc, total, bytes;  // total: where the workspace's `total` begins, 0 without
 };
 
 // rows of a tile: 8 or 16; 24 where that saves a tile and the registers suffice
@@ -744,9 +769,12 @@ Plan plan_of(const Pool &c, int dtype, int width, int B, int most, int H, int wi
   const int high = prompt_rows(dtype, c.D);
   const long long waves = ((long long)B * c.KV * ((rows + high - 1) / high) + sms - 1) / sms;
   p.prompt = rows > 24 && waves * 2 * sms <= items;
-  if (p.prompt) return p;
   long long len = (long long)width << c.lg_page;
   if (window > 0) len = std::min(len, (long long)window + most + UNIT);
+  if (p.prompt) {
+    p.bytes = fold_sums(dtype, len) ? (size_t)(B * (long long)c.KV * ((rows + high - 1) / high)) * high * total_row(c.D) * sizeof(float) : 0;
+    return p;
+  }
   const long long units = (len + UNIT - 1) / UNIT;
   const long long wave = (long long)resident(dtype, c.D, p.nq) * sms;
   p.cluster = 1;
@@ -755,6 +783,10 @@ Plan plan_of(const Pool &c, int dtype, int width, int B, int most, int H, int wi
   p.grid = (int)std::min<long long>(p.split ? std::min(wave, std::max<long long>(items * units / THIN, sms)) : items * p.cluster, 0x7fffffff);
   p.desc = p.split ? ((size_t)items * sizeof(int2) + 255) / 256 * 256 : 0;
   p.bytes = p.split ? p.desc + (size_t)p.grid * 2 * 8 * p.nq * (c.D + 3) * sizeof(float) : 0;
+  if (p.split && fold_sums(dtype, len / 2)) {
+    p.total = (p.bytes + 255) / 256 * 256;
+    p.bytes = p.total + (size_t)p.grid * THREADS * p.nq * (c.D / 4 + 2) * sizeof(float);
+  }
   return p;
 }
 
@@ -823,6 +855,9 @@ int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, 
   a.tiles = p.tiles;
   a.split = p.split;
   a.desc = static_cast<int2 *>(workspace);
+  a.total = p.prompt && p.bytes ? static_cast<float *>(workspace)
+            : p.total           ? reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + p.total)
+                                : nullptr;
   a.part = p.split ? reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + p.desc) : nullptr;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p.prompt) launch_prompt(a, dtype, st);

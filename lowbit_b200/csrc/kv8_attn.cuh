@@ -37,7 +37,19 @@ struct AttnArgs {
   int split;         // 0: a cluster an item
   int2 *desc;        // [B][tiles][KV] first and last CTA of an item
   float *part;       // [grid][2] records: O [8 NQ][D], then M, l, f [8 NQ] each
+  float *total;      // 16-bit calls over many tokens: a place for each thread's O so far (fold_sums); else null
 };
+
+// Tensor cores add to a running sum with truncation, so O drifts towards 0 with the
+// number of tokens. fp32 calls add each step's O to a sum rounded to nearest. 16-bit
+// outputs show it later: by 6.6e-9 a token in the prompt kernel with fp16's two weight
+// pieces (8.7e-4 at 131072 tokens, the output's own rounding 2.2e-4), 4.6e-9 with
+// bf16's one (6.0e-4, 1.0e-3); 2e-9 in the few-row kernel, whose four warps share
+// the tokens. Where a row can see more than FOLD tokens (fp16: an eighth of the
+// output's half ulp), or 16 times as many (bf16: a sixth), O is added to a total in
+// the workspace each FOLD tokens and begun anew (131072 tokens then: 6e-5).
+constexpr int FOLD = 8192;
+inline bool fold_sums(int dtype, long long tokens) { return dtype != LBC_F32 && tokens > (dtype == LBC_F16 ? FOLD : 16 * FOLD); }
 
 // sequence b: its rows, first position, units of UNIT tokens from the u0-th on,
 // tiles of ROWS rows
@@ -139,6 +151,8 @@ __device__ __forceinline__ float whole_pow2(float x) { return x == -127.f ? pow2
 
 // prompt chunks (kv8_prompt.cu), and the rows that one of its CTAs takes
 int prompt_rows(int dtype, int D);
+// floats of `total` a CTA of the prompt kernel needs: a row's O and its M
+constexpr int total_row(int D) { return D + 4; }
 void launch_prompt(const AttnArgs &a, int dtype, cudaStream_t st);
 
 }  // namespace kv8

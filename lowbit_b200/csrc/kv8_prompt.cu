@@ -74,7 +74,8 @@ struct Lay {
   // tokens shows in fp32 outputs: fp32 calls begin O anew in each step and add it
   // to a total (rounded to nearest, also in tensor memory; adding every fourth
   // step only drifts by 1.1e-6 and is no faster, 109 to 106 us); at D = 128 the
-  // total leaves room for one row tile. 16-bit outputs do not show it.
+  // total leaves room for one row tile. 16-bit outputs need it seldom, in the
+  // workspace (kv8_attn.cuh: fold_sums).
   static constexpr bool FOLD = sizeof(T) == 4;
   static constexpr int RT = FOLD && D == 128 ? 1 : 2, ROWS = RT * TILE;
   static constexpr int QP = QUERY_PIECES<T>, WP = WEIGHT_PIECES<T>;
@@ -95,6 +96,28 @@ __device__ __forceinline__ void reg_inc() {
 template <int N>
 __device__ __forceinline__ void reg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// adds a row's O (16 elements from c on: get) to its total, D floats and the M that they stand at, brought to M = m
+template <int D, typename Get>
+__device__ __forceinline__ void add_total(float *total, bool begun, float m, const Get &get) {
+  const float f = begun ? ex2(total[D] - m) : 0.f;
+  total[D] = m;
+#pragma unroll
+  for (int c = 0; c < D; c += 16) {
+    uint32_t o[16];
+    get(c, o);
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) {
+      float4 *t = reinterpret_cast<float4 *>(total + c + k);
+      float4 y = make_float4(u2f(o[k]), u2f(o[k + 1]), u2f(o[k + 2]), u2f(o[k + 3]));
+      if (begun) {
+        const float4 x = *t;
+        y = make_float4(fmaf(x.x, f, y.x), fmaf(x.y, f, y.y), fmaf(x.z, f, y.z), fmaf(x.w, f, y.w));
+      }
+      *t = y;
+    }
+  }
 }
 
 template <typename T, int D>
@@ -155,6 +178,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
     *abort = 1;
     return false;
   };
+  // 16-bit calls: O begins anew at steps j with j & anew == 0
+  const int anew = a.total ? kv8::FOLD / NT - 1 : 0x7fffffff;
   // tensor memory: S (and P in its place) of row tile i, buffer j; O of row tile i; its total
   auto s_col = [&](int i, int j) { return tmem + (2 * i + j) * NT; };
   auto o_col = [&](int i) { return tmem + 2 * L::RT * NT + i * D; };
@@ -211,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
 #pragma unroll
             for (int k = 0; k < NT / 16; ++k)
               tc::mma_bf16_ts(o_col(i), s_col(i, st) + 8 * k + NT / 2 * c, vd + (uint64_t)(2 * k * L::V_LBO) / 16,
-                              tc::idesc_f16_f32(D), k > 0 || c < L::WP - 1 || (!L::FOLD && j > 0));
+                              tc::idesc_f16_f32(D), k > 0 || c < L::WP - 1 || (!L::FOLD && (j & anew) != 0));
           tc::commit(&sh.pv_done[i][st]);
         }
         if (!ok) {
@@ -388,6 +413,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
     }
     tc::fence_proxy_async_smem();
     mbar_arrive(&sh.q_full);
+    auto total = [&]() {  // this row's place
+      return a.total + ((((size_t)blockIdx.z * gridDim.y + b) * gridDim.x + kvh) * L::ROWS + i * TILE + (tid & (TILE - 1))) * total_row(D);
+    };
     float m = LOWEST;
     uint64_t ls[2] = {0, 0};  // the sum l, in four parts
     int f = 0;
@@ -446,7 +474,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         f = meta.f;
       }
       const bool rise = __any_sync(0xffffffffu, mx - m > SLACK);
-      if (rise || (L::FOLD && j > 0)) {
+      const bool fold = !L::FOLD && j > 0 && (j & anew) == 0;
+      if (rise || fold || (L::FOLD && j > 0)) {
         float scale = 1.f;
         if (rise) {
           const float to = fmaxf(m, reference(mx, HEAD, SLACK));
@@ -459,18 +488,28 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
           ok = wait(&sh.pv_done[i][st ^ 1], ((j - 1) >> 1) & 1);
           if (!ok) break;
           tc::fence_after_sync();
+          if (!L::FOLD && fold) {
+            add_total<D>(total(), j > anew + 1, m, [&](int c, uint32_t (&o)[16]) {
+              tc::ld16(o_col(i) + quad + c, o);
+              tc::wait_ld();
+              tc::loaded16(o);
 #pragma unroll
-          for (int c = 0; c < D; c += 16) {
-            uint32_t o[16], t[16];
-            const bool both = L::FOLD && j > 1;
-            tc::ld16(o_col(i) + quad + c, o);
-            if (both) tc::ld16(t_col(i) + quad + c, t);
-            tc::wait_ld();
-            tc::loaded16(o);
-            if (both) tc::loaded16(t);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(u2f(o[k]) * scale);
+            });
+          } else {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint((both ? u2f(t[k]) + u2f(o[k]) : u2f(o[k])) * scale);
-            tc::st16((L::FOLD ? t_col(i) : o_col(i)) + quad + c, o);
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16], t[16];
+              const bool both = L::FOLD && j > 1;
+              tc::ld16(o_col(i) + quad + c, o);
+              if (both) tc::ld16(t_col(i) + quad + c, t);
+              tc::wait_ld();
+              tc::loaded16(o);
+              if (both) tc::loaded16(t);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint((both ? u2f(t[k]) + u2f(o[k]) : u2f(o[k])) * scale);
+              tc::st16((L::FOLD ? t_col(i) : o_col(i)) + quad + c, o);
+            }
           }
         }
       }
@@ -530,6 +569,11 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
 #pragma unroll
         for (int k = 0; k < 16; ++k)
           if (both) o[k] = __float_as_uint(u2f(o[k]) + u2f(t[k]));
+        if (!L::FOLD && steps > anew + 1LL) {
+          const float *sum = total(), f = ex2(sum[D] - m);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(fmaf(sum[c + k], f, u2f(o[k])));
+        }
       }
 #pragma unroll
       for (int k = 0; k < 16; k += E) {

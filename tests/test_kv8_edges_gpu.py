@@ -275,3 +275,39 @@ def test_rows_left_out_by_max_tokens_are_recorded(heads, b):
         lb.kv8_attention(q, cache, table, pos, starts=none, max_tokens=most)
         lb.kv8_append(qkv, cache, table, pos, cos, sin, starts=none, max_tokens=most)
         assert K.device_status(reset=True) == 0
+
+
+# A quarter of half an ulp: what the sums may drift by before a total is kept, and with one
+DRIFT = {"fp16": 2.0 ** -13, "bf16": 2.0 ** -10}
+
+
+@pytest.mark.parametrize("dt,new,b,kv,g,d,page,length", [
+    ("fp16", 100, 12, 2, 4, 128, 64, 8192), ("fp16", 100, 12, 2, 4, 128, 64, 131072), ("fp16", 90, 12, 4, 2, 64, 32, 70001),
+    ("fp16", 100, 12, 4, 2, 32, 128, 131072), ("bf16", 100, 12, 2, 4, 128, 64, 131072), ("bf16", 100, 12, 1, 4, 128, 64, 1 << 20),
+    ("fp16", 1, 148, 4, 2, 64, 64, 16384), ("fp16", 1, 64, 4, 2, 64, 64, 131072), ("fp16", 3, 64, 4, 4, 128, 16, 131071),
+    ("fp16", 5, 64, 4, 4, 32, 128, 131072), ("bf16", 1, 32, 2, 8, 128, 64, 1 << 20), ("bf16", 2, 40, 2, 8, 64, 32, 300001)])
+def test_long_sums_of_16_bit_types_do_not_drift(dt, new, b, kv, g, d, page, length):
+    """Positive values, so that truncated sums would come out small: the mean error beyond that of the correctly
+    rounded rows stays within DRIFT, at any length."""
+    pages = -(-length // page)
+    cache = lb.KV8Cache.empty(pages, kv, d, page=page)
+    cache.k.copy_(torch.randint(-60, 61, cache.k.shape, device="cuda"))
+    cache.v.copy_(torch.randint(32, 97, cache.v.shape, device="cuda"))
+    cache.k_exp.fill_(122)
+    cache.v_exp.fill_(121)
+    table = torch.randperm(pages, device="cuda").to(torch.int32)
+    tables = table[None].repeat(b, 1)  # one prefix for all
+    q = torch.randn((b * new, kv * g, d), device="cuda").to(G.TYPES[dt])
+    out = lb.kv8_attention(q, cache, tables, G.i32([length - new] * b))
+    again = lb.kv8_attention(q, cache, tables, G.i32([length - new] * b))
+    assert torch.equal(out, again)
+    rows = torch.arange(0, b * new, max(1, b * new // 24), device="cuda")
+    at = length - new + rows % new
+    e = []
+    for h in range(kv):
+        k, v = (t[table.long(), h].reshape(-1, d)[:length].double() for t in (cache.k, cache.v))
+        x = q[rows, h * g:(h + 1) * g].double()
+        s = (x @ (k.T * 2.0 ** -5) / d ** 0.5).masked_fill((torch.arange(length, device="cuda") > at[:, None])[:, None], -torch.inf)
+        ref = s.softmax(-1) @ v * 2.0 ** -6
+        e.append(((out[rows, h * g:(h + 1) * g].double() - ref.to(G.TYPES[dt]).double()) / ref).mean().item())
+    assert abs(np.mean(e)) <= DRIFT[dt], np.mean(e)

@@ -311,3 +311,37 @@ def test_long_sums_of_16_bit_types_do_not_drift(dt, new, b, kv, g, d, page, leng
         ref = s.softmax(-1) @ v * 2.0 ** -6
         e.append(((out[rows, h * g:(h + 1) * g].double() - ref.to(G.TYPES[dt]).double()) / ref).mean().item())
     assert abs(np.mean(e)) <= DRIFT[dt], np.mean(e)
+
+
+@pytest.mark.parametrize("new,b", [(1, 40), (3, 20), (100, 12)])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_fp16_weights_keep_22_bits(new, b, d):
+    """fp16 calls hold weights in two fp16 pieces. Few tokens and small scores, so that the bound of test_kv8_gpu.check
+    is narrow enough with r_p = 2^-21 (two pieces, as its fp32) to exclude weights of one piece (11 bits), which the
+    oracle shows with such weights planted in it."""
+    rng = np.random.default_rng(48)
+    pool = G.host_pool(rng, 2 * b + 8, 2, 64, d, 0.2)
+    table = np.stack([rng.permutation(2 * b + 8)[:4] for _ in range(b)])
+    q = torch.from_numpy(rng.standard_normal((b * new, 4, d)).astype(np.float32)).to(torch.float16)
+    pos, window, scale = [70] * b, 12, 0.08 / d
+    out = lb.kv8_attention(q.cuda(), G.device_pool(pool), G.i32(table), G.i32(pos), window=window, scale=scale)
+    x = q.double().numpy()
+    ref, mag, size = R.attention(pool, x, table, pos, window=window, scale=scale)
+    tol = mag * ((2 * (d + 8) * size[..., None] + window + 16) * 2.0 ** -22 + 2.0 ** -21)
+    tol += np.maximum(G.R_OUT["fp16"] * np.abs(ref), G.TINY["fp16"])
+    assert (np.abs(out.double().cpu().numpy() - ref) <= tol).all()
+    one = np.zeros_like(ref)  # the same with weights rounded to 11 bits
+    for i in range(b * new):
+        p = 70 + i % new
+        at = np.arange(p - window + 1, p + 1)
+        ids = table[i // new, at // 64]
+        for h in range(4):
+            g = h // 2
+            k = pool["k"][ids, g, at % 64] * R.pow2(pool["k_exp"][ids, g])[:, None]
+            t = scale * (k @ x[i, h]) / np.log(2) + pool["v_exp"][ids, g] - 127.0
+            w = np.exp2(t - np.ceil(t.max()) + 14)
+            w16 = w.astype(np.float16).astype(np.float64)
+            l = (w / R.pow2(pool["v_exp"][ids, g])).sum()
+            one[i, h] = w16 @ pool["v"][ids, g, at % 64] / l
+            assert np.allclose(w @ pool["v"][ids, g, at % 64] / l, ref[i, h], rtol=1e-9, atol=1e-9)
+    assert (np.abs(one - ref) > tol).mean() > 0.01

@@ -8,22 +8,12 @@ from .formats import (GROUP, MXBLOCK, AMXInt4Weights, Int4Weights, Int8Acts, MXF
                       quantize_act_int8, quantize_int4, quantize_mxfp4)
 from .kernels import (Params, amx_available, cpu_info, gemm_mxfp4, gemm_w4a8, gemm_w4a8_amx, gemm_w4a16,
                       gpu_info, w4a8_group_acc_amx)
-
-_KVCACHE = ("KV8Cache", "PagedKVCache", "kv8_append", "kv8_attention", "kv8_read")
-
-
-def __getattr__(name):
-    # the KV-cache module works on torch tensors: torch is imported when it is first asked for
-    if name in _KVCACHE:
-        from . import kvcache
-        globals().update({n: getattr(kvcache, n) for n in _KVCACHE})
-        return globals()[name]
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
-
+from .kvcache import KV8Cache, PagedKVCache, kv8_append, kv8_attention, kv8_read
 
 __version__ = "0.1.0"
 __all__ = [
     "GROUP", "MXBLOCK", "AMXInt4Weights", "Int4Weights", "Int8Acts", "MXFP4Weights", "Params", "amx_available",
     "cpu_info", "gemm_mxfp4", "gemm_w4a8", "gemm_w4a8_amx", "gemm_w4a16", "gpu_info", "pack_amx",
-    "quantize_act_int8", "quantize_int4", "quantize_mxfp4", "w4a8_group_acc_amx", *_KVCACHE,
+    "quantize_act_int8", "quantize_int4", "quantize_mxfp4", "w4a8_group_acc_amx",
+    "KV8Cache", "PagedKVCache", "kv8_append", "kv8_attention", "kv8_read",
 ]

@@ -30,14 +30,17 @@ from __future__ import annotations
 
 import ctypes as C
 
-import torch
-
 from .kernels import lib
 
 PAGES = (16, 32, 64, 128)
 HEAD_DIMS = (32, 64, 128)
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _native = None  # csrc/kv8_torch.cpp, loaded on first use
+
+
+def _torch():
+    # imported when a cache is made or read: the package's names can be imported without torch
+    import torch
+    return torch
 
 
 def _load():
@@ -75,6 +78,7 @@ class KV8Cache:
                  "_index")
 
     def __init__(self, k, v, k_exp, v_exp):
+        torch = _torch()
         if k.dim() != 4 or v.shape != k.shape or k.dtype != torch.int8 or v.dtype != torch.int8:
             raise ValueError("k and v must be int8 [pages, kv_heads, page, head_dim]")
         pages, kv, page, d = k.shape
@@ -103,6 +107,7 @@ class KV8Cache:
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, page: int = 64, device=None) -> "KV8Cache":
         """A pool of `pages` pages, all codes and scales zero."""
+        torch = _torch()
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
         shape = (int(pages), int(kv_heads), int(page), int(head_dim))
         k, v = (torch.zeros(shape, dtype=torch.int8, device=device) for _ in range(2))
@@ -134,13 +139,15 @@ def kv8_attention(q, cache: KV8Cache, table, pos, starts=None, max_tokens: int |
     return (_native or _load()).attention(cache._at, cache._index, q, table, pos, starts, max_tokens, window, scale, out)
 
 
-def kv8_read(cache: KV8Cache, pages, dtype=torch.bfloat16):
+def kv8_read(cache: KV8Cache, pages, dtype=None):
     """Keys and values of the pages ``pages`` (int32 ids on the GPU), each
     [len(pages), kv_heads, page, head_dim]: exact in bf16 and fp32; fp16 rounds
-    what lies outside its range."""
-    if dtype not in _DTYPES:
+    what lies outside its range. ``dtype`` defaults to bfloat16."""
+    torch = _torch()
+    ids = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, None: 1}
+    if dtype not in ids:
         raise ValueError("dtype must be torch.float32, bfloat16 or float16")
-    return (_native or _load()).read(cache._at, cache._index, pages, _DTYPES[dtype])
+    return (_native or _load()).read(cache._at, cache._index, pages, ids[dtype])
 
 
 class PagedKVCache:
@@ -158,6 +165,7 @@ class PagedKVCache:
     def __init__(self, cfg, max_len: int, batch: int = 1, page: int = 64, pages: int | None = None):
         if batch <= 0 or max_len <= 0:
             raise ValueError("a cache holds at least one sequence of one token")
+        torch = _torch()
         width = -(-max_len // page)
         self.batch, self.page, self._max_len, self._positions = batch, page, max_len, cfg.max_position
         n = batch * width if pages is None else int(pages)
@@ -201,6 +209,7 @@ class PagedKVCache:
             return
         for own, m in zip(self._owned, more):
             own.extend(self._free.pop() for _ in range(m))
+        torch = _torch()
         host = torch.full(self.table.shape, -1, dtype=torch.int32)
         for b, own in enumerate(self._owned):
             host[b, :len(own)] = torch.tensor(own, dtype=torch.int32)
@@ -229,6 +238,7 @@ class PagedKVCache:
         """Sets the sequences' lengths; a released place of length 0 stays padding."""
         self.lengths = [int(n) for n in lengths]
         self._released = {b for b in self._released if self.lengths[b] == 0}
+        torch = _torch()
         self.pos.copy_(torch.tensor([-1 if b in self._released else n for b, n in enumerate(self.lengths)], dtype=torch.int32))
 
     def reset(self) -> None:

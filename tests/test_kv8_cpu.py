@@ -85,3 +85,13 @@ def test_oracle_append_in_pieces_grows_only_the_step(cut):
     for n in ("k", "v"):
         np.testing.assert_array_equal(one[n + "_exp"], two[n + "_exp"])
         assert np.abs(one[n].astype(int) - two[n]).max() <= 1
+
+
+def test_names_import_without_torch():
+    """The package, all its exported names included, does not need torch before it is used."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = "import sys; sys.modules['torch'] = None\nfrom lowbit_b200 import *\nassert callable(kv8_append) and callable(KV8Cache)"
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).parents[1], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr

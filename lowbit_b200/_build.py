@@ -8,8 +8,9 @@ torch side of the KV-cache calls (csrc/kv8_torch.cpp, a CPython module on
 torch's C++ headers) the same way.
 
 Environment:
-  NVCC               nvcc binary (default: $CUDA_HOME/bin/nvcc or nvcc on PATH)
-  LOWBIT_B200_LIB    path to a prebuilt liblowbit_b200.so (skips the build)
+  NVCC                    nvcc binary (default: $CUDA_HOME/bin/nvcc or nvcc on PATH)
+  LOWBIT_B200_LIB         path to a prebuilt liblowbit_b200.so (skips the build)
+  LOWBIT_B200_TORCH_LIB   path to a prebuilt _kv8_torch.so (skips its build)
 """
 from __future__ import annotations
 
@@ -101,8 +102,23 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     return LIB
 
 
+def cuda_include() -> Path:
+    """Directory of the CUDA runtime headers; needs no compiler."""
+    dirs = [Path(os.environ.get("CUDA_HOME", "/usr/local/cuda")) / "include"]
+    dirs += [Path(p) / "nvidia" / "cuda_runtime" / "include" for p in sys.path]
+    for d in dirs:
+        if (d / "cuda_runtime_api.h").exists():
+            return d
+    try:
+        return Path(nvcc()).resolve().parents[1] / "include"
+    except RuntimeError:
+        raise RuntimeError("CUDA headers not found; set CUDA_HOME, or LOWBIT_B200_TORCH_LIB to a prebuilt module") from None
+
+
 def build_torch(force: bool = False) -> Path:
     """Compile (if needed) and return the path of the _kv8_torch module."""
+    if os.environ.get("LOWBIT_B200_TORCH_LIB"):
+        return Path(os.environ["LOWBIT_B200_TORCH_LIB"])
     import sysconfig
 
     import torch
@@ -114,13 +130,13 @@ def build_torch(force: bool = False) -> Path:
     if not force and TORCH_LIB.exists() and TORCH_STAMP.exists() and TORCH_STAMP.read_text().strip() == digest:
         return TORCH_LIB
     root = Path(torch.__file__).parent
-    cuda = Path(nvcc()).resolve().parents[1]
-    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda_include(),
            sysconfig.get_paths()["include"]]
     TORCH_STAMP.parent.mkdir(exist_ok=True)
     tmp = TORCH_LIB.with_suffix(f".so.tmp{os.getpid()}")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in inc), str(TORCH_SRC),
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(a for p in inc for a in ("-isystem", str(p))),
+           str(TORCH_SRC),
            "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
            "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -132,5 +148,7 @@ def build_torch(force: bool = False) -> Path:
 
 
 if __name__ == "__main__":
+    from importlib.util import find_spec
     print(build(verbose=True, force="--force" in sys.argv))
-    print(build_torch(force="--force" in sys.argv))
+    if find_spec("torch"):  # only the KV-cache calls need it
+        build_torch(force="--force" in sys.argv)

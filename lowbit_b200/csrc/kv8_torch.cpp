@@ -6,8 +6,8 @@
 // The library's entry points are handed over as addresses (init), so that the
 // module uses the one copy of the library that the process has loaded.
 #include <ATen/ATen.h>
-#include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/lowbit_b200.h"
@@ -87,7 +87,7 @@ const lbc_kv8 *pool(PyObject *o) { return static_cast<const lbc_kv8 *>(PyLong_As
 
 c10::Device device(PyObject *o) { return c10::Device(c10::kCUDA, (c10::DeviceIndex)as_long(o)); }
 
-void *stream(const c10::Device &d) { return at::cuda::getCurrentCUDAStream(d.index()).stream(); }
+void *stream(const c10::Device &d) { return c10::cuda::getCurrentCUDAStream(d.index()).stream(); }
 
 PyObject *status_error(int rc, const char *what) {
   PyErr_Format(rc == LBC_ERR_SHAPE || rc == LBC_ERR_PARAMS ? PyExc_ValueError : PyExc_RuntimeError, "%s failed (rc=%d): %s", what, rc,

@@ -95,3 +95,41 @@ def test_names_import_without_torch():
     code = "import sys; sys.modules['torch'] = None\nfrom lowbit_b200 import *\nassert callable(kv8_append) and callable(KV8Cache)"
     r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).parents[1], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_torch_module_builds_without_nvcc(monkeypatch, tmp_path):
+    """With a prebuilt library and no nvcc the torch side still builds (it needs CUDA's headers only), or is prebuilt too."""
+    from lowbit_b200 import _build
+    cxx = tmp_path / "cxx"
+    cxx.write_text('#!/bin/sh\necho "$@" > "$0.args"\nwhile [ "$1" != -o ]; do shift; done\ntouch "$2"\n')
+    cxx.chmod(0o755)
+
+    def none():
+        raise RuntimeError("nvcc not found; set NVCC or CUDA_HOME")
+    monkeypatch.setattr(_build, "nvcc", none)
+    monkeypatch.setattr(_build, "TORCH_LIB", tmp_path / "_kv8_torch.so")
+    monkeypatch.setattr(_build, "TORCH_STAMP", tmp_path / "stamp")
+    monkeypatch.setenv("LOWBIT_B200_LIB", str(tmp_path / "lib.so"))
+    monkeypatch.setenv("CXX", str(cxx))
+    assert _build.build() == tmp_path / "lib.so"
+    assert _build.build_torch() == tmp_path / "_kv8_torch.so" and (tmp_path / "_kv8_torch.so").exists()
+    assert str(_build.cuda_include()) in (tmp_path / "cxx.args").read_text()
+    monkeypatch.setenv("CUDA_HOME", str(tmp_path))
+    monkeypatch.setattr(_build.sys, "path", [])
+    with pytest.raises(RuntimeError, match="LOWBIT_B200_TORCH_LIB"):
+        _build.cuda_include()
+    monkeypatch.setenv("LOWBIT_B200_TORCH_LIB", str(tmp_path / "mine.so"))
+    assert _build.build_torch() == tmp_path / "mine.so"
+
+
+def test_build_command_without_torch():
+    """The build command prints the library's path alone, and does not need torch."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    from lowbit_b200 import _build
+    lib = str(_build.build())
+    code = "import runpy, sys; sys.modules['torch'] = None; runpy.run_module('lowbit_b200._build', run_name='__main__')"
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).parents[1], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.split() == [lib], r.stderr

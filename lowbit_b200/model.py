@@ -840,7 +840,7 @@ class Model:
         if cache.batch != B:
             raise ValueError(f"cache holds {cache.batch} sequences, prompts {B}")
         if not isinstance(cache, KVCache):
-            return np.asarray(self.generate_ragged(prompts, n_new, cache, timings, graph))
+            return np.asarray(self.generate_ragged(prompts, n_new, cache, timings, graph), np.int64).reshape(B, -1)
         if cache.length + T0 + max(0, n_new - 1) > cache.capacity:
             raise ValueError("KV cache too short for prompt + n_new")
         return self._generate(prompts.reshape(-1), B, T0, None, n_new, cache, timings, graph)

@@ -117,3 +117,13 @@ def test_lengths_stop_at_the_rotation_tables():
     assert c.lengths == [7, 40] and K.device_status(reset=True) == 0
     m.forward([1] * 40, m.new_cache(64, kind="kv8"))
     assert K.device_status(reset=True) == 0
+
+
+@pytest.mark.parametrize("n_new", [0, 1, 3])
+def test_generate_batch_gives_whole_numbers(n_new):
+    cfg = PM.tiny_config()
+    m = PM.Model(cfg, PM.random_weights(cfg, seed=6), backend="fp32")
+    prompts = np.arange(8).reshape(2, 4)
+    a = m.generate_batch(prompts, n_new, cache=m.new_cache(16, batch=2))
+    b = m.generate_batch(prompts, n_new, cache=m.new_cache(16, batch=2, kind="kv8"))
+    assert a.dtype == b.dtype == np.int64 and a.shape == b.shape == (2, n_new)

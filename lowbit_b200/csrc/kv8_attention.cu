@@ -761,7 +761,7 @@ int row_tiles(long long rows, int dtype, int D, int &nq) {
 //               heads 19.8 / 15.6 / 15.1 / 13.5 us; two of up to 16000, 8 KV
 //               heads 21.1 / 21.2 / 21.2 / 23.0
 constexpr int THIN = 6;
-Plan plan_of(const Pool &c, int dtype, int width, int B, int most, int H, int window, int sms) {
+Plan plan_of(const Pool &c, int dtype, int width, int B, int N, int most, int H, int window, int sms) {
   Plan p{};
   const long long rows = (long long)std::max(most, 1) * (H / c.KV);  // (max_tokens 0: one CTA a sequence records the rows left out)
   p.tiles = row_tiles(rows, dtype, c.D, p.nq);
@@ -772,7 +772,7 @@ Plan plan_of(const Pool &c, int dtype, int width, int B, int most, int H, int wi
   long long len = (long long)width << c.lg_page;
   if (window > 0) len = std::min(len, (long long)window + most + UNIT);
   if (p.prompt) {
-    p.bytes = fold_sums(dtype, len) ? (size_t)(B * (long long)c.KV * ((rows + high - 1) / high)) * high * total_row(c.D) * sizeof(float) : 0;
+    p.bytes = fold_sums(dtype, len) ? (size_t)N * H * total_row(c.D) * sizeof(float) : 0;
     return p;
   }
   const long long units = (len + UNIT - 1) / UNIT;
@@ -825,9 +825,9 @@ size_t lbc_kv8_attention_workspace(const lbc_kv8 *c, int dtype, int table_width,
                                    int window) {
   Pool p;
   int *status = nullptr, sms = 0;
-  if (check_pool(c, p) || device_ready(&status, &sms) || table_width <= 0 || B <= 0 || H <= 0 || H % p.KV || max_tokens < 0)
+  if (check_pool(c, p) || device_ready(&status, &sms) || table_width <= 0 || B <= 0 || H <= 0 || H % p.KV || max_tokens < 0 || N < 0)
     return 0;
-  return plan_of(p, dtype, table_width, B, max_tokens, H, window, sms).bytes;
+  return plan_of(p, dtype, table_width, B, N, max_tokens, H, window, sms).bytes;
 }
 
 int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, const int32_t *table, int table_width,
@@ -849,7 +849,7 @@ int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, 
     return refuse("kv8_attention: q and out must be 16-byte aligned");
   a.q = q; a.ld = ld; a.out = out; a.H = H; a.G = H / a.c.KV; a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const Plan p = plan_of(a.c, dtype, table_width, B, max_tokens, H, window, sms);
+  const Plan p = plan_of(a.c, dtype, table_width, B, N, max_tokens, H, window, sms);
   if (p.bytes && (!workspace || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return refuse("kv8_attention: workspace too small or not 256-byte aligned");
   a.tiles = p.tiles;

@@ -151,7 +151,7 @@ __device__ __forceinline__ float whole_pow2(float x) { return x == -127.f ? pow2
 
 // prompt chunks (kv8_prompt.cu), and the rows that one of its CTAs takes
 int prompt_rows(int dtype, int D);
-// floats of `total` a CTA of the prompt kernel needs: a row's O and its M
+// floats of `total` a row of the prompt kernel needs: its O and its M
 constexpr int total_row(int D) { return D + 4; }
 void launch_prompt(const AttnArgs &a, int dtype, cudaStream_t st);
 

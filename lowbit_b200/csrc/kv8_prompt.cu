@@ -98,15 +98,20 @@ __device__ __forceinline__ void reg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// adds a row's O (16 elements from c on: get) to its total, D floats and the M that they stand at, brought to M = m
+// adds a row's O (16 elements from c on: get, by the whole warp) to its total, D floats and the M that they stand at,
+// brought to M = m
 template <int D, typename Get>
-__device__ __forceinline__ void add_total(float *total, bool begun, float m, const Get &get) {
-  const float f = begun ? ex2(total[D] - m) : 0.f;
-  total[D] = m;
+__device__ __forceinline__ void add_total(float *total, bool there, bool begun, float m, const Get &get) {
+  float f = 0.f;
+  if (there) {
+    if (begun) f = ex2(total[D] - m);
+    total[D] = m;
+  }
 #pragma unroll
   for (int c = 0; c < D; c += 16) {
     uint32_t o[16];
     get(c, o);
+    if (!there) continue;
 #pragma unroll
     for (int k = 0; k < 16; k += 4) {
       float4 *t = reinterpret_cast<float4 *>(total + c + k);
@@ -120,7 +125,9 @@ __device__ __forceinline__ void add_total(float *total, bool begun, float m, con
   }
 }
 
-template <typename T, int D>
+// TOTAL: a 16-bit call that can see so many tokens that O is kept in a total (kv8_attn.cuh: fold_sums); an instance of its
+// own, because the test for it in the other's loop costs 1 to 7 % (215 to 217-231 us)
+template <typename T, int D, bool TOTAL>
 __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
   using L = Lay<T, D>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -178,8 +185,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
     *abort = 1;
     return false;
   };
-  // 16-bit calls: O begins anew at steps j with j & anew == 0
-  const int anew = a.total ? kv8::FOLD / NT - 1 : 0x7fffffff;
+  constexpr int anew = TOTAL ? kv8::FOLD / NT - 1 : 0x7fffffff;  // O begins anew at steps j with j & anew == 0
   // tensor memory: S (and P in its place) of row tile i, buffer j; O of row tile i; its total
   auto s_col = [&](int i, int j) { return tmem + (2 * i + j) * NT; };
   auto o_col = [&](int i) { return tmem + 2 * L::RT * NT + i * D; };
@@ -413,8 +419,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
     }
     tc::fence_proxy_async_smem();
     mbar_arrive(&sh.q_full);
-    auto total = [&]() {  // this row's place
-      return a.total + ((((size_t)blockIdx.z * gridDim.y + b) * gridDim.x + kvh) * L::ROWS + i * TILE + (tid & (TILE - 1))) * total_row(D);
+    auto total = [&]() {  // this row's place (a row that fills up the tile has none)
+      return a.total + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * total_row(D);
     };
     float m = LOWEST;
     uint64_t ls[2] = {0, 0};  // the sum l, in four parts
@@ -474,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         f = meta.f;
       }
       const bool rise = __any_sync(0xffffffffu, mx - m > SLACK);
-      const bool fold = !L::FOLD && j > 0 && (j & anew) == 0;
+      const bool fold = TOTAL && j > 0 && (j & anew) == 0;
       if (rise || fold || (L::FOLD && j > 0)) {
         float scale = 1.f;
         if (rise) {
@@ -488,8 +494,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
           ok = wait(&sh.pv_done[i][st ^ 1], ((j - 1) >> 1) & 1);
           if (!ok) break;
           tc::fence_after_sync();
-          if (!L::FOLD && fold) {
-            add_total<D>(total(), j > anew + 1, m, [&](int c, uint32_t (&o)[16]) {
+          if (TOTAL && fold) {
+            add_total<D>(total(), rho < s.n * a.G, j > anew + 1LL, m, [&](int c, uint32_t (&o)[16]) {
               tc::ld16(o_col(i) + quad + c, o);
               tc::wait_ld();
               tc::loaded16(o);
@@ -569,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
 #pragma unroll
         for (int k = 0; k < 16; ++k)
           if (both) o[k] = __float_as_uint(u2f(o[k]) + u2f(t[k]));
-        if (!L::FOLD && steps > anew + 1LL) {
+        if (TOTAL && steps > anew + 1LL && rho < s.n * a.G) {
           const float *sum = total(), f = ex2(sum[D] - m);
 #pragma unroll
           for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(fmaf(sum[c + k], f, u2f(o[k])));
@@ -619,14 +625,21 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool TOTAL>
 void launch(const AttnArgs &a, cudaStream_t st) {
   constexpr int smem = Lay<T, D>::SMEM;
   static_assert(smem <= 227 * 1024, "operand tiles fit an SM's shared memory");
   static std::atomic<uint64_t> allowed{0};
-  allow_smem(prompt_kernel<T, D>, smem, allowed);
+  allow_smem(prompt_kernel<T, D, TOTAL>, smem, allowed);
   const unsigned tiles = (unsigned)(((long long)std::max(a.r.most, 1) * a.G + Lay<T, D>::ROWS - 1) / Lay<T, D>::ROWS);
-  launch_chained(prompt_kernel<T, D>, dim3(a.c.KV, a.r.B, tiles), THREADS, smem, 1, st, a);
+  launch_chained(prompt_kernel<T, D, TOTAL>, dim3(a.c.KV, a.r.B, tiles), THREADS, smem, 1, st, a);
+}
+template <typename T, int D>
+void launch(const AttnArgs &a, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (a.total) return launch<T, D, true>(a, st);
+  }
+  launch<T, D, false>(a, st);
 }
 template <typename T>
 void launch(const AttnArgs &a, cudaStream_t st) {

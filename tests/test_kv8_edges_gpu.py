@@ -345,3 +345,38 @@ def test_fp16_weights_keep_22_bits(new, b, d):
             one[i, h] = w16 @ pool["v"][ids, g, at % 64] / l
             assert np.allclose(w @ pool["v"][ids, g, at % 64] / l, ref[i, h], rtol=1e-9, atol=1e-9)
     assert (np.abs(one - ref) > tol).mean() > 0.01
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+def test_totals_of_ragged_prompts(dt):
+    """Contexts long enough for totals in the workspace, sequences of very different numbers of rows, tiles that end
+    inside: the rows of equal prompts one by one, and a workspace that goes by the rows, not by sequences times rows."""
+    kv, g, d, page, length = 2, 4, 64, 64, 10000 if dt == "fp16" else 140000
+    pages = -(-length // page)
+    cache = lb.KV8Cache.empty(pages, kv, d, page=page)
+    cache.k.copy_(torch.randint(-60, 61, cache.k.shape, device="cuda"))
+    cache.v.copy_(torch.randint(-96, 97, cache.v.shape, device="cuda"))
+    cache.k_exp.fill_(122)
+    cache.v_exp.fill_(121)
+    table = torch.randperm(pages, device="cuda").to(torch.int32)
+    new = [1, 70, 0, 200, 33, 129, 64, 300, 5, 90, 128, 150]
+    b, n = len(new), sum(new)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    pos = [length - t for t in new]
+    q = torch.randn((n, kv * g, d), device="cuda").to(G.TYPES[dt])
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.max_memory_allocated()
+    out = lb.kv8_attention(q, cache, table[None].repeat(b, 1), G.i32(pos), starts=G.i32(starts))  # max_tokens left to N
+    assert torch.cuda.max_memory_allocated() - before < 8 * n * kv * g * d * 4 + (1 << 20)
+    same = lb.kv8_attention(q, cache, table[None].repeat(b, 1), G.i32(pos), starts=G.i32(starts), max_tokens=300)
+    assert torch.equal(out, same)
+    k, v = (t[table.long()].transpose(0, 1).reshape(kv, -1, d)[:, :length].double() * 2.0 ** e
+            for t, e in ((cache.k, -5), (cache.v, -6)))
+    at = torch.from_numpy(np.concatenate([np.arange(p, p + t) for p, t in zip(pos, new)])).cuda()
+    for i in list(range(0, n, 37)) + [n - 1]:
+        x = q[i].double().view(kv, g, d)
+        s = (torch.einsum("kgd,kld->kgl", x, k) / d ** 0.5)[..., :at[i] + 1]
+        ref = torch.einsum("kgl,kld->kgd", s.softmax(-1), v[:, :at[i] + 1]).view(kv * g, d)
+        mag = torch.einsum("kgl,kld->kgd", s.softmax(-1), v[:, :at[i] + 1].abs()).view(kv * g, d)
+        size = (torch.einsum("kgd,kld->kgl", x.abs(), k.abs()).amax(-1) / d ** 0.5).view(kv * g)
+        G.check(out[i], ref.cpu().numpy(), mag.cpu().numpy(), size.cpu().numpy(), dt, d, length)

@@ -391,7 +391,8 @@ int lbc_kv8_append(const lbc_kv8 *c, int dtype, const void *qkv, long long ld, c
  * max(0, p - window + 1) .. p (window <= 0: 0 .. p) of KV head h / (H / KV),
  * softmax of scale * q.k; q [N, H, D] of type dtype, rows ld elements apart
  * (16-byte aligned rows), out [N, H, D] in dtype; a row without keys is 0.
- * Softmax and sums in fp32. workspace: device scratch of
+ * Softmax and sums in fp32; a row that sees a NaN block, or whose query is
+ * not finite, is NaN. workspace: device scratch of
  * lbc_kv8_attention_workspace(...) bytes (0: may be NULL), 256-byte aligned,
  * used by this call only; its contents need no initialisation. */
 size_t lbc_kv8_attention_workspace(const lbc_kv8 *c, int dtype, int table_width, int B, int N,

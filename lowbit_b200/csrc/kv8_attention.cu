@@ -6,7 +6,7 @@
 // (scores) or 16 elements (outputs) by 8 query rows, so that few rows (one
 // token's G = H / KV heads) fill the tile. int8 codes are exact in fp16;
 // queries are scaled by a power of two per row into fp16's range (fp32 ones as
-// two pieces, 22 bits), weights likewise (fp32: two pieces; 16-bit types: one).
+// two pieces, 22 bits), weights likewise (fp32 and fp16: two pieces; bf16: one).
 // Contraction indices may be permuted freely, and are: a lane loads 16
 // contiguous bytes of its token's key (or of four tokens' values) as operand
 // registers. Codes reach shared memory by cp.async in whole rows (half rows
@@ -32,11 +32,11 @@
 // joins its sums through distributed shared memory: one launch, no workspace.
 //
 // Bounds: long batches HBM (bf16, 32 heads, 8 KV heads of 128: 64 sequences to
-// 8192 tokens 120 us, 5.5 TB/s; one of 131071 57 us, 4.7 TB/s, the rest is the
-// pipelines' start and the join); short ones the chain of launch, page lookup
-// and units (14 heads, 2 KV heads of 64, fp32: 510 tokens 6.1 us, 16 sequences
-// to 4096 11.2 us); tiles of 24 rows issue and tensor-core latency (16 sequences
-// of 5 tokens, 32 heads, window 1024: 23.6 us).
+// 8192 tokens 120-131 us from GPU to GPU, 5.0-5.5 TB/s; one of 131071 58 us, 4.6
+// TB/s, the rest is the pipelines' start and the join); short ones the chain of
+// launch, page lookup and units (14 heads, 2 KV heads of 64, fp32: 510 tokens 6.3
+// us, 16 sequences to 4096 11.4 us); tiles of 24 rows issue and tensor-core latency
+// (16 sequences of 5 tokens, 32 heads, window 1024, fp16: 24 us).
 #include <algorithm>
 #include <cstdio>
 
@@ -270,7 +270,7 @@ struct Warp {
         for (int n = 0; n < NQ; ++n) {
           if constexpr (sizeof(T) == 4) {
             // tensor cores add with truncation, which drifts over many steps: the running sum is rounded to
-            // nearest (58 sequences of 40700 tokens, error 4.0e-6 without; 16-bit outputs do not show it)
+            // nearest (58 sequences of 40700 tokens, error 4.0e-6 without; 16-bit calls: fold_sums)
             float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int r = 0; r < WP; ++r) mma16816(y, op, b[n][r][0], b[n][r][1]);
@@ -383,7 +383,7 @@ template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_kernel(AttnArgs a) {
   constexpr int R = 8 * NQ, PAD = D + 4;
   __shared__ Meta meta;
-  __shared__ long long total_s, scan[WARPS];
+  __shared__ long long scan[WARPS];
   __shared__ int found;
   __shared__ long long found_at;
   __shared__ Seq found_seq;
@@ -749,9 +749,12 @@ int row_tiles(long long rows, int dtype, int D, int &nq) {
 }
 
 // Which kernel, and how its work is cut.
-//   prompt      Measured at D = 128: the prompt kernel takes 1.35 us a wave of
-//               its CTAs and 64 tokens, this one 1.3 us for 2 SMs' worth of
-//               units; so it takes over when its waves are the fewer.
+//   prompt      Measured in bf16 at D = 128: the prompt kernel takes 1.35 us a
+//               wave of its CTAs and 64 tokens, this one 1.3 us for 2 SMs' worth of
+//               units; so it takes over when its waves are the fewer. Other types
+//               and sizes go by the same rule, unmeasured; it leaves out that a tile
+//               here goes through all that its sequence sees, the causal or windowed
+//               part of its own rows or not.
 //   cluster     a CTA goes through at most 16 units (1024 tokens), and a wave
 //               holds the clusters of every item where there is more than one CTA
 //   split       otherwise; more CTAs than SMs only where each gets THIN units of

@@ -414,7 +414,7 @@ void launch_read(const Pool &c, const int32_t *ids, int n, void *k_out, void *v_
 
 template <typename T>
 void launch_append(const AppendArgs &a, long long kv_ctas, cudaStream_t st) {
-  // 16 threads a token and more: up to 4 tokens need no more than 64
+  // 2 to 16 threads a token: up to 4 tokens need no more than 64
   const unsigned threads = a.r.most <= 4 ? 64 : APPEND, ctas = (unsigned)(kv_ctas + (a.r.N + threads / 32 - 1) / (threads / 32));
   if (a.c.D == 32) launch_chained(append_kernel<T, 32>, dim3(ctas), threads, 0, 1, st, a);
   else if (a.c.D == 64) launch_chained(append_kernel<T, 64>, dim3(ctas), threads, 0, 1, st, a);

@@ -21,8 +21,8 @@
 // Bound: the row warps' own chain of a step (tensor-memory load, scale, maximum,
 // vote, exponentials, store): 2500-2600 cycles, of which the tensor pipe works
 // 1288 and the exponential unit 1024. Two prompts to 4096 tokens, 32 heads, 8 KV
-// heads of 128, bf16: 211 us, 699 TFLOP/s; 2048 fp32 tokens after 2047, 14 heads
-// of 64: 106 us. 64 tokens a step and not 128, so that two steps' scores fit
+// heads of 128, bf16: 216-218 us, 680 TFLOP/s; 2048 fp32 tokens after 2047, 14 heads
+// of 64: 104-105 us. 64 tokens a step and not 128, so that two steps' scores fit
 // tensor memory beside two row tiles' outputs (128 with one: 293 us); two row
 // tiles share each conversion of the codes.
 #include <algorithm>
@@ -126,7 +126,7 @@ __device__ __forceinline__ void add_total(float *total, bool there, bool begun, 
 }
 
 // TOTAL: a 16-bit call that can see so many tokens that O is kept in a total (kv8_attn.cuh: fold_sums); an instance of its
-// own, because the test for it in the other's loop costs 1 to 7 % (215 to 217-231 us)
+// own, because the test for it in the other's loop costs 1 to 7 % (prompts to 4096 tokens: 215 us, 217 to 231 with it)
 template <typename T, int D, bool TOTAL>
 __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
   using L = Lay<T, D>;
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
           for (int c = L::WP - 1; c >= 0; --c)  // small pieces first: the sum they are cut to is small
 #pragma unroll
             for (int k = 0; k < NT / 16; ++k)
-              tc::mma_bf16_ts(o_col(i), s_col(i, st) + 8 * k + NT / 2 * c, vd + (uint64_t)(2 * k * L::V_LBO) / 16,
+              tc::mma_f16_ts(o_col(i), s_col(i, st) + 8 * k + NT / 2 * c, vd + (uint64_t)(2 * k * L::V_LBO) / 16,
                               tc::idesc_f16_f32(D), k > 0 || c < L::WP - 1 || (!L::FOLD && (j & anew) != 0));
           tc::commit(&sh.pv_done[i][st]);
         }

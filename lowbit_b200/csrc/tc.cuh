@@ -123,8 +123,8 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(int n) {
 }
 
 // ------------------------------------------------------------ MMA
-// D[tmem] (+)= A[tmem] . B[smem]^T, issued by one thread.
-__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+// D[tmem] (+)= A[tmem] . B[smem]^T, issued by one thread. kind::f16: A and B both bf16 or both fp16, as idesc says.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
                                             uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"

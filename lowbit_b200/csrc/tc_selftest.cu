@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(128, 1) tc_selftest_kernel(int kind, int32_t *
     for (int s = 0; s < 2; ++s) {
       const uint64_t bd = tc::smem_desc(smem_u32(bsm) + 256 * s, 128, kind == 0 ? (K / 8) * 128 : (K / 16) * 128);
       if (kind == 0)
-        tc::mma_bf16_ts(tbase + d_col, tbase + 8 * s, bd, tc::idesc_bf16_f32(16), s > 0);
+        tc::mma_f16_ts(tbase + d_col, tbase + 8 * s, bd, tc::idesc_bf16_f32(16), s > 0);
       else
         tc::mma_s8_ts(tbase + d_col, tbase + 8 * s, bd, tc::idesc_s8_s32(16), s > 0);
     }

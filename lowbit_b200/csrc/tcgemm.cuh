@@ -389,7 +389,7 @@ __global__ void __maxnreg__(80) tcgemm_kernel(const __grid_constant__ CUtensorMa
           if (I8)
             tc::mma_s8_ts(dcol, acol0 + 8 * j, bd0 + 16u * j, idesc, j > 0);
           else
-            tc::mma_bf16_ts(dcol, acol0 + 8 * j, bd0 + 16u * j, idesc, j > 0);
+            tc::mma_f16_ts(dcol, acol0 + 8 * j, bd0 + 16u * j, idesc, j > 0);
         }
         tc::commit(&d_full[d]);
         tc::commit(&a_empty[ab]);

@@ -318,8 +318,8 @@ struct Warp {
 // joins the sums of a cluster's CTAs (each the four warps' O in `so`, M and l in
 // sm and sl) and writes the item's rows; the formula is join_kernel's
 template <typename T, int D, int NQ>
-__device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, int tile, int kvh, int b, int f, float *so,
-                                             float (*sm)[8 * NQ], float (*sl)[8 * NQ]) {
+__device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, int tile, int kvh, float *so, float (*sm)[8 * NQ],
+                                             float (*sl)[8 * NQ], const float *sf) {
   constexpr int R = 8 * NQ, PAD = D + 4;
   __shared__ float mine[3][R];  // M, f, l
   const int tid = threadIdx.x, size = gridDim.x, rank = blockIdx.x;
@@ -336,7 +336,7 @@ __device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, in
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) l = fmaf(sl[i][tid], ex2(sm[i][tid] - m), l);
     mine[0][tid] = m;
-    mine[1][tid] = (float)(f - 127);
+    mine[1][tid] = sf[tid];
     mine[2][tid] = l;
   }
   cluster_sync();
@@ -371,9 +371,9 @@ __device__ __forceinline__ void join_cluster(const AttnArgs &a, const Seq &s, in
         y[3] = fmaf(u2f(v[c].w), w, y[3]);
       }
     }
-    const float w = l == 0.f ? 0.f : 1.f / l, top = mg > LOWEST ? whole_pow2(mg - ag) : 1.f;
+    const float w = l == 0.f ? 0.f : 1.f / l, top = mg > LOWEST ? mg - ag : 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = y[i] * w * top;
+    for (int i = 0; i < 4; ++i) y[i] = times_pow2(y[i] * w, top);
     store4<T>(static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D + d, y);
   }
   cluster_sync();  // this CTA's sums are read until here
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
   __shared__ int found;
   __shared__ long long found_at;
   __shared__ Seq found_seq;
-  __shared__ float sm[WARPS][R], sl[WARPS][R];
+  __shared__ float sm[WARPS][R], sl[WARPS][R], sf[R];  // sf: f of each row
   extern __shared__ __align__(16) uint8_t ring[];  // [WARPS][STAGES] steps; then the warps' O [WARPS][R][PAD]
   after_previous_kernel();
   if (!a.split) next_kernel_may_start();
@@ -559,22 +559,29 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
     if (far) {  // the segment anew, a row a warp; the other warps' places hold nothing
       __syncthreads();
       const int j0 = (s.u0 + u) * UNIT, j1 = (s.u0 + u1) * UNIT, lift = far_lift(a, b, kvh, j0, j1, lane);
-      f = 127 + lift;
       for (int r = warp; r < R && first_rho + r < s.n * a.G; r += WARPS) {
         const int rho = first_rho + r;
         float m, l, o[D / 32];
         far_row<T, D>(a, b, kvh, static_cast<const T *>(a.q) + (s.r0 + rho / a.G) * a.ld + (size_t)(kvh * a.G + rho % a.G) * D,
                       row_pos(a, s, rho), j0, j1, lift, lane, m, l, o);
+        // O to about 2^20 and M as much higher, which is where the other records' M stand (zeros: far below)
+        float top = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) top = fmaxf(top, fabsf(o[d]));
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+        const float at = m + (top > 0.f ? floorf(log2f(top)) - 20.f : -300.f), shift = m > LOWEST ? at - m : 0.f;  // (as it rounds)
 #pragma unroll
         for (int i = 0; i < WARPS; ++i) {
 #pragma unroll
-          for (int d = 0; d < D / 32; ++d) so[(i * R + r) * PAD + lane * (D / 32) + d] = i ? 0.f : o[d];
-          sm[i][r] = i ? LOWEST : m;
+          for (int d = 0; d < D / 32; ++d) so[(i * R + r) * PAD + lane * (D / 32) + d] = i ? 0.f : times_pow2(o[d], -shift);
+          sm[i][r] = i || m == LOWEST ? LOWEST : at;
           sl[i][r] = i ? 0.f : l;
         }
+        sf[r] = shift + (float)lift;
       }
     } else {
       // the warps' sums, brought to a common M
+      if (tid < R) sf[tid] = (float)(f - 127);
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -601,12 +608,11 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
     }
     __syncthreads();
     if (!a.split && gridDim.x > 1) {
-      join_cluster<T, D, NQ>(a, s, tile, kvh, b, f, so, sm, sl);
+      join_cluster<T, D, NQ>(a, s, tile, kvh, so, sm, sl, sf);
       return;
     }
     const bool whole = u == 0 && u1 == s.units;
     float *rec = whole ? nullptr : a.part + (cta * 2 + (u == 0 ? 1 : 0)) * (size_t)(R * (D + 3));
-    const float top = pow2_e8m0(f);
     for (int x = tid; x < R * (D / 4); x += THREADS) {
       const int r = x / (D / 4), d = x % (D / 4) * 4, rho = first_rho + r;
       if (rho >= s.n * a.G) continue;
@@ -620,14 +626,14 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
         y[i] = (so[r * PAD + d + i] + so[(R + r) * PAD + d + i]) + (so[(2 * R + r) * PAD + d + i] + so[(3 * R + r) * PAD + d + i]);
       if (whole) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = l == 0.f ? 0.f : y[i] / l * top;
+        for (int i = 0; i < 4; ++i) y[i] = l == 0.f ? 0.f : times_pow2(y[i] / l, sf[r]);
         store4<T>(static_cast<T *>(a.out) + ((size_t)(s.r0 + rho / a.G) * a.H + kvh * a.G + rho % a.G) * D + d, y);
       } else {
         *reinterpret_cast<float4 *>(rec + r * D + d) = make_float4(y[0], y[1], y[2], y[3]);
         if (d == 0) {
           rec[R * D + r] = mx;
           rec[R * (D + 1) + r] = l;
-          rec[R * (D + 2) + r] = (float)(f - 127);
+          rec[R * (D + 2) + r] = sf[r];
         }
       }
     }
@@ -731,8 +737,8 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttnArgs a) {
     y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
   }
   l = den[0] + den[1] + den[2] + den[3];
-  const float f = l == 0.f ? 0.f : 1.f / l, top = mg > LOWEST ? whole_pow2(mg - ag) : 1.f;
-  const float out[4] = {y.x * f * top, y.y * f * top, y.z * f * top, y.w * f * top};
+  const float f = l == 0.f ? 0.f : 1.f / l, top = mg > LOWEST ? mg - ag : 0.f;
+  const float out[4] = {times_pow2(y.x * f, top), times_pow2(y.y * f, top), times_pow2(y.z * f, top), times_pow2(y.w * f, top)};
   store4<T>(dst, out);
 }
 

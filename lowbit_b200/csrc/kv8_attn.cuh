@@ -148,8 +148,11 @@ __device__ __forceinline__ int far_lift(const AttnArgs &a, int b, int kvh, int j
   return __any_sync(0xffffffffu, top > 220) ? 20 : 0;
 }
 
-// 2^x of a whole number (the exponential unit would make 2^-127, of a block of exponent 0, a zero)
-__device__ __forceinline__ float whole_pow2(float x) { return x == -127.f ? pow2_e8m0(0) : ex2(x); }
+// y 2^x for a whole number x, in two steps, since 2^x alone may be too small for fp32
+__device__ __forceinline__ float times_pow2(float y, float x) {
+  const float h = truncf(0.5f * x);
+  return y * ex2(h) * ex2(x - h);
+}
 
 // prompt chunks (kv8_prompt.cu), and the rows that one of its CTAs takes
 int prompt_rows(int dtype, int D);

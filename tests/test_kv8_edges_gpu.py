@@ -1,6 +1,7 @@
 """Edges of the paged 8-bit KV cache: tiles of padding, value scales far apart,
 queries that are not finite, limits of the calls. Helpers, bounds and the
-oracle are test_kv8_gpu.py's."""
+oracle are test_kv8_gpu.py's. With two KV heads and 100 rows a sequence, 12
+sequences take the few-row kernel, 24 the prompt kernel."""
 import numpy as np
 import pytest
 import torch
@@ -31,7 +32,7 @@ def test_tiles_of_padding_are_zero(dt, d):
     pos = np.array([0, -150, 70, -1000, 33, -130, 7, -149, 100, -150, 150, -64])
     q = torch.randn((b * new, 8, d), device="cuda").to(G.TYPES[dt])
     at = (pos[:, None] + np.arange(new)).reshape(-1)
-    ref, mag, size = R.attention(pool, q.double().cpu().numpy(), table, pos)
+    ref, mag, size, _ = attention(pool, q.double().cpu().numpy(), table, pos)
     out = torch.empty_like(q)
     for _ in range(20):
         out.fill_(7.0)
@@ -40,7 +41,7 @@ def test_tiles_of_padding_are_zero(dt, d):
         G.check(out, ref, mag, size, dt, d, 300)
     assert K.device_status(reset=True) == 0
     far = np.where(pos < 0, 2000, pos)  # rows past the table, whose window is past it too
-    ref, mag, size = R.attention(pool, q.double().cpu().numpy(), table, np.where(pos < 0, -1000, pos), window=40)
+    ref, mag, size, _ = attention(pool, q.double().cpu().numpy(), table, np.where(pos < 0, -1000, pos), window=40)
     for _ in range(20):
         out.fill_(7.0)
         lb.kv8_attention(q, cache, G.i32(table), G.i32(far), window=40, out=out)
@@ -51,24 +52,48 @@ def test_tiles_of_padding_are_zero(dt, d):
 
 # ---------------------------------------------------------------- value scales far apart
 
+def attention(pool, q, table, pos, window=0, scale=None):
+    """R.attention in torch, 64 bits, for equal row counts (the same formulas, a sequence at a time), and
+    max_i p_i 2^b_i times 127 times the number of visible tokens, b the value exponents [N, H, 1]."""
+    kv, page, d = pool["k"].shape[1:]
+    n, heads = q.shape[:2]
+    new, g = n // len(pos), heads // kv
+    scale = 1.0 / d ** 0.5 if scale is None else scale
+    parts = []
+    for i, p0 in enumerate(pos):
+        at = p0 + torch.arange(new, device="cuda")
+        length = max(1, int(p0) + new)
+        ids = table[i, :-(-length // page)]
+        x = torch.from_numpy(q[i * new:(i + 1) * new]).cuda().view(new, kv, g, d)
+        k, v = (torch.from_numpy((pool[m][ids] * R.pow2(pool[m + "_exp"][ids])[..., None, None]).transpose(1, 0, 2, 3)
+                                 .reshape(kv, -1, d)[:, :length]).cuda() for m in "kv")
+        b = torch.from_numpy(R.pow2(pool["v_exp"][ids]).repeat(page, 0)[:length].T.copy()).cuda()
+        j = torch.arange(length, device="cuda")
+        seen = ((j <= at[:, None]) & ((j > at[:, None] - window) if window else True))[:, None, None]
+        none = ~seen.any(-1)
+        p = (scale * torch.einsum("tkgd,kld->tkgl", x, k)).masked_fill(~seen, -torch.inf).softmax(-1)
+        p = p.masked_fill(none[..., None], 0.0)
+        size = (scale * torch.einsum("tkgd,kld->tkgl", x.abs(), k.abs())).masked_fill(~seen, 0.0).amax(-1)
+        floor = (p * b[None, :, None]).amax(-1, keepdim=True) * 127 * seen.sum(-1, keepdim=True)
+        parts.append([y.reshape(new, heads, *y.shape[3:]).cpu().numpy() for y in (
+            torch.einsum("tkgl,kld->tkgd", p, v), torch.einsum("tkgl,kld->tkgd", p, v.abs()), size, floor)])
+    return [np.concatenate(y) for y in zip(*parts)]
+
+
+def test_the_two_oracles_agree():
+    rng = np.random.default_rng(39)
+    pool = G.host_pool(rng, 12, 2, 16, 32)
+    table, q = rng.permutation(12).reshape(3, 4), rng.standard_normal((15, 4, 32))
+    for window in (0, 7):
+        for a, b in zip(R.attention(pool, q, table, [-3, 0, 50], window=window), attention(pool, q, table, [-3, 0, 50], window)):
+            np.testing.assert_allclose(a, b, rtol=1e-12, atol=1e-15)
+
+
 def check(out, pool, q, table, pos, window, dt, d):
     """test_kv8_gpu.check with what weights held in fp16 lose at their lower end: half a subnormal step, 2^-25, where the
     row's largest p_i 2^b_i (b: the value exponent) stands for 2^13 or more: at most 2^-38 of it a code."""
-    ref, mag, size = R.attention(pool, q, table, pos, window=window)
-    kv, page = pool["k"].shape[1:3]
-    n, heads = q.shape[:2]
-    floor, new = np.zeros((n, heads, 1)), n // len(pos)
-    for i in range(n):
-        p = pos[i // new] + i % new
-        lo = max(0, p - window + 1) if window else 0
-        ids = table[i // new, :-(-(p + 1) // page)]
-        for h in range(heads):
-            g = h // (heads // kv)
-            k = (pool["k"][ids, g] * R.pow2(pool["k_exp"][ids, g])[:, None, None]).reshape(-1, d)[lo:p + 1]
-            s = k @ q[i, h] / d ** 0.5
-            w = np.exp(s - s.max())
-            floor[i, h] = (w / w.sum() * R.pow2(pool["v_exp"][ids, g]).repeat(page)[lo:p + 1]).max() * 127 * len(w)
-    u, longest = 2.0 ** -22, max(pos) + new
+    ref, mag, size, floor = attention(pool, q, table, pos, window)
+    u, longest = 2.0 ** -22, max(pos) + len(q) // len(pos)
     tol = mag * ((2 * (d + 8) * size[..., None] + longest + 16) * u + G.R_P[dt]) + floor * 2.0 ** -38
     err = np.abs(out.double().cpu().numpy() - ref)
     assert np.isfinite(err).all()
@@ -106,13 +131,14 @@ def test_rows_that_see_small_values_only(dt, gap, page, d):
     """Later, larger tokens do not change a row that does not see them: few rows, prompts, windows."""
     far_case(dt, [page - 2], 5, 0, gap, page, d)                # the first rows end inside the small block
     far_case(dt, [2 * page - 3], 6, 1, gap, page, d, window=2)  # some rows' windows hold small tokens only
-    far_case(dt, [0] * 12, 100, 0, gap, page, d, b=12)
-    far_case(dt, [3] * 12, 140, [1, 2], gap, page, d, window=9, b=12)
+    for b in (12, 24):  # the few-row kernel, the prompt kernel
+        far_case(dt, [0] * b, 100, 0, gap, page, d, b=b)
+        far_case(dt, [3] * b, 140, [1, 2], gap, page, d, window=9, b=b)
 
 
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])
 @pytest.mark.parametrize("gap", GAPS)
-@pytest.mark.parametrize("new,b", [(1, 1), (5, 3), (100, 12)])
+@pytest.mark.parametrize("new,b", [(1, 1), (5, 3), (100, 12), (100, 24)])
 def test_weight_on_small_values(dt, gap, new, b):
     """Large values are seen, but the weight lies on small ones."""
     far_case(dt, [150] * b, new, [1, 3], gap, 32, 64, steer=True, b=b)
@@ -146,7 +172,7 @@ def test_scales_that_rise_along_a_long_context(dt, new, page, step):
         G.check(out, ref.cpu().numpy(), mag.cpu().numpy(), size.cpu().numpy(), dt, d, length)
 
 
-@pytest.mark.parametrize("new,b", [(1, 1), (100, 12)])
+@pytest.mark.parametrize("new,b", [(1, 1), (100, 12), (100, 24)])
 def test_largest_and_smallest_values_together(new, b):
     """Values near the type's end beside ones 2^200 below: sums stay finite."""
     rng = np.random.default_rng(43)
@@ -158,11 +184,11 @@ def test_largest_and_smallest_values_together(new, b):
     q = rng.standard_normal((b * new, 4, 64)).astype(np.float32)
     pos = [256 - new] * b
     out = lb.kv8_attention(torch.from_numpy(q).cuda(), G.device_pool(pool), G.i32(table), G.i32(pos))
-    G.check(out, *R.attention(pool, q, table, pos), "fp32", 64, 256)
+    G.check(out, *attention(pool, q.astype(np.float64), table, pos)[:3], "fp32", 64, 256)
 
 
 @pytest.mark.parametrize("dt", G.TYPES)
-@pytest.mark.parametrize("new,b", [(3, 2), (100, 12)])
+@pytest.mark.parametrize("new,b", [(3, 2), (100, 12), (100, 24)])
 def test_far_scales_with_bad_places(dt, new, b):
     """Where the scales are far apart too: a NaN block spoils the rows that see it, a missing page is left out."""
     rng = np.random.default_rng(44)
@@ -202,7 +228,7 @@ def test_far_scales_with_bad_places(dt, new, b):
 
 
 @pytest.mark.parametrize("dt", G.TYPES)
-@pytest.mark.parametrize("new,b,length", [(1, 1, 500), (1, 1, 60000), (3, 40, 900), (100, 12, 300)])
+@pytest.mark.parametrize("new,b,length", [(1, 1, 500), (1, 1, 60000), (3, 40, 900), (100, 12, 300), (100, 24, 300)])
 def test_scores_past_2_to_24(dt, new, b, length):
     """Scores so large that whole numbers are no longer exact in fp32: a row stays between its smallest and largest
     visible value (a factor 2 of the softmax's references would leave that range)."""
@@ -221,7 +247,7 @@ def test_scores_past_2_to_24(dt, new, b, length):
 
 
 @pytest.mark.parametrize("dt", G.TYPES)
-@pytest.mark.parametrize("new,b", [(1, 1), (1, 40), (3, 2), (100, 12)])
+@pytest.mark.parametrize("new,b", [(1, 1), (1, 40), (3, 2), (100, 12), (100, 24)])
 def test_infinite_queries(dt, new, b):
     """softmax of infinite scores is NaN, whatever their signs; a row that sees nothing is 0 whatever its query;
     other rows are as without them."""
@@ -283,7 +309,7 @@ DRIFT = {"fp16": 2.0 ** -13, "bf16": 2.0 ** -10}
 
 @pytest.mark.parametrize("dt,new,b,kv,g,d,page,length", [
     ("fp16", 100, 12, 2, 4, 128, 64, 8192), ("fp16", 100, 12, 2, 4, 128, 64, 131072), ("fp16", 90, 12, 4, 2, 64, 32, 70001),
-    ("fp16", 100, 12, 4, 2, 32, 128, 131072), ("bf16", 100, 12, 2, 4, 128, 64, 131072), ("bf16", 100, 12, 1, 4, 128, 64, 1 << 20),
+    ("fp16", 100, 12, 4, 2, 32, 128, 131072), ("bf16", 100, 12, 2, 4, 128, 64, 131072), ("bf16", 100, 12, 2, 4, 128, 64, 1 << 20),
     ("fp16", 1, 148, 4, 2, 64, 64, 16384), ("fp16", 1, 64, 4, 2, 64, 64, 131072), ("fp16", 3, 64, 4, 4, 128, 16, 131071),
     ("fp16", 5, 64, 4, 4, 32, 128, 131072), ("bf16", 1, 32, 2, 8, 128, 64, 1 << 20), ("bf16", 2, 40, 2, 8, 64, 32, 300001)])
 def test_long_sums_of_16_bit_types_do_not_drift(dt, new, b, kv, g, d, page, length):
@@ -313,7 +339,7 @@ def test_long_sums_of_16_bit_types_do_not_drift(dt, new, b, kv, g, d, page, leng
     assert abs(np.mean(e)) <= DRIFT[dt], np.mean(e)
 
 
-@pytest.mark.parametrize("new,b", [(1, 40), (3, 20), (100, 12)])
+@pytest.mark.parametrize("new,b", [(1, 40), (3, 20), (100, 24)])
 @pytest.mark.parametrize("d", [32, 64, 128])
 def test_fp16_weights_keep_22_bits(new, b, d):
     """fp16 calls hold weights in two fp16 pieces. Few tokens and small scores, so that the bound of test_kv8_gpu.check
@@ -326,7 +352,7 @@ def test_fp16_weights_keep_22_bits(new, b, d):
     pos, window, scale = [70] * b, 12, 0.08 / d
     out = lb.kv8_attention(q.cuda(), G.device_pool(pool), G.i32(table), G.i32(pos), window=window, scale=scale)
     x = q.double().numpy()
-    ref, mag, size = R.attention(pool, x, table, pos, window=window, scale=scale)
+    ref, mag, size, _ = attention(pool, x, table, pos, window, scale)
     tol = mag * ((2 * (d + 8) * size[..., None] + window + 16) * 2.0 ** -22 + 2.0 ** -21)
     tol += np.maximum(G.R_OUT["fp16"] * np.abs(ref), G.TINY["fp16"])
     assert (np.abs(out.double().cpu().numpy() - ref) <= tol).all()
@@ -380,3 +406,29 @@ def test_totals_of_ragged_prompts(dt):
         mag = torch.einsum("kgl,kld->kgd", s.softmax(-1), v[:, :at[i] + 1].abs()).view(kv * g, d)
         size = (torch.einsum("kgd,kld->kgl", x.abs(), k.abs()).amax(-1) / d ** 0.5).view(kv * g)
         G.check(out[i], ref.cpu().numpy(), mag.cpu().numpy(), size.cpu().numpy(), dt, d, length)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("new,b,length", [(1, 1, 20000), (1, 9, 3000), (4, 12, 1500), (100, 12, 1500)])
+@pytest.mark.parametrize("gap", [45, 80, 120])
+def test_far_scales_in_one_part_of_a_long_row(dt, new, b, length, gap):
+    """The row is cut over the grid: parts with scales far apart, computed otherwise, join parts of large or of small
+    values only; the weight lies where the values are small, or large, or anywhere."""
+    rng = np.random.default_rng(51)
+    page, d = 64, 64
+    width = -(-length // page)
+    pool = G.host_pool(rng, b * width, 2, page, d, 0.0)
+    table = rng.permutation(b * width).reshape(b, width)
+    small = table[:, :width * 3 // 4]
+    pool["v_exp"][small] -= gap
+    for weight in (0, 1, -1):
+        part = {n: a.copy() for n, a in pool.items()}
+        q = rng.standard_normal((b * new, 4, d))
+        if weight:  # on the small values, or on the large ones
+            part["k"] = -weight * np.abs(part["k"])
+            part["k"][small] = weight * np.abs(part["k"][small])
+            q = np.abs(q)
+        q = torch.from_numpy(q.astype(np.float32)).to(G.TYPES[dt])
+        for pos in ([length - new] * b, [width * 3 // 4 * page - 2] * b):
+            out = lb.kv8_attention(q.cuda(), G.device_pool(part), G.i32(table), G.i32(pos))
+            check(out, part, q.double().numpy(), table, pos, 0, dt, d)

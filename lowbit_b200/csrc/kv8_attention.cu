@@ -305,13 +305,16 @@ struct Warp {
       }
   }
 
-  // f grew by d <= RISE
+  // f grew by d: by RISE at most, or from 0 after blocks of zeros, whose M moves so that l stays in range (O is 0)
   __device__ __forceinline__ void raise(int d) {
-    const float f = ex2((float)d);
+    const float by = (float)max(0, d - RISE), f = ex2((float)d - by);
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) l[n][i] *= f;
+      for (int i = 0; i < 2; ++i) {
+        if (m[n][i] > LOWEST) m[n][i] += by;
+        l[n][i] *= f;
+      }
   }
 };
 
@@ -515,11 +518,25 @@ __global__ void __launch_bounds__(THREADS, resident(DTYPE<T>, D, NQ)) attention_
       __syncthreads();
       const int f_old = f;
       f = meta.f;
-      if (c0 == u) f_first = f;
+      if (f_first == 0) f_first = f;
       if (tid < pages)
         meta.s[tid] = make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(ev - 127),
                                   ev == 255 ? 1.f : pow2_e8m0(min(127 + f - ev, 254)), id >= 0 ? 1.f : 0.f);
-      far = __syncthreads_or(id >= 0 && ev < f - FAR) || f > f_first + RISE;
+      far = f > f_first + RISE;
+      if (__syncthreads_or(id >= 0 && ev < f - FAR) || (c0 > u && f_old == 0 && f > 0)) {
+        // blocks of zeros are not far: these here count with f - FAR, the ones before, if f was 0, through raise
+        for (int o = c0 > u && f_old == 0 ? (s.u0 + u) * UNIT >> a.c.lg_page : o0; o < o0 + pages && !far; ++o) {
+          const int page = (o + 1) << a.c.lg_page > see0 && o << a.c.lg_page <= see1 ? page_id(a.c, a.r, b, o) : -1;
+          const int e = page < 0 ? 255 : a.c.v_exp[page * a.c.exp_stride + kvh];
+          if (e >= f - FAR) continue;
+          far = __syncthreads_or(e > 0 || has_value(a, page, kvh, tid, THREADS));
+          if (tid == 0 && o >= o0) {
+            meta.s[o - o0].y = (float)(f - FAR - 127);
+            meta.s[o - o0].z = pow2_e8m0(127 + FAR);
+          }
+        }
+        __syncthreads();
+      }
       if (far) {  // (copies on their way land before the ring's memory is used otherwise)
         copy_wait<0>();
         break;

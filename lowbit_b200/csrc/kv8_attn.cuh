@@ -14,7 +14,9 @@ constexpr float LOWEST = -3e38f;  // M before any visible token
 // l does not, is sound while the exponents looked up together lie within FAR and
 // f grows by at most RISE after that (l <= 2^(15 + FAR + RISE) a token; a lost
 // weight is below 2^-50 of l). Where they lie farther apart, the rows are computed
-// by far_row.
+// by far_row. Blocks of exponent 0 whose codes are all 0 (a cache that was not
+// filled) are left out of that: their codes do not matter, and their l counts with
+// f - FAR, or, where f was 0 so far, follows f by way of M.
 constexpr int FAR = 60, RISE = 30;
 
 // fp16 pieces of queries and of weights: fp32 needs 22 bits of both; bf16 and
@@ -146,6 +148,19 @@ __device__ __forceinline__ int far_lift(const AttnArgs &a, int b, int kvh, int j
     if (ev != 255) top = max(top, ev);
   }
   return __any_sync(0xffffffffu, top > 220) ? 20 : 0;
+}
+
+// whether a 16-byte piece of block (page id, head kvh)'s value codes is not 0: of those that this thread, one of `step`, takes
+__device__ __forceinline__ bool has_value(const AttnArgs &a, int id, int kvh, int thread, int step) {
+  const int n = a.c.page * a.c.D / 16;
+  const uint4 *p = reinterpret_cast<const uint4 *>(a.c.v + id * a.c.page_stride + (long long)kvh * a.c.page * a.c.D);
+  uint32_t any = 0;
+#pragma unroll 4
+  for (int i = thread; i < n; i += step) {
+    const uint4 v = p[i];
+    any |= v.x | v.y | v.z | v.w;
+  }
+  return any != 0;
 }
 
 // y 2^x for a whole number x, in two steps, since 2^x alone may be too small for fp32

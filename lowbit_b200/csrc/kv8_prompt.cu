@@ -296,14 +296,26 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       const bool there = (unsigned)id < (unsigned)a.c.pages;
       if (!there) set_status(a.r.status, LBC_ERR_PAGE);
       const int ek = there ? a.c.k_exp[id * a.c.exp_stride + kvh] : 0, ev = there ? a.c.v_exp[id * a.c.exp_stride + kvh] : 0;
+      const int f_old = f;
       f = max(f, __reduce_max_sync(0xffffffffu, ev == 255 ? 0 : ev));
-      if (j == 0) f_first = f;
+      if (f_first == 0) f_first = f;
+      if (f > f_first + RISE) far = APART;
       const int all = __all_sync(0xffffffffu, there);
-      if (__any_sync(0xffffffffu, there && ev < f - FAR) || f > f_first + RISE) far = APART;
+      int at = ev;
+      if (__any_sync(0xffffffffu, there && ev < f - FAR) || (j > 0 && f_old == 0 && f > 0)) {
+        // blocks of zeros are not far: these here count with f - FAR, the ones before, if f was 0, by way of M
+        const int o0 = (t0 + j) * NT >> a.c.lg_page, o1 = min(((t0 + j + META) * NT - 1) >> a.c.lg_page, o_hi);
+        for (int o = j > 0 && f_old == 0 ? o_lo : max(o0, o_lo); o <= o1 && !far; ++o) {
+          const int page = ids[o];
+          const int e = (unsigned)page >= (unsigned)a.c.pages ? 255 : a.c.v_exp[page * a.c.exp_stride + kvh];
+          if (e < f - FAR && __any_sync(0xffffffffu, e > 0 || has_value(a, page, kvh, lane, 32))) far = APART;
+        }
+        at = max(ev, f - FAR);
+      }
       if (!wait(&sh.meta_empty[set], (j / META >> 1 & 1) ^ 1u)) break;
       sh.meta[set].g[lane / (NT / 16)][lane % (NT / 16)] =
-          make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(ev - 127),
-                      ev == 255 ? 1.f : pow2_e8m0(min(127 + f - ev, 254)), there ? 1.f : 0.f);
+          make_float4(pow2_e8m0(ek), ev == 255 ? __uint_as_float(0x7fc00000u) : (float)(at - 127),
+                      ev == 255 ? 1.f : pow2_e8m0(min(127 + f - at, 254)), there ? 1.f : 0.f);
       if (lane == 0) {
         sh.meta[set].f = f + far;
         sh.meta[set].all = all;
@@ -471,9 +483,11 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
         mg[g] = fmaxf(m0, m1);
       }
       const float mx = fmaxf(fmaxf(mg[0], mg[1]), fmaxf(mg[2], mg[3]));
-      if (meta.f > f) {  // a larger f scales l
+      // a larger f scales l; from 0, after blocks of zeros, it also moves M (kv8_attention.cu: raise)
+      if (meta.f > f) {
         if (j > 0) {
-          const float w = ex2((float)(meta.f - f));
+          const float by = (float)max(0, meta.f - f - RISE), w = ex2((float)(meta.f - f) - by);
+          if (m > LOWEST) m += by;
           ls[0] = mul2(ls[0], pair(w, w));
           ls[1] = mul2(ls[1], pair(w, w));
         }

@@ -408,6 +408,50 @@ def test_totals_of_ragged_prompts(dt):
         G.check(out[i], ref.cpu().numpy(), mag.cpu().numpy(), size.cpu().numpy(), dt, d, length)
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("new,b,page,length", [(1, 1, 16, 700), (1, 2, 64, 300), (5, 3, 32, 500), (100, 12, 64, 1500), (130, 12, 16, 1100), (100, 24, 64, 1300)])
+@pytest.mark.parametrize("where", ["first", "last", "mixed"])
+@pytest.mark.parametrize("tiny", [False, True])
+def test_blocks_of_exponent_0(dt, new, b, page, length, where, tiny):
+    """All-zero value blocks before, behind and among ordinary ones (a cache that was not filled) count in the softmax;
+    blocks of exponent 0 with codes are values of 2^-127 a code, and rows that see only those get them."""
+    rng = np.random.default_rng(49)
+    width = -(-length // page)
+    pool = G.host_pool(rng, b * width, 2, page, 64, 0.3)
+    table = rng.permutation(b * width).reshape(b, width)
+    o = {"first": range(width - 1), "last": range(1, width), "mixed": range(0, width, 3)}[where]
+    ids = table[:, list(o)].ravel()
+    pool["v_exp"][ids] = 0
+    if not tiny:
+        pool["v"][ids] = 0
+    q = torch.from_numpy(rng.standard_normal((b * new, 4, 64)).astype(np.float32)).to(G.TYPES[dt])
+    for pos, window in ((length - new, 0), (length - new, 40), (0, 0)):
+        out = lb.kv8_attention(q.cuda(), G.device_pool(pool), G.i32(table), G.i32([pos] * b), window=window)
+        check(out, pool, q.double().numpy(), table, [pos] * b, window, dt, 64)
+
+
+@pytest.mark.parametrize("new,b", [(1, 200), (3, 150)])
+def test_zeros_before_values_in_a_long_segment(new, b):
+    """The zeros end after several lookups of a block of the grid; the tokens behind them are the only values."""
+    kv, d, length, page = 8, 32, 8192, 16
+    rng = np.random.default_rng(50)
+    n = length // page
+    pool = G.host_pool(rng, n, kv, page, d)
+    for first in (100, 300, 500):
+        part = {m: a.copy() for m, a in pool.items()}
+        part["v"][:first], part["v_exp"][:first] = 0, 0
+        q = torch.randn((b * new, kv, d), device="cuda")
+        out = lb.kv8_attention(q, G.device_pool(part), G.i32(np.broadcast_to(np.arange(n), (b, n))), G.i32([length - new] * b))
+        k, v = (torch.from_numpy((part[m] * R.pow2(part[m + "_exp"])[..., None, None]).transpose(1, 0, 2, 3).reshape(kv, length, d)).cuda()
+                for m in "kv")
+        at = (length - new + torch.arange(new, device="cuda")).repeat(b)
+        s = torch.einsum("rhd,hld->rhl", q.double(), k) / d ** 0.5
+        size = torch.einsum("rhd,hld->rhl", q.double().abs(), k.abs()).amax(-1) / d ** 0.5
+        p = s.masked_fill((torch.arange(length, device="cuda") > at[:, None])[:, None], -torch.inf).softmax(-1)
+        G.check(out, *(t.cpu().numpy() for t in (torch.einsum("rhl,hld->rhd", p, v), torch.einsum("rhl,hld->rhd", p, v.abs()), size)),
+                "fp32", d, length)
+
+
 @pytest.mark.parametrize("dt", ["fp32", "bf16"])
 @pytest.mark.parametrize("new,b,length", [(1, 1, 20000), (1, 9, 3000), (4, 12, 1500), (100, 12, 1500)])
 @pytest.mark.parametrize("gap", [45, 80, 120])

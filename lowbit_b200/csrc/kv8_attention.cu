@@ -305,9 +305,9 @@ struct Warp {
       }
   }
 
-  // f grew by d: by RISE at most, or from 0 after blocks of zeros, whose M moves so that l stays in range (O is 0)
+  // f grew by d: by RISE at most, or from 0 after blocks of zeros (O is 0), which then count with f - FAR as well
   __device__ __forceinline__ void raise(int d) {
-    const float by = (float)max(0, d - RISE), f = ex2((float)d - by);
+    const float by = (float)max(0, d - FAR), f = ex2((float)d - by);
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll

@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(AttnArgs a) {
       // a larger f scales l; from 0, after blocks of zeros, it also moves M (kv8_attention.cu: raise)
       if (meta.f > f) {
         if (j > 0) {
-          const float by = (float)max(0, meta.f - f - RISE), w = ex2((float)(meta.f - f) - by);
+          const float by = (float)max(0, meta.f - f - FAR), w = ex2((float)(meta.f - f) - by);
           if (m > LOWEST) m += by;
           ls[0] = mul2(ls[0], pair(w, w));
           ls[1] = mul2(ls[1], pair(w, w));

@@ -476,3 +476,27 @@ def test_far_scales_in_one_part_of_a_long_row(dt, new, b, length, gap):
         for pos in ([length - new] * b, [width * 3 // 4 * page - 2] * b):
             out = lb.kv8_attention(q.cuda(), G.device_pool(part), G.i32(table), G.i32(pos))
             check(out, part, q.double().numpy(), table, pos, 0, dt, d)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("new,b,page,length", [(1, 1, 64, 500), (1, 200, 16, 4100), (5, 3, 16, 1100), (100, 24, 64, 1300)])
+@pytest.mark.parametrize("zeros", ["first", "last"])
+def test_weight_on_blocks_of_zeros(dt, new, b, page, length, zeros):
+    """The softmax lies on blocks of zeros, by 2^64: what is left of the values keeps its digits."""
+    rng = np.random.default_rng(52)
+    width, kv, d = -(-length // page), 2 if b < 200 else 8, 64
+    pool = G.host_pool(rng, width, kv, page, d, 0.0)
+    table = np.broadcast_to(rng.permutation(width), (b, width))
+    ids = table[0, :width // 2] if zeros == "first" else table[0, width // 2:]
+    pool["v"][ids], pool["v_exp"][ids] = 0, 0
+    pool["k_exp"][:] -= 4
+    pool["k"][ids], pool["k_exp"][ids] = 64, 122
+    q = torch.from_numpy((2.775 + 0.01 * rng.standard_normal((b * new, 2 * kv, d))).astype(np.float32)).to(G.TYPES[dt])
+    pos = [length - new] * b
+    out = lb.kv8_attention(q.cuda(), G.device_pool(pool), G.i32(table), G.i32(pos))
+    ref, mag, size, _ = attention(pool, q.double().numpy(), table, pos)
+    assert 2.0 ** -70 < mag.max() < 2.0 ** -50
+    if dt == "fp16":
+        assert not out.any()
+    else:
+        G.check(out, ref, mag, size, dt, d, length)

@@ -21,8 +21,8 @@
 // Bound: the row warps' own chain of a step (tensor-memory load, scale, maximum,
 // vote, exponentials, store): 2500-2600 cycles, of which the tensor pipe works
 // 1288 and the exponential unit 1024. Two prompts to 4096 tokens, 32 heads, 8 KV
-// heads of 128, bf16: 216-218 us, 680 TFLOP/s; 2048 fp32 tokens after 2047, 14 heads
-// of 64: 104-105 us. 64 tokens a step and not 128, so that two steps' scores fit
+// heads of 128, bf16: 213-218 us, 680-690 TFLOP/s; 2048 fp32 tokens after 2047, 14
+// heads of 64: 106 us. 64 tokens a step and not 128, so that two steps' scores fit
 // tensor memory beside two row tiles' outputs (128 with one: 293 us); two row
 // tiles share each conversion of the codes.
 #include <algorithm>

@@ -394,7 +394,9 @@ int lbc_kv8_append(const lbc_kv8 *c, int dtype, const void *qkv, long long ld, c
  * Softmax and sums in fp32; a row that sees a NaN block, or whose query is
  * not finite, is NaN. workspace: device scratch of
  * lbc_kv8_attention_workspace(...) bytes (0: may be NULL), 256-byte aligned,
- * used by this call only; its contents need no initialisation. */
+ * used by this call only; its contents need no initialisation. Prompts in 16
+ * bits whose table spans more than 8192 tokens (fp16) or 131072 (bf16) take
+ * N * H * (D + 4) floats of it, other calls some megabytes at most. */
 size_t lbc_kv8_attention_workspace(const lbc_kv8 *c, int dtype, int table_width, int B, int N,
                                    int max_tokens, int H, int window);
 int lbc_kv8_attention(const lbc_kv8 *c, int dtype, const void *q, long long ld, const int32_t *table,

@@ -34,9 +34,9 @@
 // Bounds: long batches HBM (bf16, 32 heads, 8 KV heads of 128: 64 sequences to
 // 8192 tokens 120-131 us from GPU to GPU, 5.0-5.5 TB/s; one of 131071 58 us, 4.6
 // TB/s, the rest is the pipelines' start and the join); short ones the chain of
-// launch, page lookup and units (14 heads, 2 KV heads of 64, fp32: 510 tokens 6.3
+// launch, page lookup and units (14 heads, 2 KV heads of 64, fp32: 510 tokens 6.4
 // us, 16 sequences to 4096 11.4 us); tiles of 24 rows issue and tensor-core latency
-// (16 sequences of 5 tokens, 32 heads, window 1024, fp16: 24 us).
+// (16 sequences of 5 tokens, 32 heads, window 1024, fp16: 24-25.5 us).
 #include <algorithm>
 #include <cstdio>
 
